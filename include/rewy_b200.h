@@ -251,6 +251,112 @@ int rewy_qk_front_bwd(const RewyRowMap* map, const void* yq, const void* yk, con
                       const void* dyq, const void* dyk, int32_t dy_is_f32, void* dq, void* dk, int32_t H, int32_t G,
                       rewy_stream_t stream);
 
+/* Operators around a recurrence (no counterpart in the reference, whose layers take them from FLA): the short causal
+ * convolution in front of it, the selective state space scan beside the delta rules, the norms before and after a block with
+ * its gate and residual scale, and the delta rules' step for single tokens.  Element types: dtype for activations and
+ * convolution states, param_dtype for weights; sums, decays and recurrent states are FP32.  Row strides are in elements; the
+ * last dimension is contiguous; no alignment is asked for (rows that start on 16 bytes are moved in whole accesses).
+ * Packed sequences: cu_seqlens (device int32 [num_seqs + 1]) with B = 1; then states are [num_seqs, ...].  `slots` of a step
+ * (device int32, or int64 with slots_i64; optional): row b works on state slots[b] of a pool of `pool` states.  A row whose
+ * index is outside the pool, or the same as that of a row before it, is skipped: its output is zero and no state changes. */
+enum { REWY_BF16 = 0, REWY_F16 = 1, REWY_F32 = 2 };
+
+/* y_t = act(bias + sum_w weight[:,w] x_(t-W+1+w)), 2 <= W <= 4, activation 0 none, 1 SiLU.  States [.., W-1, D]: the last
+ * inputs of a sequence, the oldest first.  dinitial_state may be NULL; dbias too. */
+typedef struct RewyConvArgs {
+  int32_t dtype, param_dtype, activation, B, T, D, W, num_seqs;
+  int64_t x_batch_stride, x_token_stride;
+  const void *x, *weight, *bias, *initial_state; /* [B,T,D], [D,W], [D], [.,W-1,D] */
+  const int32_t* cu_seqlens;
+  void *y, *final_state;                         /* [B,T,D], [.,W-1,D] or NULL */
+  const void *dy, *dfinal_state;                 /* backward: [B,T,D], [.,W-1,D] or NULL */
+  void *dx, *dweight, *dbias, *dinitial_state;
+  void* workspace;
+  size_t workspace_bytes;
+} RewyConvArgs;
+typedef struct RewyConvStepArgs {
+  int32_t dtype, param_dtype, activation, B, D, W, slots_i64;
+  int64_t x_stride, pool;
+  const void *x, *weight, *bias, *slots; /* [B,D], [D,W], [D] */
+  void *state, *y;                       /* [pool,W-1,D] updated in place, [B,D] */
+} RewyConvStepArgs;
+int rewy_conv_fwd(const RewyConvArgs* args, rewy_stream_t stream);
+int rewy_conv_bwd(const RewyConvArgs* args, rewy_stream_t stream);
+size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D, int32_t W);
+int rewy_conv_step(const RewyConvStepArgs* args, rewy_stream_t stream);
+
+/* dt = softplus(dt_raw + dt_bias) or dt_raw + dt_bias;  h_t = exp(dt_t A) h_(t-1) + dt_t u_t B_t;  y_t = (C_t h_t + D u_t) silu(z_t).
+ * u, dt, z [B,T,M]; Bm, C [B,T,G,N] (channel m reads group m / (M/G)); A [M,N], D, dt_bias [M] FP32 (D, z, dt_bias may be
+ * NULL); states [.,M,N] FP32; 1 <= N <= 64.  Strides are {batch, token} of u, dt, z and {batch, token, group} of Bm and C.
+ * With `checkpoints` (FP32, rewy_scan_checkpoint_bytes) the forward keeps the state before every 16th token for the
+ * backward, which reads it.  dC, dB are [B,T,G,N] and du, ddt, dz [B,T,M] contiguous, in dtype; the others FP32. */
+typedef struct RewyScanArgs {
+  int32_t dtype, B, T, M, N, G, softplus, num_seqs;
+  int64_t u_stride[2], dt_stride[2], z_stride[2], B_stride[3], C_stride[3];
+  const void *u, *dt, *z, *Bm, *C;
+  const float *A, *D, *dt_bias, *initial_state;
+  const int32_t* cu_seqlens;
+  void* y;
+  float *final_state, *checkpoints;
+  const void* dy;
+  const float* dfinal_state;
+  void *du, *ddt, *dz, *dB, *dC;
+  float *dA, *dD, *ddt_bias, *dinitial_state;
+  void* workspace;
+  size_t workspace_bytes;
+} RewyScanArgs;
+typedef struct RewyScanStepArgs {
+  int32_t dtype, B, M, N, G, softplus, slots_i64;
+  int64_t u_stride, dt_stride, z_stride, B_stride[2], C_stride[2], pool;
+  const void *u, *dt, *z, *Bm, *C, *slots; /* [B,M], [B,G,N] */
+  const float *A, *D, *dt_bias;
+  float* state;                            /* [pool,M,N] updated in place */
+  void* y;
+} RewyScanStepArgs;
+size_t rewy_scan_checkpoint_bytes(int32_t B, int32_t T, int32_t M, int32_t N);
+size_t rewy_scan_workspace_bytes(int32_t B, int32_t T, int32_t M, int32_t N, int32_t G, int32_t backward);
+int rewy_scan_fwd(const RewyScanArgs* args, rewy_stream_t stream);
+int rewy_scan_bwd(const RewyScanArgs* args, rewy_stream_t stream);
+int rewy_scan_step(const RewyScanStepArgs* args, rewy_stream_t stream);
+
+/* Rows of D values; row r of an input starts at (r / inner) * stride[0] + (r % inner) * stride[1].  Outputs and gradients are
+ * contiguous.  Gated: y = n(x) weight act(gate), or with gate_first n(x act(gate)) weight; activation 0 SiLU, 1 sigmoid;
+ * n(v) = v / sqrt(mean v^2 + eps).  Residual: residual_out = residual + scale x (residual may be NULL: 0; scale a number, or
+ * with scale_vector one per channel), y = n(residual_out before its rounding) weight.  D <= 16384. */
+typedef struct RewyNormArgs {
+  int32_t dtype, residual_dtype, param_dtype, scale_dtype, activation, gate_first, D;
+  int64_t rows;
+  int64_t x_inner, x_stride[2], other_inner, other_stride[2]; /* other: gate or residual */
+  float eps, scale;
+  const void *x, *gate, *residual, *weight, *scale_vector;
+  void *y, *residual_out;
+  const void *dy, *dresidual_out; /* dresidual_out may be NULL */
+  void *dx, *dgate, *dresidual, *dweight, *dscale;
+  void* workspace;
+  size_t workspace_bytes;
+} RewyNormArgs;
+size_t rewy_norm_bwd_workspace_bytes(int64_t rows, int32_t D);
+int rewy_gated_norm_fwd(const RewyNormArgs* args, rewy_stream_t stream);
+int rewy_gated_norm_bwd(const RewyNormArgs* args, rewy_stream_t stream);
+int rewy_residual_norm_fwd(const RewyNormArgs* args, rewy_stream_t stream);
+int rewy_residual_norm_bwd(const RewyNormArgs* args, rewy_stream_t stream);
+
+/* One token of a delta rule for every row: the recurrence that the four families' chunked operators compute over a sequence.
+ * q, k [B,H,K]; v, w_gate [B,HV,V]; b_gate [B,HV,K]; g [B,HV] (GDN) or [B,HV,K] natural logarithms of the decay, or with A_log
+ * [HV] the raw gate input of KDA (dt_bias [HV*K] or NULL); beta [B,HV]; state [pool,HV,K,V] ([pool,HV,V,K] with
+ * state_v_first) FP32, updated in place; o [B,HV,V].  HV a multiple of H; 1 <= K, V <= 128.  All contiguous.
+ * qk_norm: q and k are L2-normalised; beta_scale: 0 takes beta as it is, else beta_scale * sigmoid(beta). */
+typedef struct RewyDeltaStepArgs {
+  int32_t family, dtype, gate_dtype, beta_dtype, B, H, HV, K, V, state_v_first, qk_norm, slots_i64;
+  float scale, beta_scale;
+  int64_t pool;
+  const void *q, *k, *v, *g, *beta, *b_gate, *w_gate, *slots;
+  const float *A_log, *dt_bias;
+  float* state;
+  void* o;
+} RewyDeltaStepArgs;
+int rewy_delta_step(const RewyDeltaStepArgs* args, rewy_stream_t stream);
+
 /* Optional per-stage device timing of the whole-family calls (no counterpart in the reference, which
  * times stages by re-capturing them: research/operators/a800_ablation/audit.py:38-47).  While enabled, each
  * whole-family call records CUDA events on its stream around its stage launches (up to 256 calls).

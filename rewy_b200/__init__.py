@@ -8,6 +8,10 @@ Public surface (same names and meaning as the reference's, __init__.py:6-40):
     use_backend(backend, strict=True, ops=None)                           context manager
     stats(reset=False), assert_used(ops=None, backward=True)              dispatch report / audit
     chunk_kda, chunk_gated_delta_rule, chunk_gdn2, chunk_delta_rule       the four operators
+and, beside the reference's surface, the operators around them in a layer (``rewy_b200.layers``):
+    causal_conv, selective_scan, gated_rms_norm, residual_rms_norm        for training and prompts
+    causal_conv_step, selective_scan_step, step_kda,                      for single tokens
+    step_gated_delta_rule, step_gdn2, step_delta_rule
 """
 from .runtime import use_backend, stats, assert_used, dispatch_report
 
@@ -55,3 +59,19 @@ def chunk_gdn2(*args, **kwargs):
 def chunk_delta_rule(*args, **kwargs):
     from .runtime import operator
     return operator("delta")(*args, **kwargs)
+
+
+_LAYERS = ("causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "gated_rms_norm", "residual_rms_norm",
+           "step_kda", "step_gated_delta_rule", "step_gdn2", "step_delta_rule")
+
+
+def __getattr__(name):   # the layer operators, on first use: importing the package loads no torch
+    if name in _LAYERS:
+        from . import layers
+        value = globals()[name] = getattr(layers, name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted([*globals(), *_LAYERS])

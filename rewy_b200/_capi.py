@@ -10,7 +10,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "librewy_b200.so"
-TORCH_LIB_PATH = PKG / "rewy_b200_torch.so"   # torch operators over it (csrc/binding.cpp)
+TORCH_LIB_PATH = PKG / "rewy_b200_torch.so"   # torch operators over it (csrc/binding.cpp, csrc/layers.cpp)
 
 DELTA, GDN, KDA, GDN2 = 0, 1, 2, 3
 FAMILY_ID = {"delta": DELTA, "gdn": GDN, "kda": KDA, "gdn2": GDN2}
@@ -27,6 +27,10 @@ EXPORTS = (
     "rewy_l2norm_fwd", "rewy_l2norm_bwd", "rewy_beta_sigmoid_fwd", "rewy_beta_sigmoid_bwd", "rewy_gate_cumsum_fwd",
     "rewy_gate_act_bwd", "rewy_gate_act_bwd_bf16", "rewy_chunk_fwd", "rewy_scalar_gate_cumsum_fwd", "rewy_set_forward_variant",
     "rewy_rows_pad", "rewy_rows_cut", "rewy_qk_front_fwd", "rewy_qk_front_bwd",
+    "rewy_conv_fwd", "rewy_conv_bwd", "rewy_conv_bwd_workspace_bytes", "rewy_conv_step",
+    "rewy_scan_checkpoint_bytes", "rewy_scan_workspace_bytes", "rewy_scan_fwd", "rewy_scan_bwd", "rewy_scan_step",
+    "rewy_norm_bwd_workspace_bytes", "rewy_gated_norm_fwd", "rewy_gated_norm_bwd", "rewy_residual_norm_fwd", "rewy_residual_norm_bwd",
+    "rewy_delta_step",
     "rewy_last_error", "rewy_version", "rewy_kernel_launch_count",
 )
 

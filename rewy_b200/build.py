@@ -13,7 +13,9 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "csrc" / "build"
 LIB = PKG / "librewy_b200.so"
 TORCH_LIB = PKG / "rewy_b200_torch.so"
-SOURCES = ("capi.cu", "prepare.cu", "prepare_tc.cu", "state_scan.cu", "state_scan_tc.cu", "state_scan_split.cu", "chunk_adjoint.cu", "chunk_adjoint_tc.cu", "tc_selftest.cu", "wrappers.cu", "rows.cu", "chunk_fwd.cu", "chunk_fwd_tc.cu", "chunk_output_tc.cu")
+SOURCES = ("capi.cu", "prepare.cu", "prepare_tc.cu", "state_scan.cu", "state_scan_tc.cu", "state_scan_split.cu", "chunk_adjoint.cu", "chunk_adjoint_tc.cu", "tc_selftest.cu", "wrappers.cu", "rows.cu", "chunk_fwd.cu", "chunk_fwd_tc.cu", "chunk_output_tc.cu",
+           "conv.cu", "selective_scan.cu", "norms.cu", "delta_step.cu")
+TORCH_SOURCES = ("binding.cpp", "layers.cpp")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--expt-relaxed-constexpr", "--expt-extended-lambda", "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -36,23 +38,33 @@ def _digest(paths):
 
 
 def _build_torch_library():
-    """csrc/binding.cpp against the headers of the installed torch, linked to librewy_b200.so beside it."""
+    """TORCH_SOURCES against the headers of the installed torch, linked to librewy_b200.so beside it."""
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", str(CSRC / "binding.cpp"), "-o", str(TORCH_LIB),
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-isystem{p}" for p in (root / "include", root / "include/torch/csrc/api/include", cuda / "include")),
-           f"-L{root / 'lib'}", f"-L{PKG}", "-l:librewy_b200.so", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
-           "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"the torch operator library did not build:\n{r.stderr[-6000:]}")
+    gxx = shutil.which("g++") or "g++"
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"the torch operator library did not build:\n{r.stderr[-6000:]}")
+
+    def compile_one(src):
+        obj = OBJ / (src[:-4] + ".torch.o")
+        run([gxx, "-O2", "-std=c++17", "-fPIC", "-c", str(CSRC / src), "-o", str(obj),
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *(f"-isystem{p}" for p in (root / "include", root / "include/torch/csrc/api/include", cuda / "include"))])
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=len(TORCH_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, TORCH_SOURCES))
+    run([gxx, "-shared", *objs, "-o", str(TORCH_LIB), f"-L{root / 'lib'}", f"-L{PKG}", "-l:librewy_b200.so", "-ltorch", "-ltorch_cpu",
+         "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
 
 
 def build(force=False, verbose=False):
     """Compile every .cu under csrc/ for sm_100a and link the shared library.  Returns its path."""
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + [CSRC / "binding.cpp"] + [PKG.parent / "include" / "rewy_b200.h"]
+    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.cpp")) + [PKG.parent / "include" / "rewy_b200.h"]
     stamp = OBJ / "stamp.txt"
     digest = _digest(deps)
     if not force and LIB.exists() and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == digest:

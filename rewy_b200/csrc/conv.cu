@@ -1,0 +1,391 @@
+// Short causal convolution per channel in front of a recurrence, with its activation, its state between calls and its gradients.
+//
+//   y_t = act(bias + sum_w weight[w] x_(t-W+1+w))       x before a sequence: its initial state (W-1 rows, the oldest first) or 0
+//   g_t = dy_t act'(pre_t),  dx_t = sum_w weight[w] g_(t+W-1-w),  dweight[w] = sum_t g_t x_(t-W+1+w),  dbias = sum_t g_t
+//
+// Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx; a multiply-add per tap and two special
+// functions per element hide behind that.  A warp owns neighbouring channels (16 bytes per lane forward, 8 backward) and
+// a block of tokens, and slides the W-1 last inputs (backward: and the W-1 last g) through registers, so that an element is
+// loaded once but for the W-1 rows between blocks of tokens, which come from the caches.  The pre-activation is computed
+// again in the backward rather than kept (a multiply-add per tap against a read of n elements).  All sums are FP32; an output
+// is rounded once.  dweight and dbias: FP32 sums in registers over the warp's tokens, over the CTA's warps in shared memory, and
+// over the CTAs in a second kernel, always in the same order.
+#include "layer.cuh"
+
+namespace rewy {
+namespace {
+
+constexpr int WARPS = 8;
+
+struct ConvParams {
+  RewyConvArgs a;
+  int token_block, token_blocks, channel_blocks;  // tokens per warp; CTAs per sequence row; CTAs per token
+  bool wide;                                      // every row of x starts on a whole access
+};
+
+struct Span {  // the sequence a token lies in
+  int s, begin, end;
+};
+__device__ __forceinline__ Span span_at(const RewyConvArgs& a, int b, int t) {
+  if (a.cu_seqlens == nullptr) return {b, 0, a.T};
+  const int s = packed_sequence(a.cu_seqlens, a.num_seqs, t);
+  return {s, min(max(a.cu_seqlens[s], 0), t), s + 1 < a.num_seqs ? min(max(a.cu_seqlens[s + 1], t + 1), a.T) : a.T};
+}
+__device__ __forceinline__ Span span_after(const RewyConvArgs& a, const Span& p) {  // p is not the last one
+  const int s = p.s + 1;
+  return {s, p.end, s + 1 < a.num_seqs ? min(max(a.cu_seqlens[s + 1], p.end + 1), a.T) : a.T};
+}
+
+template <class T, int W, int V>
+struct Columns {  // a warp's channels
+  const RewyConvArgs& a;
+  const T* x;
+  long long state_row;  // elements of one sequence's state
+  int c0, valid;
+  bool wide;
+  float weight[W][V], bias[V];
+
+  __device__ __forceinline__ Columns(const ConvParams& p, int b, int channel)
+      : a(p.a), x(static_cast<const T*>(p.a.x) + b * p.a.x_batch_stride), state_row((long long)(W - 1) * p.a.D), c0(channel),
+        valid(p.a.D - channel), wide(p.wide) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+#pragma unroll
+      for (int w = 0; w < W; w++) weight[w][i] = i < valid ? param_at(a.weight, a.param_dtype, (long long)(c0 + i) * W + w) : 0.f;
+      bias[i] = a.bias != nullptr && i < valid ? param_at(a.bias, a.param_dtype, c0 + i) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void load_x(Pack<T, V>& d, int t) const { load_some<T, V>(d, x + t * a.x_token_stride + c0, valid, wide); }
+  __device__ __forceinline__ long long at(int row, long long rows_before) const { return (rows_before + row) * a.D + c0; }
+  // the W-1 inputs before token t of sequence s
+  __device__ __forceinline__ void window(float (&win)[W - 1][V], const Span& s, int t) const {
+#pragma unroll
+    for (int j = 0; j < W - 1; j++) {
+      const int pos = t - (W - 1) + j;
+      Pack<T, V> v;
+      if (pos >= s.begin) load_x(v, pos);
+      else if (a.initial_state != nullptr)
+        load_some<T, V>(v, static_cast<const T*>(a.initial_state) + s.s * state_row + (long long)(W - 1 + pos - s.begin) * a.D + c0, valid, wide);
+      else zero_pack(v);
+#pragma unroll
+      for (int i = 0; i < V; i++) win[j][i] = to_f32(v.v[i]);
+    }
+  }
+};
+
+template <class T, int W, int V>
+__global__ void __launch_bounds__(WARPS * 32) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
+  constexpr int U = 8;
+  const int channel = (blockIdx.x % p.channel_blocks * 32 + (threadIdx.x & 31)) * V;
+  const unsigned rest = blockIdx.x / p.channel_blocks;
+  const int b = rest / p.token_blocks;
+  const long long first = ((long long)(rest % p.token_blocks) * WARPS + (threadIdx.x >> 5)) * p.token_block;
+  if (channel >= p.a.D || first >= p.a.T) return;
+  const int t0 = (int)first, t1 = (int)min(first + p.token_block, (long long)p.a.T);
+  const Columns<T, W, V> c(p, b, channel);
+  T* y = static_cast<T*>(p.a.y) + (long long)b * p.a.T * p.a.D + channel;
+  Span s = span_at(p.a, b, t0);
+  float win[W - 1][V];
+  c.window(win, s, t0);
+  for (int t = t0; t < t1; t += U) {
+    Pack<T, V> in[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (t + u < t1) c.load_x(in[u], t + u);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (t + u >= t1) break;
+      if (t + u == s.end) {
+        s = span_after(p.a, s);
+        c.window(win, s, t + u);
+      }
+      Pack<T, V> out;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float now = to_f32(in[u].v[i]);
+        float pre = fmaf(c.weight[W - 1][i], now, c.bias[i]);
+#pragma unroll
+        for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
+        out.v[i] = from_f32<T>(p.a.activation ? pre * sigmoid_fast(pre) : pre);
+#pragma unroll
+        for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
+        win[W - 2][i] = now;
+      }
+      store_some<T, V>(y + (long long)(t + u) * p.a.D, out, c.valid, c.wide);
+      if (p.a.final_state != nullptr && t + u == s.end - 1) {
+#pragma unroll
+        for (int j = 0; j < W - 1; j++) {
+          Pack<T, V> v;
+#pragma unroll
+          for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(win[j][i]);
+          store_some<T, V>(static_cast<T*>(p.a.final_state) + s.s * c.state_row + (long long)j * p.a.D + channel, v, c.valid, c.wide);
+        }
+      }
+    }
+  }
+}
+
+template <class T, int W, int V>
+__global__ void __launch_bounds__(WARPS * 32) conv_bwd_kernel(const __grid_constant__ ConvParams p, float* __restrict__ partial) {
+  constexpr int U = 4;
+  __shared__ float sums[WARPS][W + 1][32 * V];
+  const RewyConvArgs& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int channel = (blockIdx.x % p.channel_blocks * 32 + lane) * V;
+  const unsigned rest = blockIdx.x / p.channel_blocks;
+  const int b = rest / p.token_blocks;
+  const long long first = ((long long)(rest % p.token_blocks) * WARPS + warp) * p.token_block;
+  float dw[W][V] = {}, db[V] = {};
+  if (channel < a.D && first < a.T) {
+    const int t0 = (int)first, t1 = (int)min(first + p.token_block, (long long)a.T);
+    const Columns<T, W, V> c(p, b, channel);
+    const long long row = (long long)b * a.T;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.D + channel;
+    T* dx = static_cast<T*>(a.dx) + row * a.D + channel;
+    Span s = span_at(a, b, t0);
+    for (int from = t0; from < t1;) {        // the part of one sequence that lies in the block
+      const int to = min(t1, s.end);
+      float win[W - 1][V], g[W - 1][V] = {};
+      c.window(win, s, from);
+      const int stop = to + W - 1, real = min(stop, s.end);   // beyond the sequence there is no g
+      for (int t = from; t < stop; t += U) {
+        Pack<T, V> in[U], d[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (t + u < real) {
+            c.load_x(in[u], t + u);
+            load_some<T, V>(d[u], dy + (long long)(t + u) * a.D, c.valid, c.wide);
+          }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const int now = t + u;
+          if (now >= stop) break;
+          float fresh[V], out[V];
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            fresh[i] = 0.f;
+            if (now < real) {
+              const float x = to_f32(in[u].v[i]);
+              float gi = to_f32(d[u].v[i]);
+              if (a.activation) {
+                float pre = fmaf(c.weight[W - 1][i], x, c.bias[i]);
+#pragma unroll
+                for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
+                const float sig = sigmoid_fast(pre);
+                gi *= sig * fmaf(pre, 1.f - sig, 1.f);
+              }
+              if (now < to) {
+#pragma unroll
+                for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi, win[w][i], dw[w][i]);
+                dw[W - 1][i] = fmaf(gi, x, dw[W - 1][i]);
+                db[i] += gi;
+              }
+#pragma unroll
+              for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
+              win[W - 2][i] = x;
+              fresh[i] = gi;
+            }
+            out[i] = c.weight[0][i] * fresh[i];
+#pragma unroll
+            for (int w = 1; w < W; w++) out[i] = fmaf(c.weight[w][i], g[W - 1 - w][i], out[i]);
+#pragma unroll
+            for (int j = 0; j < W - 2; j++) g[j][i] = g[j + 1][i];
+            g[W - 2][i] = fresh[i];
+          }
+          const int pos = now - (W - 1);       // its gradient is complete
+          const bool before = pos < from;      // a row of the initial state, or a token of the block before
+          if (before && from != s.begin) continue;
+          if (before && a.dinitial_state == nullptr) continue;
+          if (a.dfinal_state != nullptr && pos >= s.end - (W - 1)) {
+            Pack<T, V> v;
+            load_some<T, V>(v, static_cast<const T*>(a.dfinal_state) + s.s * c.state_row + (long long)(pos - (s.end - (W - 1))) * a.D + channel,
+                            c.valid, c.wide);
+#pragma unroll
+            for (int i = 0; i < V; i++) out[i] += to_f32(v.v[i]);
+          }
+          Pack<T, V> v;
+#pragma unroll
+          for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
+          T* to_row = before ? static_cast<T*>(a.dinitial_state) + s.s * c.state_row + (long long)(W - 1 + pos - s.begin) * a.D + channel
+                             : dx + (long long)pos * a.D;
+          store_some<T, V>(to_row, v, c.valid, c.wide);
+        }
+      }
+      from = to;
+      if (from < t1) s = span_after(a, s);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+#pragma unroll
+    for (int w = 0; w < W; w++) sums[warp][w][lane * V + i] = dw[w][i];
+    sums[warp][W][lane * V + i] = db[i];
+  }
+  __syncthreads();
+  const int c0 = blockIdx.x % p.channel_blocks * 32 * V;
+  for (int i = threadIdx.x; i < (W + 1) * 32 * V; i += blockDim.x) {
+    const int w = i / (32 * V), col = i % (32 * V);
+    if (c0 + col >= a.D) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; k++) sum += sums[k][w][col];
+    partial[((long long)rest * (W + 1) + w) * a.D + c0 + col] = sum;
+  }
+}
+
+// dweight [D,W] and dbias [D] from the CTAs' sums [parts][W+1][D]
+__global__ void __launch_bounds__(256) conv_sums_kernel(const float* __restrict__ partial, int parts, int D, int W, void* dweight, void* dbias,
+                                                        int param_dtype) {
+  const long long n = (long long)(W + 1) * D, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < parts; k++) sum += partial[k * n + i];
+  const int w = (int)(i / D), c = (int)(i % D);
+  if (w < W) param_store(dweight, param_dtype, (long long)c * W + w, sum);
+  else if (dbias != nullptr) param_store(dbias, param_dtype, c, sum);
+}
+
+// One token per row, the state of its slot shifted by it.
+template <class T, int V>
+__global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ RewyConvStepArgs a, int channel_blocks, bool wide) {
+  const int b = blockIdx.x / channel_blocks, c0 = (blockIdx.x % channel_blocks * 128 + threadIdx.x) * V;
+  const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
+  if (c0 >= a.D) return;
+  const int valid = a.D - c0, W = a.W;
+  T* y = static_cast<T*>(a.y) + (long long)b * a.D + c0;
+  Pack<T, V> now;
+  if (slot < 0) {
+    zero_pack(now);
+    store_some<T, V>(y, now, valid, wide);
+    return;
+  }
+  T* state = static_cast<T*>(a.state) + slot * (W - 1) * a.D + c0;
+  load_some<T, V>(now, static_cast<const T*>(a.x) + b * a.x_stride + c0, valid, wide);
+  Pack<T, V> old[3];
+#pragma unroll
+  for (int j = 0; j < 3; j++)
+    if (j < W - 1) {   // (written in this kernel: not through the read-only path)
+      if (wide && valid >= V) old[j] = *reinterpret_cast<const Pack<T, V>*>(state + (long long)j * a.D);
+      else
+        for (int i = 0; i < V; i++) old[j].v[i] = i < valid ? state[(long long)j * a.D + i] : from_f32<T>(0.f);
+    }
+  Pack<T, V> out;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    if (i >= valid) continue;
+    const long long row = (long long)(c0 + i) * W;
+    float pre = fmaf(param_at(a.weight, a.param_dtype, row + W - 1), to_f32(now.v[i]), a.bias != nullptr ? param_at(a.bias, a.param_dtype, c0 + i) : 0.f);
+#pragma unroll
+    for (int j = 0; j < 3; j++)
+      if (j < W - 1) pre = fmaf(param_at(a.weight, a.param_dtype, row + j), to_f32(old[j].v[i]), pre);
+    out.v[i] = from_f32<T>(a.activation ? pre * sigmoid_fast(pre) : pre);
+  }
+  store_some<T, V>(y, out, valid, wide);
+#pragma unroll
+  for (int j = 0; j < 3; j++)
+    if (j < W - 1) store_some<T, V>(state + (long long)j * a.D, j + 1 < W - 1 ? old[j + 1 < 3 ? j + 1 : 2] : now, valid, wide);
+}
+
+int check_conv(const RewyConvArgs* a) {
+  LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
+  LAYER_REQUIRE(known_dtype(a->dtype) && known_dtype(a->param_dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
+  LAYER_REQUIRE(a->W >= 2 && a->W <= 4, REWY_ERR_UNSUPPORTED, "the convolution takes 2 to 4 taps");
+  LAYER_REQUIRE(a->B > 0 && a->T > 0 && a->D > 0, REWY_ERR_SHAPE, "B, T and D must be positive");
+  LAYER_REQUIRE((long long)a->B * a->T <= (1LL << 30) && a->D <= (1 << 24), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or D 2^24 channels");
+  LAYER_REQUIRE(((long long)a->B * a->T / 64 + a->B) * (a->D / 128 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more tokens and channels than one grid holds");
+  LAYER_REQUIRE(a->x != nullptr && a->weight != nullptr, REWY_ERR_NULL, "x or weight is NULL");
+  LAYER_REQUIRE(a->cu_seqlens == nullptr || (a->B == 1 && a->num_seqs > 0), REWY_ERR_SHAPE, "packed sequences need B = 1 and num_seqs > 0");
+  return REWY_OK;
+}
+
+// Tokens per warp.  Long blocks load fewer rows twice (W-1 per block) and leave fewer sums; short ones give a small problem
+// enough warps: B=1 T=2000 D=1024 has 4 warps of channels, blocks of 8 make 1000 warps of them.
+int token_block(long long tokens, int warps_per_token) {
+  int block = 32;
+  while (block > 8 && tokens / block * warps_per_token < 148 * 24) block /= 2;
+  return block;
+}
+
+ConvParams conv_params(const RewyConvArgs& a, int V, bool rows_wide) {
+  ConvParams p;
+  p.a = a;
+  const int e = element_bytes(a.dtype), access = V * e;
+  p.channel_blocks = (a.D + 32 * V - 1) / (32 * V);
+  p.token_block = token_block((long long)a.B * a.T, p.channel_blocks);
+  p.token_blocks = (a.T + p.token_block * WARPS - 1) / (p.token_block * WARPS);
+  auto row = [&](const void* q) { return (reinterpret_cast<uintptr_t>(q) % access) == 0; };
+  p.wide = rows_wide && a.D % V == 0 && a.x_token_stride % V == 0 && a.x_batch_stride % V == 0 && row(a.x) && row(a.y) && row(a.dy) && row(a.dx) &&
+           row(a.initial_state) && row(a.final_state) && row(a.dfinal_state) && row(a.dinitial_state);
+  return p;
+}
+template <class F>
+void with_taps(int W, F&& f) {
+  if (W == 2) f(std::integral_constant<int, 2>());
+  else if (W == 3) f(std::integral_constant<int, 3>());
+  else f(std::integral_constant<int, 4>());
+}
+
+}  // namespace
+}  // namespace rewy
+
+using namespace rewy;
+
+extern "C" int rewy_conv_fwd(const RewyConvArgs* a, rewy_stream_t st) {
+  if (const int rc = check_conv(a)) return rc;
+  LAYER_REQUIRE(a->y != nullptr, REWY_ERR_NULL, "y is NULL");
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    const ConvParams p = conv_params(*a, V, true);
+    const unsigned grid = (unsigned)((long long)p.channel_blocks * p.token_blocks * a->B);
+    with_taps(a->W, [&](auto w) { conv_fwd_kernel<T, w.value, V><<<grid, WARPS * 32, 0, (cudaStream_t)st>>>(p); });
+  });
+  return launched("causal convolution forward");
+}
+
+extern "C" size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D, int32_t W) {
+  if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4) return 0;
+  RewyConvArgs a{};
+  a.B = B; a.T = T; a.D = D; a.W = W;
+  const ConvParams p = conv_params(a, 4, true);
+  return (size_t)p.token_blocks * B * (W + 1) * D * sizeof(float);
+}
+
+extern "C" int rewy_conv_bwd(const RewyConvArgs* a, rewy_stream_t st) {
+  if (const int rc = check_conv(a)) return rc;
+  LAYER_REQUIRE(a->dy != nullptr && a->dx != nullptr && a->dweight != nullptr, REWY_ERR_NULL, "dy, dx or dweight is NULL");
+  LAYER_REQUIRE(a->workspace != nullptr && a->workspace_bytes >= rewy_conv_bwd_workspace_bytes(a->B, a->T, a->D, a->W), REWY_ERR_WORKSPACE,
+                "the workspace of the convolution backward is too small");
+  constexpr int V = 4;
+  const ConvParams p = conv_params(*a, V, true);
+  const int parts = p.token_blocks * a->B;
+  float* partial = static_cast<float*>(a->workspace);
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    const unsigned grid = (unsigned)((long long)p.channel_blocks * parts);
+    with_taps(a->W, [&](auto w) { conv_bwd_kernel<T, w.value, V><<<grid, WARPS * 32, 0, (cudaStream_t)st>>>(p, partial); });
+  });
+  conv_sums_kernel<<<(unsigned)(((long long)(a->W + 1) * a->D + 255) / 256), 256, 0, (cudaStream_t)st>>>(partial, parts, a->D, a->W, a->dweight, a->dbias,
+                                                                                                         a->param_dtype);
+  return launched("causal convolution backward", 2);
+}
+
+extern "C" int rewy_conv_step(const RewyConvStepArgs* a, rewy_stream_t st) {
+  LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
+  LAYER_REQUIRE(known_dtype(a->dtype) && known_dtype(a->param_dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
+  LAYER_REQUIRE(a->W >= 2 && a->W <= 4, REWY_ERR_UNSUPPORTED, "the convolution takes 2 to 4 taps");
+  LAYER_REQUIRE(a->B > 0 && a->D > 0 && a->pool > 0, REWY_ERR_SHAPE, "B, D and the pool must be positive");
+  LAYER_REQUIRE(a->D <= (1 << 24) && (long long)a->B * (a->D / 256 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more rows and channels than one grid holds");
+  LAYER_REQUIRE(a->slots != nullptr || a->pool >= a->B, REWY_ERR_SHAPE, "fewer states than rows");
+  LAYER_REQUIRE(a->x != nullptr && a->weight != nullptr && a->state != nullptr && a->y != nullptr, REWY_ERR_NULL, "x, weight, state or y is NULL");
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 8 / sizeof(T);
+    const int access = V * (int)sizeof(T), channel_blocks = (a->D + 128 * V - 1) / (128 * V);
+    auto row = [&](const void* q) { return (reinterpret_cast<uintptr_t>(q) % access) == 0; };
+    const bool wide = a->D % V == 0 && a->x_stride % V == 0 && row(a->x) && row(a->y) && row(a->state);
+    conv_step_kernel<T, V><<<(unsigned)((long long)channel_blocks * a->B), 128, 0, (cudaStream_t)st>>>(*a, channel_blocks, wide);
+  });
+  return launched("causal convolution step");
+}

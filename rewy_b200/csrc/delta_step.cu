@@ -1,0 +1,185 @@
+// One token of a delta rule for every row of a decoding batch, the state of its slot updated in place:
+//
+//   S <- diag(exp g) S;  r = beta (v - k^T S)  (GDN2: w v - (b k)^T S);  S <- S + k r^T;  o = scale q^T S
+//
+// Bound by HBM: the FP32 state of a (row, value head) is 64 KB, read and written once; everything else is a few hundred
+// bytes.  A CTA takes 32 value channels of one state (16 KB, eight 16-byte loads per thread in flight before anything is
+// waited for), so that even one sequence with few heads fills the SMs.  The state stays in registers between load and store.
+// Both products over the key channels come from one exchange: q^T (S + k r^T) = q^T S + (q k) r.  q, k and the gates are
+// read, normalised and activated by every CTA for itself.  All arithmetic is FP32.
+#include "layer.cuh"
+
+namespace rewy {
+namespace {
+
+constexpr int NT = 128, SLICE = 32, ROWS = 8;  // threads, value channels per CTA, state vectors per thread
+
+__device__ __forceinline__ float4 load_state(const float* p, int valid, bool wide) {
+  if (wide && valid >= 4) return *reinterpret_cast<const float4*>(p);
+  return make_float4(valid > 0 ? p[0] : 0.f, valid > 1 ? p[1] : 0.f, valid > 2 ? p[2] : 0.f, valid > 3 ? p[3] : 0.f);
+}
+__device__ __forceinline__ void store_state(float* p, float4 x, int valid, bool wide) {
+  if (wide && valid >= 4) {
+    *reinterpret_cast<float4*>(p) = x;
+    return;
+  }
+  if (valid > 0) p[0] = x.x;
+  if (valid > 1) p[1] = x.y;
+  if (valid > 2) p[2] = x.z;
+  if (valid > 3) p[3] = x.w;
+}
+
+template <class T, bool V_FIRST>
+__global__ void __launch_bounds__(NT) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices, bool wide) {
+  __shared__ float sk[NT], sq[NT], serase[NT], sdecay[NT], red[4][3], part[4][2][SLICE];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slice = blockIdx.x % slices;
+  const unsigned rest = blockIdx.x / slices;
+  const int hv = rest % a.HV, b = rest / a.HV, v0 = slice * SLICE;
+  const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool), head = (long long)b * a.HV + hv;
+  T* o = static_cast<T*>(a.o) + head * a.V;
+  if (slot < 0) {
+    if (tid < SLICE && v0 + tid < a.V) o[v0 + tid] = from_f32<T>(0.f);
+    return;
+  }
+  float* state = a.state + (slot * a.HV + hv) * ((long long)a.K * a.V);
+  // this thread's state vectors: [K,V] four value channels of key rows kr + 16 i; [V,K] four key channels of value rows vr + 4 i
+  const int c4 = V_FIRST ? lane * 4 : (tid & 7) * 4, r0 = V_FIRST ? warp : tid >> 3;
+  float4 S[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    const int r = V_FIRST ? v0 + r0 + 4 * i : r0 + 16 * i, c = V_FIRST ? c4 : v0 + c4;
+    const int rows = V_FIRST ? a.V : a.K, cols = V_FIRST ? a.K : a.V;
+    S[i] = load_state(state + (long long)r * cols + c, r < rows ? cols - c : 0, wide);
+  }
+  const long long qk = ((long long)b * a.H + hv / (a.HV / a.H)) * a.K;
+  float q = 0.f, k = 0.f, erase = 1.f, decay = 1.f;
+  if (tid < a.K) {
+    q = to_f32(static_cast<const T*>(a.q)[qk + tid]);
+    k = to_f32(static_cast<const T*>(a.k)[qk + tid]);
+    if (a.family == REWY_GDN2) erase = to_f32(static_cast<const T*>(a.b_gate)[head * a.K + tid]);
+    if (a.family == REWY_GDN) {
+      decay = ex2(LOG2E * param_at(a.g, a.gate_dtype, head));
+    } else if (a.family != REWY_DELTA) {
+      float g = param_at(a.g, a.gate_dtype, head * a.K + tid);
+      if (a.A_log != nullptr) {
+        float sig;
+        g = -ex2(LOG2E * a.A_log[hv]) * softplus_fast(g + (a.dt_bias != nullptr ? a.dt_bias[(long long)hv * a.K + tid] : 0.f), sig);
+      }
+      decay = ex2(LOG2E * g);
+    }
+  }
+  float qq = q * q, kk = k * k, dot = q * k;
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    qq += __shfl_xor_sync(0xffffffffu, qq, m);
+    kk += __shfl_xor_sync(0xffffffffu, kk, m);
+    dot += __shfl_xor_sync(0xffffffffu, dot, m);
+  }
+  if (lane == 0) { red[warp][0] = qq; red[warp][1] = kk; red[warp][2] = dot; }
+  __syncthreads();
+  qq = red[0][0] + red[1][0] + red[2][0] + red[3][0];
+  kk = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+  dot = red[0][2] + red[1][2] + red[2][2] + red[3][2];
+  const float qn = a.qk_norm ? rsqrtf(qq + 1e-6f) : 1.f, kn = a.qk_norm ? rsqrtf(kk + 1e-6f) : 1.f;
+  dot *= qn * kn;
+  sq[tid] = q * qn;
+  sk[tid] = k * kn;
+  serase[tid] = k * kn * erase;
+  sdecay[tid] = decay;
+  __syncthreads();
+  float beta = 1.f;
+  if (a.family != REWY_GDN2) {
+    beta = param_at(a.beta, a.beta_dtype, head);
+    if (a.beta_scale != 0.f) beta = a.beta_scale * sigmoid_fast(beta);
+  }
+  auto target = [&](int v) {   // what the state should give for k, before the erase part is taken off
+    const float x = v < a.V ? to_f32(static_cast<const T*>(a.v)[head * a.V + v]) : 0.f;
+    return a.family == REWY_GDN2 && v < a.V ? x * to_f32(static_cast<const T*>(a.w_gate)[head * a.V + v]) : x;
+  };
+
+  if constexpr (!V_FIRST) {
+    float e[4] = {}, p[4] = {};
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      const int r = r0 + 16 * i;
+      const float d = sdecay[r], x = serase[r], y = sq[r];
+      S[i].x *= d; S[i].y *= d; S[i].z *= d; S[i].w *= d;
+      e[0] = fmaf(x, S[i].x, e[0]); e[1] = fmaf(x, S[i].y, e[1]); e[2] = fmaf(x, S[i].z, e[2]); e[3] = fmaf(x, S[i].w, e[3]);
+      p[0] = fmaf(y, S[i].x, p[0]); p[1] = fmaf(y, S[i].y, p[1]); p[2] = fmaf(y, S[i].z, p[2]); p[3] = fmaf(y, S[i].w, p[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+      for (int m = 16; m >= 8; m >>= 1) {
+        e[i] += __shfl_xor_sync(0xffffffffu, e[i], m);
+        p[i] += __shfl_xor_sync(0xffffffffu, p[i], m);
+      }
+      if (lane < 8) { part[warp][0][c4 + i] = e[i]; part[warp][1][c4 + i] = p[i]; }
+    }
+    __syncthreads();
+    float r4[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int c = c4 + i;
+      const float erased = (part[0][0][c] + part[1][0][c]) + (part[2][0][c] + part[3][0][c]);
+      const float seen = (part[0][1][c] + part[1][1][c]) + (part[2][1][c] + part[3][1][c]);
+      r4[i] = beta * (target(v0 + c) - erased);
+      if (tid < 8 && v0 + c < a.V) o[v0 + c] = from_f32<T>(a.scale * fmaf(dot, r4[i], seen));
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      const int r = r0 + 16 * i;
+      const float x = sk[r];
+      S[i].x = fmaf(x, r4[0], S[i].x); S[i].y = fmaf(x, r4[1], S[i].y); S[i].z = fmaf(x, r4[2], S[i].z); S[i].w = fmaf(x, r4[3], S[i].w);
+      store_state(state + (long long)r * a.V + v0 + c4, S[i], r < a.K ? a.V - v0 - c4 : 0, wide);
+    }
+  } else {
+    const float4 d = *reinterpret_cast<const float4*>(sdecay + c4), x = *reinterpret_cast<const float4*>(serase + c4),
+                 y = *reinterpret_cast<const float4*>(sq + c4), kx = *reinterpret_cast<const float4*>(sk + c4);
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      const int v = v0 + r0 + 4 * i;
+      S[i].x *= d.x; S[i].y *= d.y; S[i].z *= d.z; S[i].w *= d.w;
+      float e = fmaf(x.x, S[i].x, x.y * S[i].y) + fmaf(x.z, S[i].z, x.w * S[i].w);
+      float p = fmaf(y.x, S[i].x, y.y * S[i].y) + fmaf(y.z, S[i].z, y.w * S[i].w);
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) {
+        e += __shfl_xor_sync(0xffffffffu, e, m);
+        p += __shfl_xor_sync(0xffffffffu, p, m);
+      }
+      const float r = beta * (target(v) - e);
+      if (lane == 0 && v < a.V) o[v] = from_f32<T>(a.scale * fmaf(dot, r, p));
+      S[i].x = fmaf(kx.x, r, S[i].x); S[i].y = fmaf(kx.y, r, S[i].y); S[i].z = fmaf(kx.z, r, S[i].z); S[i].w = fmaf(kx.w, r, S[i].w);
+      store_state(state + (long long)v * a.K + c4, S[i], v < a.V ? a.K - c4 : 0, wide);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace rewy
+
+using namespace rewy;
+
+extern "C" int rewy_delta_step(const RewyDeltaStepArgs* a, rewy_stream_t st) {
+  LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
+  LAYER_REQUIRE(a->family >= REWY_DELTA && a->family <= REWY_GDN2, REWY_ERR_UNSUPPORTED, "unknown family");
+  LAYER_REQUIRE(known_dtype(a->dtype) && known_dtype(a->gate_dtype) && known_dtype(a->beta_dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
+  LAYER_REQUIRE(a->B > 0 && a->H > 0 && a->HV > 0 && a->pool > 0 && a->HV % a->H == 0, REWY_ERR_SHAPE, "bad B, H, HV or pool");
+  LAYER_REQUIRE(a->K >= 1 && a->K <= 128 && a->V >= 1 && a->V <= 128, REWY_ERR_UNSUPPORTED, "the step takes head dimensions of 1 to 128");
+  LAYER_REQUIRE(a->slots != nullptr || a->pool >= a->B, REWY_ERR_SHAPE, "fewer states than rows");
+  const int slices = (a->V + SLICE - 1) / SLICE;
+  LAYER_REQUIRE((long long)a->B * a->HV * slices < (1LL << 31), REWY_ERR_SHAPE, "more rows and heads than one grid holds");
+  LAYER_REQUIRE(a->q != nullptr && a->k != nullptr && a->v != nullptr && a->state != nullptr && a->o != nullptr, REWY_ERR_NULL, "q, k, v, state or o is NULL");
+  LAYER_REQUIRE(a->family == REWY_DELTA || a->g != nullptr, REWY_ERR_NULL, "g is NULL");
+  LAYER_REQUIRE(a->family == REWY_GDN2 ? a->b_gate != nullptr && a->w_gate != nullptr : a->beta != nullptr, REWY_ERR_NULL, "beta, or b_gate and w_gate, are NULL");
+  LAYER_REQUIRE(a->A_log == nullptr || a->family == REWY_KDA, REWY_ERR_UNSUPPORTED, "the fused gate belongs to KDA");
+  const bool wide = (a->state_v_first ? a->K : a->V) % 4 == 0 && !unaligned16(a->state);
+  const unsigned grid = (unsigned)((long long)a->B * a->HV * slices);
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (a->state_v_first) delta_step_kernel<T, true><<<grid, NT, 0, (cudaStream_t)st>>>(*a, slices, wide);
+    else delta_step_kernel<T, false><<<grid, NT, 0, (cudaStream_t)st>>>(*a, slices, wide);
+  });
+  return launched("delta-rule step");
+}

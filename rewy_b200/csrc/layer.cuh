@@ -1,0 +1,171 @@
+// What the kernels around a recurrence share (conv.cu, selective_scan.cu, norms.cu, delta_step.cu): element types, groups of
+// elements between memory and FP32 registers, the activations, and the host-side checks of their entry points.
+#pragma once
+#include <cuda_fp16.h>
+#include <cstdio>
+#include "common.cuh"
+
+namespace rewy {
+
+using half_t = __half;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(half_t x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ half_t from_f32<half_t>(float x) { return __float2half_rn(x); }
+
+// V consecutive elements as they lie in memory; accesses of up to 16 bytes
+template <class T, int V>
+struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
+  T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ void load_pack(Pack<T, V>& d, const T* p) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4*>(&d)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else if constexpr (BYTES == 8) {
+    *reinterpret_cast<uint2*>(&d) = __ldg(reinterpret_cast<const uint2*>(p));
+  } else if constexpr (BYTES == 4) {
+    *reinterpret_cast<uint32_t*>(&d) = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) d.v[i] = p[i];
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& s) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&s)[i];
+  } else if constexpr (BYTES == 8) {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&s);
+  } else if constexpr (BYTES == 4) {
+    *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(&s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) p[i] = s.v[i];
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void zero_pack(Pack<T, V>& d) {
+#pragma unroll
+  for (int i = 0; i < V; i++) d.v[i] = from_f32<T>(0.f);
+}
+// V elements of which the first `valid` exist; `wide`: the address is aligned for whole accesses
+template <class T, int V>
+__device__ __forceinline__ void load_some(Pack<T, V>& d, const T* p, int valid, bool wide) {
+  if (wide && valid >= V) {
+    load_pack<T, V>(d, p);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) d.v[i] = i < valid ? p[i] : from_f32<T>(0.f);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_some(T* p, const Pack<T, V>& s, int valid, bool wide) {
+  if (wide && valid >= V) {
+    store_pack<T, V>(p, s);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++)
+    if (i < valid) p[i] = s.v[i];
+}
+
+// A parameter (weights, biases, scales): its own type, read once per thread
+__device__ __forceinline__ float param_at(const void* p, int dtype, long long i) {
+  if (dtype == REWY_F32) return static_cast<const float*>(p)[i];
+  if (dtype == REWY_BF16) return to_f32(static_cast<const bf16*>(p)[i]);
+  return to_f32(static_cast<const half_t*>(p)[i]);
+}
+__device__ __forceinline__ void param_store(void* p, int dtype, long long i, float x) {
+  if (dtype == REWY_F32) static_cast<float*>(p)[i] = x;
+  else if (dtype == REWY_BF16) static_cast<bf16*>(p)[i] = from_f32<bf16>(x);
+  else static_cast<half_t*>(p)[i] = from_f32<half_t>(x);
+}
+
+__device__ __forceinline__ float ex2(float x) {  // 2 ulp, results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {  // 1 ulp
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+// 1 / (1 + e^-x): e^-x overflows to infinity and its reciprocal to 0 for very negative x, as the sigmoid does
+__device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + ex2(-LOG2E * x)); }
+// softplus(x) = max(x, 0) + log(1 + e^-|x|), the logarithm as 2 atanh(s), s = e / (2 + e) <= 1/3 (series to s^13: 1.4e-8 of the
+// value); sig: its derivative, from the same exponential
+__device__ __forceinline__ float softplus_fast(float x, float& sig) {
+  const float e = ex2(-LOG2E * fabsf(x)), r = rcp_fast(1.f + e);
+  sig = x >= 0.f ? r : e * r;
+  const float s = e * rcp_fast(2.f + e), z = s * s;
+  float p = fmaf(z, 1.f / 13, 1.f / 11);
+  p = fmaf(z, p, 1.f / 9);
+  p = fmaf(z, p, 1.f / 7);
+  p = fmaf(z, p, 1.f / 5);
+  p = fmaf(z, p, 1.f / 3);
+  p = fmaf(z, p, 1.f);
+  return fmaxf(x, 0.f) + 2.f * s * p;
+}
+
+// Sequence of a packed batch that holds token t: the last s with cu[s] <= t
+__device__ __forceinline__ int packed_sequence(const int* cu, int num_seqs, int t) {
+  int lo = 0, hi = num_seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// The row of a state pool that row b of a batch of single tokens works on: -1 (nothing is done) if the index is outside the pool
+// or an earlier row has the same one.  Called by all threads of a block.
+__device__ __forceinline__ long long pool_row(const void* slots, int slots_are_i64, int b, long long pool) {
+  if (slots == nullptr) return b;
+  auto at = [&](int i) { return slots_are_i64 ? static_cast<const long long*>(slots)[i] : (long long)static_cast<const int*>(slots)[i]; };
+  const long long mine = at(b);
+  bool again = false;
+  for (int i = threadIdx.x; i < b; i += blockDim.x) again |= at(i) == mine;
+  const int any = __syncthreads_or(again);
+  return any || mine < 0 || mine >= pool ? -1 : mine;
+}
+
+inline bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+inline int element_bytes(int dtype) { return dtype == REWY_F32 ? 4 : 2; }
+inline bool known_dtype(int dtype) { return dtype == REWY_BF16 || dtype == REWY_F16 || dtype == REWY_F32; }
+inline int launched(const char* what, int n = 1) {
+  count_launch(n);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return REWY_OK;
+  char msg[200];
+  snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
+  return report_error(REWY_ERR_LAUNCH, msg);
+}
+// f(T()) with T the element type
+template <class F>
+inline void with_type(int dtype, F&& f) {
+  if (dtype == REWY_BF16) f(bf16());
+  else if (dtype == REWY_F16) f(half_t());
+  else f(float());
+}
+
+}  // namespace rewy
+
+#define LAYER_REQUIRE(ok, code, text) \
+  do {                                \
+    if (!(ok)) return report_error(code, text); \
+  } while (0)

@@ -1,0 +1,896 @@
+// Selective state space scan: a diagonal recurrence per channel whose decay and input weights depend on the token.
+//
+//   dt = softplus(dt_raw + bias);  a_t = exp(dt_t A);  h_t = a_t h_(t-1) + dt_t u_t B_t;  y_t = (C_t h_t + D u_t) silu(z_t)
+//   with dy' = dy silu(z):  gh_t = C_t dy'_t + a_(t+1) gh_(t+1);  drive_t = sum_n gh_t B_t;  q_t = gh_t h_(t-1) a_t
+//   du = dt drive + D dy';  ddt = sum_n q A + u drive;  dA = sum_t q dt;  dB = sum_m gh dt u;  dC = sum_m dy' h
+//
+// Everything is FP32 between the element types at both ends; nothing is kept in fewer bits in between.
+//
+// A thread holds four states of one channel, L neighbouring lanes the states of a channel (N <= 4 L), a CTA of 128 threads
+// 128 / L channels, which it takes through a segment of the tokens in tiles of 32: the tile's dt and dt u per channel and its B
+// and C are put into shared memory as FP32 once, with the softplus, by a pass that reads 8 elements per thread.  What bounds
+// the forward is one exponential per (token, channel, state) at 16 per clock and SM; the rest is 27 issue slots per token
+// and warp beside the 32 cycles that its four exponentials take.
+// The backward needs h_(t-1) in reverse: the forward leaves the state before every 16th token (4 N / 16 bytes per token and
+// channel), from which 16 tokens are run forward into registers (h and a, one exponential each) and walked back.
+// Sums over the states of a channel are exchanged for four tokens at a time (three shuffles for four lanes and four sums);
+// those over channels (dB, dC) leave each warp scattered over its lanes (seven shuffles for eight values and eight lanes), are
+// added over the CTA's warps in shared memory and over the CTAs by a second kernel, in one order: results repeat bit for bit.
+//
+// Few channels: the token axis is cut into segments.  A first pass finds each segment's end state from a zero start (backward:
+// the gradient that leaves its first token), and the main pass starts every segment from those before it, joined by
+// h <- exp(A sum dt) h + end.  That doubles the exponentials and pays only where most SMs would idle.
+#include <climits>
+#include "layer.cuh"
+
+namespace rewy {
+namespace {
+
+constexpr int TT = 32;    // tokens per tile
+constexpr int NT = 128;   // threads per CTA
+constexpr int S = 4;      // states per thread
+constexpr int CK = 16;    // tokens between checkpoints
+constexpr float LN2 = 0.6931471805599453f;
+
+struct ScanParams {
+  RewyScanArgs a;
+  int Mg, blocks, segments, seg_len;   // channels per group, CTAs per group, segments of seg_len tokens
+  float *seg_state, *seg_dt;           // [B][segments][M][N], [B][segments][M]
+  float *part_bc, *part_m;             // [blocks][B*T][G][2][N]; [B*segments][M*N + 2 M]
+  bool wide, wide_bc, wide_state;      // whole accesses possible for u, dt, z, y; B, C; the FP32 states
+};
+
+// Where a CTA works.
+template <int L>
+struct Place {
+  static constexpr int CH = NT / L, NP = S * L;
+  int b, seg, g, cb, m0, valid;        // first channel and how many exist
+  int t0, t1;                          // tokens of the segment
+  __device__ __forceinline__ Place(const ScanParams& p, int seg_offset, int seg_count) {
+    unsigned i = blockIdx.x;
+    cb = i % p.blocks; i /= p.blocks;
+    g = i % p.a.G; i /= p.a.G;
+    seg = i % seg_count + seg_offset;
+    b = i / seg_count;
+    m0 = g * p.Mg + cb * CH;
+    valid = min(CH, p.Mg - cb * CH);
+    t0 = seg * p.seg_len;
+    t1 = min(p.a.T, t0 + p.seg_len);
+  }
+};
+
+// Sequence bookkeeping of a CTA that moves forward through tokens.
+struct Sequence {
+  int s, begin, next;  // sequence, its first token, the first token of the one behind it (INT_MAX: none)
+  __device__ __forceinline__ void at(const RewyScanArgs& a, int b, int t) {
+    if (a.cu_seqlens == nullptr) { s = b; begin = 0; next = INT_MAX; return; }
+    s = packed_sequence(a.cu_seqlens, a.num_seqs, t);
+    begin = min(max(a.cu_seqlens[s], 0), t);
+    next = s + 1 < a.num_seqs ? max(a.cu_seqlens[s + 1], t + 1) : INT_MAX;
+  }
+  __device__ __forceinline__ void advance(const RewyScanArgs& a) {
+    s++;
+    begin = next;
+    next = s + 1 < a.num_seqs ? max(a.cu_seqlens[s + 1], begin + 1) : INT_MAX;
+  }
+};
+
+__device__ __forceinline__ void load4(float (&x)[S], const float* p, int n0, int N, bool ok, bool wide) {
+  if (ok && wide && n0 < N) {
+    const float4 v = *reinterpret_cast<const float4*>(p + n0);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < S; i++) x[i] = ok && n0 + i < N ? p[n0 + i] : 0.f;
+}
+__device__ __forceinline__ void store4(float* p, const float (&x)[S], int n0, int N, bool ok, bool wide) {
+  if (!ok) return;
+  if (wide) {
+    if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(x[0], x[1], x[2], x[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < S; i++)
+    if (n0 + i < N) p[n0 + i] = x[i];
+}
+
+// Sums of x over the L lanes of a channel.  Afterwards lane l of them holds in x[0] (L = 2: x[0], x[1]) the sum of value
+// sum_owner(l) (L = 2: and the next one); lanes of the same l % 4 hold the same.
+template <int L>
+__device__ __forceinline__ void sum_states(float (&x)[4], int l) {
+#pragma unroll
+  for (int m = L / 2; m >= 4; m >>= 1)
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], m);
+  const bool odd = l & 1;
+  const float k0 = odd ? x[2] : x[0], k1 = odd ? x[3] : x[1], s0 = odd ? x[0] : x[2], s1 = odd ? x[1] : x[3];
+  x[0] = k0 + __shfl_xor_sync(0xffffffffu, s0, 1);
+  x[1] = k1 + __shfl_xor_sync(0xffffffffu, s1, 1);
+  if constexpr (L >= 4) {
+    const bool up = l & 2;
+    const float k = up ? x[1] : x[0], s = up ? x[0] : x[1];
+    x[0] = k + __shfl_xor_sync(0xffffffffu, s, 2);
+  }
+}
+template <int L>
+__device__ __forceinline__ void put_sums(float* at, int stride, const float (&x)[4], int l) {  // at: row of the first of four tokens
+  const int first = (l & 1) * 2;
+  if constexpr (L == 2) {
+    at[first * stride] = x[0];
+    at[(first + 1) * stride] = x[1];
+  } else {
+    if (l < 4) at[(first + ((l >> 1) & 1)) * stride] = x[0];
+  }
+}
+
+// Sums of v over the warp's 32 / L channels (lanes that differ in the bits from L up); values are handed out on the way.  Calls
+// put(value index, sum) for those the lane ends with.
+template <int L, class F>
+__device__ __forceinline__ void sum_channels(float (&v)[8], int lane, F&& put) {
+  int base = 0;
+  int n = 8;
+#pragma unroll
+  for (int m = 16; m >= L; m >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = lane & m;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (i < n) {
+          const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+        }
+      base += up ? n : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (i < n) put(base + i, v[i]);
+}
+
+// A tile's rows of one [B,T,M] tensor: 8 channels per access.
+template <class T, int L>
+struct Rows {
+  static constexpr int CH = NT / L, PER_TOKEN = CH / 8, COUNT = TT * PER_TOKEN, EACH = (COUNT + NT - 1) / NT;
+  __device__ static __forceinline__ bool mine(int k, int& tok, int& c) {
+    const int i = threadIdx.x + k * NT;
+    tok = i / PER_TOKEN;
+    c = i % PER_TOKEN * 8;
+    return i < COUNT;
+  }
+};
+template <class T>
+__device__ __forceinline__ void fetch8(Pack<T, 8>& d, const T* base, long long token_stride, int t, int t1, int c, int valid, bool wide) {
+  load_some<T, 8>(d, base + t * token_stride + c, t < t1 ? valid - c : 0, wide);
+}
+// B and C of a tile as FP32 [TT][NP]; WHICH: 1 B, 2 C, 3 both
+template <class T, int L, int WHICH>
+struct Shared {
+  static constexpr int NP = S * L, PER_TOKEN = NP / 8, TENSORS = WHICH == 3 ? 2 : 1, COUNT = TT * PER_TOKEN * TENSORS, EACH = (COUNT + NT - 1) / NT;
+  Pack<T, 8> v[EACH];
+  __device__ __forceinline__ void fetch(const ScanParams& p, const T* B, const T* C, int t0, int t1) {
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int i = threadIdx.x + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      const int t = t0 + j / PER_TOKEN, n = j % PER_TOKEN * 8;
+      if (i < COUNT)
+        load_some<T, 8>(v[k], (which ? C + t * p.a.C_stride[1] : B + t * p.a.B_stride[1]) + n, t < t1 ? p.a.N - n : 0, p.wide_bc);
+    }
+  }
+  __device__ __forceinline__ void publish(float* sB, float* sC) const {
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int i = threadIdx.x + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      if (i < COUNT) {
+        float* to = (which ? sC : sB) + j * 8;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<float4*>(to + e) = make_float4(to_f32(v[k].v[e]), to_f32(v[k].v[e + 1]), to_f32(v[k].v[e + 2]), to_f32(v[k].v[e + 3]));
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float step_of(float raw, float bias, bool softplus) {
+  float sig;
+  return softplus ? softplus_fast(raw + bias, sig) : raw + bias;
+}
+
+// State at the first token of segment `seg` of a sequence that began before it, from the ends of the segments between.
+__device__ __forceinline__ void join_forward(float (&h)[S], const ScanParams& p, int b, int seg, int begin, long long m, const float (&A2)[S], int n0, bool ok) {
+  const int first = begin / p.seg_len;
+  for (int j = first; j < seg; j++) {
+    const long long row = ((long long)b * p.segments + j) * p.a.M + m;
+    float end[S];
+    load4(end, p.seg_state + row * p.a.N, n0, p.a.N, ok, p.wide_state);
+    const float d = ok ? p.seg_dt[row] : 0.f;
+#pragma unroll
+    for (int i = 0; i < S; i++) h[i] = j == first ? end[i] : fmaf(ex2(A2[i] * d), h[i], end[i]);
+  }
+}
+
+// STATE_ONLY: the first pass of a scan in segments (all but the last one).
+template <class T, int L, bool STATE_ONLY>
+__global__ void __launch_bounds__(NT) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
+  using R = Rows<T, L>;
+  __shared__ __align__(16) float sdt[TT * CH], sdu[TT * CH], sB[TT * NP], sC[STATE_ONLY ? 4 : TT * NP], sy[STATE_ONLY ? 4 : TT * YS], sbias[CH], sD[CH];
+  const RewyScanArgs& a = p.a;
+  const Place<L> at(p, 0, STATE_ONLY ? p.segments - 1 : p.segments);
+  const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
+  const bool ok = ch < at.valid;
+  const long long m = at.m0 + ch;
+  const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
+  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+  const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
+  const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
+  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+  for (int c = threadIdx.x; c < CH; c += NT) {
+    sbias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
+    sD[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
+  }
+  float A2[S], h[S] = {};
+  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+#pragma unroll
+  for (int i = 0; i < S; i++) A2[i] *= LOG2E;
+
+  Sequence q;
+  q.at(a, at.b, at.t0);
+  auto start = [&](int s) { load4(h, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state); };
+  auto finish = [&](int s) {
+    if (!STATE_ONLY && a.final_state != nullptr) store4(a.final_state + ((long long)s * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
+  };
+  if (q.begin == at.t0) start(q.s);
+  else if (!STATE_ONLY) join_forward(h, p, at.b, at.seg, q.begin, m, A2, n0, ok);
+
+  Pack<T, 8> ru[R::EACH], rd[R::EACH], rz[R::EACH], nu[R::EACH], nd[R::EACH], nz[R::EACH];
+  Shared<T, L, STATE_ONLY ? 1 : 3> bc;
+  auto fetch = [&](Pack<T, 8>(&xu)[R::EACH], Pack<T, 8>(&xd)[R::EACH], Pack<T, 8>(&xz)[R::EACH], int t) {
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c)) continue;
+      fetch8(xu[k], u, a.u_stride[1], t + tok, at.t1, c, at.valid, p.wide);
+      fetch8(xd[k], dt, a.dt_stride[1], t + tok, at.t1, c, at.valid, p.wide);
+      if (!STATE_ONLY && a.z != nullptr) fetch8(xz[k], z, a.z_stride[1], t + tok, at.t1, c, at.valid, p.wide);
+    }
+    bc.fetch(p, Bm, C, t, at.t1);
+  };
+  auto publish = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c)) continue;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool real = t + tok < at.t1 && c + e < at.valid;   // a token that does not exist: no decay, no input
+        const float d = real ? step_of(to_f32(rd[k].v[e]), sbias[c + e], a.softplus) : 0.f;
+        sdt[tok * CH + c + e] = d;
+        sdu[tok * CH + c + e] = real ? d * to_f32(ru[k].v[e]) : 0.f;
+      }
+    }
+    bc.publish(sB, sC);
+  };
+  fetch(ru, rd, rz, at.t0);
+  __syncthreads();   // sbias, sD
+  publish(at.t0);
+
+  float total = 0.f;
+  for (int t0 = at.t0; t0 < at.t1; t0 += TT) {
+    const bool more = t0 + TT < at.t1;
+    if (more) fetch(nu, nd, nz, t0 + TT);
+    __syncthreads();
+#pragma unroll 2
+    for (int k = 0; k < TT; k += 4) {
+      if (!STATE_ONLY && k % CK == 0 && a.checkpoints != nullptr && t0 + k < a.T)
+        store4(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + k) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
+      float y[4];
+      auto token = [&](int j) {
+        const float d = sdt[(k + j) * CH + ch], x = sdu[(k + j) * CH + ch];
+        const float4 Bv = *reinterpret_cast<const float4*>(sB + (k + j) * NP + n0);
+        h[0] = fmaf(ex2(d * A2[0]), h[0], x * Bv.x);
+        h[1] = fmaf(ex2(d * A2[1]), h[1], x * Bv.y);
+        h[2] = fmaf(ex2(d * A2[2]), h[2], x * Bv.z);
+        h[3] = fmaf(ex2(d * A2[3]), h[3], x * Bv.w);
+        if constexpr (STATE_ONLY) {
+          total += d;
+        } else {
+          const float4 Cv = *reinterpret_cast<const float4*>(sC + (k + j) * NP + n0);
+          y[j] = fmaf(Cv.x, h[0], Cv.y * h[1]) + fmaf(Cv.z, h[2], Cv.w * h[3]);
+        }
+      };
+      if (t0 + k + 3 < q.next) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) token(j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (t0 + k + j == q.next && t0 + k + j < at.t1) {
+            finish(q.s);
+            q.advance(a);
+            start(q.s);
+          }
+          token(j);
+        }
+      }
+      if constexpr (!STATE_ONLY) {
+        sum_states<L>(y, sl);
+        put_sums<L>(sy + k * YS + ch, YS, y, sl);
+      }
+    }
+    __syncthreads();
+    if constexpr (!STATE_ONLY) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
+        Pack<T, 8> out;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          float v = fmaf(sD[c + e], to_f32(ru[k].v[e]), sy[tok * YS + c + e]);
+          if (a.z != nullptr) {
+            const float g = to_f32(rz[k].v[e]);
+            v *= g * sigmoid_fast(g);
+          }
+          out.v[e] = from_f32<T>(v);
+        }
+        store_some<T, 8>(static_cast<T*>(a.y) + ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c, out, at.valid - c, p.wide);
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) { ru[k] = nu[k]; rd[k] = nd[k]; rz[k] = nz[k]; }
+      publish(t0 + TT);
+    }
+  }
+  if constexpr (STATE_ONLY) {
+    const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
+    store4(p.seg_state + row * a.N, h, n0, a.N, ok, p.wide_state);
+    if (ok && sl == 0) p.seg_dt[row] = total;
+  } else {
+    if (at.t1 == a.T || at.t1 == q.next) finish(q.s);
+  }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------
+
+// Gradient of the state that token t1 - 1 hands on: from the segments behind, or from the final state's gradient.
+template <int L>
+__device__ __forceinline__ void join_backward(float (&carry)[S], const ScanParams& p, const Place<L>& at, long long m, const float (&A2)[S], int n0, bool ok) {
+  const RewyScanArgs& a = p.a;
+  Sequence q;
+  q.at(a, at.b, at.t1 - 1);
+  const int end = min(q.next, a.T);
+  if (end <= at.t1) {   // the sequence ends with this segment
+    load4(carry, a.dfinal_state + ((long long)q.s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state);
+    return;
+  }
+  const int last = (end - 1) / p.seg_len;
+  for (int j = last; j > at.seg; j--) {
+    const long long row = ((long long)at.b * p.segments + j) * a.M + m;
+    float out[S];
+    load4(out, p.seg_state + row * a.N, n0, a.N, ok, p.wide_state);
+    const float d = ok ? p.seg_dt[row] : 0.f;
+#pragma unroll
+    for (int i = 0; i < S; i++) carry[i] = j == last ? out[i] : fmaf(ex2(A2[i] * d), carry[i], out[i]);
+  }
+}
+
+// First pass over the segments but the first: the gradient that leaves each one's first token for the state before it.
+template <class T, int L>
+__global__ void __launch_bounds__(NT) scan_bwd_state_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = NT / L, NP = S * L;
+  using R = Rows<T, L>;
+  __shared__ __align__(16) float sdt[TT * CH], sdy[TT * CH], sC[TT * NP], sbias[CH];
+  const RewyScanArgs& a = p.a;
+  const Place<L> at(p, 1, p.segments - 1);
+  const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
+  const bool ok = ch < at.valid;
+  const long long m = at.m0 + ch;
+  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+  const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
+  const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
+  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+  for (int c = threadIdx.x; c < CH; c += NT) sbias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
+  float A2[S], carry[S] = {}, total = 0.f;
+  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+#pragma unroll
+  for (int i = 0; i < S; i++) A2[i] *= LOG2E;
+  Sequence q;
+  q.at(a, at.b, at.t1 - 1);
+  auto last_of = [&](int s) { load4(carry, a.dfinal_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state); };
+  if (min(q.next, a.T) <= at.t1) last_of(q.s);
+  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  for (int tile = tiles - 1; tile >= 0; tile--) {
+    const int t0 = at.t0 + tile * TT;
+    __syncthreads();   // sbias; the tile before has been read
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c)) continue;
+      Pack<T, 8> xd, xy, xz;
+      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+      if (a.z != nullptr) fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool real = t0 + tok < at.t1 && c + e < at.valid;
+        float g = to_f32(xy.v[e]);
+        if (a.z != nullptr) {
+          const float v = to_f32(xz.v[e]);
+          g *= v * sigmoid_fast(v);
+        }
+        sdt[tok * CH + c + e] = real ? step_of(to_f32(xd.v[e]), sbias[c + e], a.softplus) : 0.f;
+        sdy[tok * CH + c + e] = real ? g : 0.f;
+      }
+    }
+    Shared<T, L, 2> cc;
+    cc.fetch(p, nullptr, C, t0, at.t1);
+    cc.publish(nullptr, sC);
+    __syncthreads();
+#pragma unroll 4
+    for (int k = TT - 1; k >= 0; k--) {
+      const float d = sdt[k * CH + ch], g = sdy[k * CH + ch];
+      const float4 Cv = *reinterpret_cast<const float4*>(sC + k * NP + n0);
+      carry[0] = ex2(d * A2[0]) * fmaf(Cv.x, g, carry[0]);
+      carry[1] = ex2(d * A2[1]) * fmaf(Cv.y, g, carry[1]);
+      carry[2] = ex2(d * A2[2]) * fmaf(Cv.z, g, carry[2]);
+      carry[3] = ex2(d * A2[3]) * fmaf(Cv.w, g, carry[3]);
+      total += d;
+      if (a.cu_seqlens != nullptr && t0 + k == q.begin && q.s > 0 && t0 + k > at.t0) {   // what flows on belongs to the sequence before
+        q.at(a, at.b, t0 + k - 1);
+        last_of(q.s);
+      }
+    }
+  }
+  const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
+  store4(p.seg_state + row * a.N, carry, n0, a.N, ok, p.wide_state);
+  if (ok && sl == 0) p.seg_dt[row] = total;
+}
+
+template <int L>
+struct BwdShared {
+  static constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
+  float dt[TT * CH], du[TT * CH], dy[TT * CH], B[TT * NP], C[TT * NP];
+  float drive[TT * YS], decay[TT * YS], y[TT * YS];   // per token and channel: sum gh B, sum q A2, sum C h
+  float bc[NT / 32][TT][2 * NP];                      // each warp's sums over its channels
+  float dD[TT * CH], dbias[TT * CH];                  // running sums, one entry per token of the tile
+  float bias[CH], D[CH];
+};
+
+template <class T, int L>
+__global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
+  using R = Rows<T, L>;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  BwdShared<L>& sm = *reinterpret_cast<BwdShared<L>*>(raw_smem);
+  const RewyScanArgs& a = p.a;
+  const Place<L> at(p, 0, p.segments);
+  const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool ok = ch < at.valid, gated = a.z != nullptr;
+  const long long m = at.m0 + ch;
+  const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
+  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+  const T* z = static_cast<const T*>(a.z) + (gated ? at.b * a.z_stride[0] + at.m0 : 0);
+  const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
+  const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
+  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+  for (int c = threadIdx.x; c < CH; c += NT) {
+    sm.bias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
+    sm.D[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
+  }
+  for (int i = threadIdx.x; i < TT * CH; i += NT) sm.dD[i] = sm.dbias[i] = 0.f;
+  float A2[S], carry[S] = {}, dA[S] = {};
+  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+#pragma unroll
+  for (int i = 0; i < S; i++) A2[i] *= LOG2E;
+  join_backward<L>(carry, p, at, m, A2, n0, ok);
+
+  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  for (int tile = tiles - 1; tile >= 0; tile--) {
+    const int t0 = at.t0 + tile * TT;
+    __syncthreads();   // bias, D and the zeroed sums; the tile behind has been read
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c)) continue;
+      Pack<T, 8> xu, xd, xy, xz;
+      fetch8(xu, u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+      if (gated) fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int i = tok * CH + c + e;
+        const bool real = t0 + tok < at.t1 && c + e < at.valid;
+        const float d = real ? step_of(to_f32(xd.v[e]), sm.bias[c + e], a.softplus) : 0.f;
+        float g = to_f32(xy.v[e]);
+        if (gated) {
+          const float v = to_f32(xz.v[e]);
+          g *= v * sigmoid_fast(v);
+        }
+        sm.dt[i] = d;
+        sm.du[i] = real ? d * to_f32(xu.v[e]) : 0.f;
+        sm.dy[i] = real ? g : 0.f;
+      }
+    }
+    {
+      Shared<T, L, 3> bc;
+      bc.fetch(p, Bm, C, t0, at.t1);
+      bc.publish(sm.B, sm.C);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int sub = TT / CK - 1; sub >= 0; sub--) {
+      const int k0 = sub * CK, ts = t0 + k0;
+      if (ts >= at.t1) continue;
+      // bit j: a sequence starts at token ts + j; `s_last`: the sequence of the last one that does
+      unsigned starts = ts == 0 ? 1u : 0u;
+      int s_last = at.b, s_low = at.b;
+      if (a.cu_seqlens != nullptr) {
+        Sequence q;
+        q.at(a, at.b, ts);
+        starts = q.begin == ts ? 1u : 0u;
+        s_low = q.s;
+        while (q.next < min(ts + CK, at.t1)) {
+          q.advance(a);
+          starts |= 1u << (q.begin - ts);
+        }
+        s_last = q.s;
+      }
+      float before[S], h[CK][S], dec[CK][S];
+      load4(before, a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + ts / CK) * a.M + m) * a.N, n0, a.N, ok, p.wide_state);
+      auto initial = [&](float(&x)[S], int s) {
+        load4(x, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
+      };
+      {
+        float x[S];
+        int s = s_low;
+#pragma unroll
+        for (int i = 0; i < S; i++) x[i] = before[i];
+        if (starts & 1u) {
+          initial(before, s);
+#pragma unroll
+          for (int i = 0; i < S; i++) x[i] = before[i];
+        }
+#pragma unroll
+        for (int j = 0; j < CK; j++) {
+          if (j > 0 && (starts >> j & 1u)) initial(x, ++s);
+          const float d = sm.dt[(k0 + j) * CH + ch], w = sm.du[(k0 + j) * CH + ch];
+          const float4 Bv = *reinterpret_cast<const float4*>(sm.B + (k0 + j) * NP + n0);
+          const float b4[S] = {Bv.x, Bv.y, Bv.z, Bv.w};
+#pragma unroll
+          for (int i = 0; i < S; i++) {
+            dec[j][i] = ex2(d * A2[i]);
+            x[i] = fmaf(dec[j][i], x[i], w * b4[i]);
+            h[j][i] = x[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
+        float drive[4], decay[4], y[4];
+#pragma unroll
+        for (int jj = 3; jj >= 0; jj--) {
+          const int j = j4 + jj;
+          const float d = sm.dt[(k0 + j) * CH + ch], w = sm.du[(k0 + j) * CH + ch], g = sm.dy[(k0 + j) * CH + ch];
+          const float4 Bv = *reinterpret_cast<const float4*>(sm.B + (k0 + j) * NP + n0), Cv = *reinterpret_cast<const float4*>(sm.C + (k0 + j) * NP + n0);
+          const float b4[S] = {Bv.x, Bv.y, Bv.z, Bv.w}, c4[S] = {Cv.x, Cv.y, Cv.z, Cv.w};
+          const bool first = starts >> j & 1u;
+          float old[S];
+#pragma unroll
+          for (int i = 0; i < S; i++) old[i] = j == 0 ? before[i] : h[j > 0 ? j - 1 : 0][i];
+          if (j > 0 && first) initial(old, s_last);
+          float v[8], dr = 0.f, de = 0.f, yy = 0.f;
+#pragma unroll
+          for (int i = 0; i < S; i++) {
+            const float gh = fmaf(c4[i], g, carry[i]);
+            carry[i] = dec[j][i] * gh;
+            const float qv = carry[i] * old[i];
+            dr = fmaf(gh, b4[i], dr);
+            de = fmaf(qv, A2[i], de);
+            yy = fmaf(c4[i], h[j][i], yy);
+            dA[i] = fmaf(qv, d, dA[i]);
+            v[i] = gh * w;
+            v[4 + i] = g * h[j][i];
+          }
+          drive[jj] = dr; decay[jj] = de; y[jj] = yy;
+          sum_channels<L>(v, lane, [&](int i, float x) { sm.bc[warp][k0 + j][(i >> 2) * NP + n0 + (i & 3)] = x; });
+          if (first) {
+            if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s_last * a.M + m) * a.N, carry, n0, a.N, ok, p.wide_state);
+            s_last--;
+            const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s_last >= 0;
+            load4(carry, a.dfinal_state + ((long long)(has ? s_last : 0) * a.M + m) * a.N, n0, a.N, ok && has, p.wide_state);
+          }
+        }
+        sum_states<L>(drive, sl);
+        put_sums<L>(sm.drive + (k0 + j4) * YS + ch, YS, drive, sl);
+        sum_states<L>(decay, sl);
+        put_sums<L>(sm.decay + (k0 + j4) * YS + ch, YS, decay, sl);
+        if (gated) {
+          sum_states<L>(y, sl);
+          put_sums<L>(sm.y + (k0 + j4) * YS + ch, YS, y, sl);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
+      Pack<T, 8> xu, xd, xy, xz, ou, od, oz;
+      fetch8(xu, u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      if (gated) {
+        fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+        fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int i = tok * CH + c + e, iy = tok * YS + c + e;
+        const float uv = to_f32(xu.v[e]), g = sm.dy[i], drive = sm.drive[iy], Dv = sm.D[c + e];
+        float dd = fmaf(uv, drive, LN2 * sm.decay[iy]);
+        if (a.softplus) dd *= sigmoid_fast(to_f32(xd.v[e]) + sm.bias[c + e]);
+        ou.v[e] = from_f32<T>(fmaf(Dv, g, drive * sm.dt[i]));
+        od.v[e] = from_f32<T>(dd);
+        sm.dD[i] = fmaf(g, uv, sm.dD[i]);
+        sm.dbias[i] += dd;
+        if (gated) {
+          const float v = to_f32(xz.v[e]), sig = sigmoid_fast(v);
+          oz.v[e] = from_f32<T>(to_f32(xy.v[e]) * fmaf(Dv, uv, sm.y[iy]) * sig * fmaf(v, 1.f - sig, 1.f));
+        }
+      }
+      const long long to = ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c;
+      store_some<T, 8>(static_cast<T*>(a.du) + to, ou, at.valid - c, p.wide);
+      store_some<T, 8>(static_cast<T*>(a.ddt) + to, od, at.valid - c, p.wide);
+      if (gated) store_some<T, 8>(static_cast<T*>(a.dz) + to, oz, at.valid - c, p.wide);
+    }
+    for (int i = threadIdx.x; i < TT * 2 * NP; i += NT) {
+      const int tok = i / (2 * NP), v = i % (2 * NP), n = v % NP;
+      if (t0 + tok >= at.t1 || n >= a.N) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NT / 32; w++) sum += sm.bc[w][tok][v];
+      p.part_bc[((((long long)at.cb * a.B + at.b) * a.T + t0 + tok) * a.G + at.g) * 2 * a.N + v / NP * a.N + n] = sum;
+    }
+  }
+  float* part = p.part_m + ((long long)at.b * p.segments + at.seg) * ((long long)a.M * (a.N + 2));
+  store4(part + m * a.N, dA, n0, a.N, ok, false);
+  __syncthreads();
+  for (int c = threadIdx.x; c < at.valid; c += NT) {
+    float x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < TT; k++) { x += sm.dD[k * CH + c]; y += sm.dbias[k * CH + c]; }
+    part[(long long)a.M * a.N + at.m0 + c] = x;
+    part[(long long)a.M * (a.N + 1) + at.m0 + c] = y;
+  }
+}
+
+// dB, dC [B*T][G][N] from the CTAs' sums [blocks][B*T][G][2][N]
+template <class T>
+__global__ void __launch_bounds__(256) scan_sum_bc_kernel(const float* __restrict__ part, int blocks, long long rows, int N, T* __restrict__ dB, T* __restrict__ dC) {
+  const long long n = rows * 2 * N, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < blocks; k++) sum += part[k * n + i];
+  const long long row = i / (2 * N);
+  const int v = (int)(i % (2 * N));
+  (v < N ? dB + row * N + v : dC + row * N + v - N)[0] = from_f32<T>(sum);
+}
+// dA [M,N], dD and ddt_bias [M] from the sums [parts][M N + 2 M]
+__global__ void __launch_bounds__(256) scan_sum_m_kernel(const float* __restrict__ part, int parts, long long MN, int M, float* dA, float* dD, float* dbias) {
+  const long long n = MN + 2 * M, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < parts; k++) sum += part[k * n + i];
+  float* to = i < MN ? dA + i : i < MN + M ? (dD != nullptr ? dD + (i - MN) : nullptr) : (dbias != nullptr ? dbias + (i - MN - M) : nullptr);
+  if (to != nullptr) *to = sum;
+}
+
+// One token per row: a channel's states over L lanes as above.
+template <class T, int L>
+__global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide) {
+  constexpr int CH = NT / L;
+  const int b = blockIdx.x / blocks, ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
+  const long long m = (long long)(blockIdx.x % blocks) * CH + ch;
+  const bool ok = m < a.M;
+  const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
+  T* y = static_cast<T*>(a.y) + (long long)b * a.M + m;
+  if (slot < 0) {
+    if (ok && sl == 0) *y = from_f32<T>(0.f);
+    return;
+  }
+  float out = 0.f, uv = 0.f;
+  if (ok) {
+    float* state = a.state + (slot * a.M + m) * a.N;
+    const int g = (int)(m / (a.M / a.G));
+    const T* Bm = static_cast<const T*>(a.Bm) + b * a.B_stride[0] + g * a.B_stride[1];
+    const T* C = static_cast<const T*>(a.C) + b * a.C_stride[0] + g * a.C_stride[1];
+    float h[S], A2[S];
+    load4(h, state, n0, a.N, true, wide);
+    load4(A2, a.A + m * a.N, n0, a.N, true, wide);
+    uv = to_f32(static_cast<const T*>(a.u)[b * a.u_stride + m]);
+    const float d = step_of(to_f32(static_cast<const T*>(a.dt)[b * a.dt_stride + m]), a.dt_bias != nullptr ? a.dt_bias[m] : 0.f, a.softplus);
+#pragma unroll
+    for (int i = 0; i < S; i++) {
+      const bool real = n0 + i < a.N;
+      const float Bv = real ? to_f32(Bm[n0 + i]) : 0.f, Cv = real ? to_f32(C[n0 + i]) : 0.f;
+      h[i] = fmaf(ex2(d * (A2[i] * LOG2E)), h[i], d * uv * Bv);
+      out = fmaf(Cv, h[i], out);
+    }
+    store4(state, h, n0, a.N, true, wide);
+  }
+#pragma unroll
+  for (int k = L / 2; k > 0; k >>= 1) out += __shfl_xor_sync(0xffffffffu, out, k);
+  if (ok && sl == 0) {
+    if (a.D != nullptr) out = fmaf(a.D[m], uv, out);
+    if (a.z != nullptr) {
+      const float g = to_f32(static_cast<const T*>(a.z)[b * a.z_stride + m]);
+      out *= g * sigmoid_fast(g);
+    }
+    *y = from_f32<T>(out);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+
+int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+template <class F>
+void with_lanes(int N, F&& f) {
+  switch (lanes_of(N)) {
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 8: f(std::integral_constant<int, 8>()); break;
+    default: f(std::integral_constant<int, 16>()); break;
+  }
+}
+
+struct Plan {
+  int blocks, segments, seg_len;
+  long long ctas;                                     // per segment
+  size_t seg_state, seg_dt, bc, m;                    // floats
+};
+Plan make_plan(int B, int T, int M, int N, int G, bool backward) {
+  Plan p{};
+  const int CH = NT / lanes_of(N), Mg = M / G;
+  p.blocks = (Mg + CH - 1) / CH;
+  p.ctas = (long long)p.blocks * G * B;
+  const int tiles = (T + TT - 1) / TT;
+  long long want = p.ctas >= 74 ? 1 : 148 * 3 / p.ctas;
+  if (want > tiles / 4) want = tiles / 4;
+  if (want < 3) want = 1;                             // two segments cost what they save
+  const int tiles_per = (int)((tiles + want - 1) / want);
+  p.seg_len = tiles_per * TT;
+  p.segments = (T + p.seg_len - 1) / p.seg_len;
+  const size_t rows = (size_t)B * p.segments * M;
+  p.seg_state = p.segments > 1 ? rows * N : 0;
+  p.seg_dt = p.segments > 1 ? rows : 0;
+  if (backward) {
+    p.bc = (size_t)p.blocks * B * T * G * 2 * N;
+    p.m = (size_t)B * p.segments * M * (N + 2);
+  }
+  auto up = [](size_t x) { return (x + 63) & ~size_t(63); };
+  p.seg_state = up(p.seg_state); p.seg_dt = up(p.seg_dt); p.bc = up(p.bc); p.m = up(p.m);
+  return p;
+}
+
+int check_scan(const RewyScanArgs* a, bool backward, Plan& plan) {
+  LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
+  LAYER_REQUIRE(known_dtype(a->dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
+  LAYER_REQUIRE(a->B > 0 && a->T > 0 && a->M > 0 && a->G > 0, REWY_ERR_SHAPE, "B, T, M and G must be positive");
+  LAYER_REQUIRE(a->N >= 1 && a->N <= 64, REWY_ERR_UNSUPPORTED, "the scan takes 1 to 64 states per channel");
+  LAYER_REQUIRE(a->M % a->G == 0, REWY_ERR_SHAPE, "the channels must divide into the groups of B and C");
+  LAYER_REQUIRE((long long)a->B * a->T <= (1LL << 30) && a->M <= (1 << 24), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or M 2^24 channels");
+  LAYER_REQUIRE(a->u != nullptr && a->dt != nullptr && a->Bm != nullptr && a->C != nullptr && a->A != nullptr, REWY_ERR_NULL, "u, dt, B, C or A is NULL");
+  LAYER_REQUIRE(a->cu_seqlens == nullptr || (a->B == 1 && a->num_seqs > 0), REWY_ERR_SHAPE, "packed sequences need B = 1 and num_seqs > 0");
+  plan = make_plan(a->B, a->T, a->M, a->N, a->G, backward);
+  LAYER_REQUIRE(plan.ctas * plan.segments < (1LL << 31), REWY_ERR_SHAPE, "more rows and channels than one grid holds");
+  const size_t need = (plan.seg_state + plan.seg_dt + plan.bc + plan.m) * sizeof(float);
+  LAYER_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need), REWY_ERR_WORKSPACE, "the workspace of the scan is too small");
+  return REWY_OK;
+}
+
+ScanParams scan_params(const RewyScanArgs& a, const Plan& plan) {
+  ScanParams p{};
+  p.a = a;
+  p.Mg = a.M / a.G; p.blocks = plan.blocks; p.segments = plan.segments; p.seg_len = plan.seg_len;
+  float* w = static_cast<float*>(a.workspace);
+  p.seg_state = w; w += plan.seg_state;
+  p.seg_dt = w; w += plan.seg_dt;
+  p.part_bc = w; w += plan.bc;
+  p.part_m = w;
+  const int e = element_bytes(a.dtype), per16 = 16 / e;
+  auto row = [&](const void* q) { return !unaligned16(q); };
+  auto step = [&](int64_t s) { return s % per16 == 0; };
+  p.wide = p.Mg % 8 == 0 && row(a.u) && row(a.dt) && row(a.z) && row(a.y) && row(a.dy) && row(a.du) && row(a.ddt) && row(a.dz);
+  for (int i = 0; i < 2; i++) p.wide = p.wide && step(a.u_stride[i]) && step(a.dt_stride[i]) && (a.z == nullptr || step(a.z_stride[i]));
+  p.wide_bc = a.N % 8 == 0 && row(a.Bm) && row(a.C);
+  for (int i = 0; i < 3; i++) p.wide_bc = p.wide_bc && step(a.B_stride[i]) && step(a.C_stride[i]);
+  p.wide_state = a.N % 4 == 0 && row(a.A) && row(a.initial_state) && row(a.final_state) && row(a.checkpoints) && row(a.dfinal_state) &&
+                 row(a.dinitial_state) && row(a.workspace);
+  return p;
+}
+
+}  // namespace
+}  // namespace rewy
+
+using namespace rewy;
+
+extern "C" size_t rewy_scan_checkpoint_bytes(int32_t B, int32_t T, int32_t M, int32_t N) {
+  if (B <= 0 || T <= 0 || M <= 0 || N <= 0) return 0;
+  return (size_t)B * ((T + CK - 1) / CK) * M * N * sizeof(float);
+}
+
+extern "C" size_t rewy_scan_workspace_bytes(int32_t B, int32_t T, int32_t M, int32_t N, int32_t G, int32_t backward) {
+  if (B <= 0 || T <= 0 || M <= 0 || N <= 0 || N > 64 || G <= 0 || M % G) return 0;
+  const Plan p = make_plan(B, T, M, N, G, backward != 0);
+  return (p.seg_state + p.seg_dt + p.bc + p.m) * sizeof(float);
+}
+
+extern "C" int rewy_scan_fwd(const RewyScanArgs* a, rewy_stream_t st) {
+  Plan plan;
+  if (const int rc = check_scan(a, false, plan)) return rc;
+  LAYER_REQUIRE(a->y != nullptr, REWY_ERR_NULL, "y is NULL");
+  const ScanParams p = scan_params(*a, plan);
+  const cudaStream_t s = (cudaStream_t)st;
+  with_type(a->dtype, [&](auto t) {
+    with_lanes(a->N, [&](auto l) {
+      using T = decltype(t);
+      if (plan.segments > 1) scan_fwd_kernel<T, l.value, true><<<(unsigned)(plan.ctas * (plan.segments - 1)), NT, 0, s>>>(p);
+      scan_fwd_kernel<T, l.value, false><<<(unsigned)(plan.ctas * plan.segments), NT, 0, s>>>(p);
+    });
+  });
+  return launched("selective scan forward", plan.segments > 1 ? 2 : 1);
+}
+
+extern "C" int rewy_scan_bwd(const RewyScanArgs* a, rewy_stream_t st) {
+  Plan plan;
+  if (const int rc = check_scan(a, true, plan)) return rc;
+  LAYER_REQUIRE(a->dy != nullptr && a->checkpoints != nullptr && a->du != nullptr && a->ddt != nullptr && a->dB != nullptr && a->dC != nullptr && a->dA != nullptr,
+                REWY_ERR_NULL, "dy, checkpoints or a gradient is NULL");
+  LAYER_REQUIRE((a->z == nullptr) == (a->dz == nullptr), REWY_ERR_NULL, "dz goes with z");
+  const ScanParams p = scan_params(*a, plan);
+  const cudaStream_t s = (cudaStream_t)st;
+  cudaError_t e = cudaSuccess;
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    with_lanes(a->N, [&](auto l) {
+      constexpr int L = l.value;
+      e = ensure_dynamic_smem<scan_bwd_kernel<T, L>>(sizeof(BwdShared<L>));
+      if (e != cudaSuccess) return;
+      if (plan.segments > 1) scan_bwd_state_kernel<T, L><<<(unsigned)(plan.ctas * (plan.segments - 1)), NT, 0, s>>>(p);
+      scan_bwd_kernel<T, L><<<(unsigned)(plan.ctas * plan.segments), NT, sizeof(BwdShared<L>), s>>>(p);
+    });
+    if (e != cudaSuccess) return;
+    const long long rows = (long long)a->B * a->T * a->G;
+    scan_sum_bc_kernel<T><<<(unsigned)((rows * 2 * a->N + 255) / 256), 256, 0, s>>>(p.part_bc, plan.blocks, rows, a->N, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
+  });
+  if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
+  const long long MN = (long long)a->M * a->N;
+  scan_sum_m_kernel<<<(unsigned)((MN + 2 * a->M + 255) / 256), 256, 0, s>>>(p.part_m, a->B * plan.segments, MN, a->M, a->dA, a->dD, a->ddt_bias);
+  return launched("selective scan backward", plan.segments > 1 ? 4 : 3);
+}
+
+extern "C" int rewy_scan_step(const RewyScanStepArgs* a, rewy_stream_t st) {
+  LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
+  LAYER_REQUIRE(known_dtype(a->dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
+  LAYER_REQUIRE(a->N >= 1 && a->N <= 64, REWY_ERR_UNSUPPORTED, "the scan takes 1 to 64 states per channel");
+  LAYER_REQUIRE(a->B > 0 && a->M > 0 && a->G > 0 && a->pool > 0 && a->M % a->G == 0, REWY_ERR_SHAPE, "bad B, M, G or pool");
+  LAYER_REQUIRE(a->slots != nullptr || a->pool >= a->B, REWY_ERR_SHAPE, "fewer states than rows");
+  LAYER_REQUIRE(a->M <= (1 << 24) && (long long)a->B * (a->M / 8 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more rows and channels than one grid holds");
+  LAYER_REQUIRE(a->u != nullptr && a->dt != nullptr && a->Bm != nullptr && a->C != nullptr && a->A != nullptr && a->state != nullptr && a->y != nullptr,
+                REWY_ERR_NULL, "a required pointer of the scan step is NULL");
+  const bool wide = a->N % 4 == 0 && !unaligned16(a->state) && !unaligned16(a->A);
+  with_type(a->dtype, [&](auto t) {
+    with_lanes(a->N, [&](auto l) {
+      const int CH = NT / l.value, blocks = (a->M + CH - 1) / CH;
+      scan_step_kernel<decltype(t), l.value><<<(unsigned)((long long)blocks * a->B), NT, 0, (cudaStream_t)st>>>(*a, blocks, wide);
+    });
+  });
+  return launched("selective scan step");
+}
