@@ -16,6 +16,7 @@ namespace rewy {
 namespace {
 
 constexpr int WARPS = 8;
+constexpr int FWD_V = 4, BWD_V = 2;  // neighbouring channels per lane
 
 struct ConvParams {
   RewyConvArgs a;
@@ -74,8 +75,8 @@ struct Columns {  // a warp's channels
 };
 
 template <class T, int W, int V>
-__global__ void __launch_bounds__(WARPS * 32) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
-  constexpr int U = 8;
+__global__ void __launch_bounds__(WARPS * 32, 3) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
+  constexpr int U = 4;
   const int channel = (blockIdx.x % p.channel_blocks * 32 + (threadIdx.x & 31)) * V;
   const unsigned rest = blockIdx.x / p.channel_blocks;
   const int b = rest / p.token_blocks;
@@ -85,24 +86,15 @@ __global__ void __launch_bounds__(WARPS * 32) conv_fwd_kernel(const __grid_const
   const Columns<T, W, V> c(p, b, channel);
   T* y = static_cast<T*>(p.a.y) + (long long)b * p.a.T * p.a.D + channel;
   Span s = span_at(p.a, b, t0);
-  float win[W - 1][V];
-  c.window(win, s, t0);
-  for (int t = t0; t < t1; t += U) {
-    Pack<T, V> in[U];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (t + u < t1) c.load_x(in[u], t + u);
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (t + u >= t1) break;
-      if (t + u == s.end) {
-        s = span_after(p.a, s);
-        c.window(win, s, t + u);
-      }
+  for (int from = t0; from < t1;) {   // the part of one sequence that lies in the block
+    const int to = min(t1, s.end);
+    float win[W - 1][V];
+    c.window(win, s, from);
+    auto token = [&](int t, const Pack<T, V>& in) {
       Pack<T, V> out;
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float now = to_f32(in[u].v[i]);
+        const float now = to_f32(in.v[i]);
         float pre = fmaf(c.weight[W - 1][i], now, c.bias[i]);
 #pragma unroll
         for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
@@ -111,22 +103,42 @@ __global__ void __launch_bounds__(WARPS * 32) conv_fwd_kernel(const __grid_const
         for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
         win[W - 2][i] = now;
       }
-      store_some<T, V>(y + (long long)(t + u) * p.a.D, out, c.valid, c.wide);
-      if (p.a.final_state != nullptr && t + u == s.end - 1) {
+      store_some<T, V>(y + (long long)t * p.a.D, out, c.valid, c.wide);
+    };
+    Pack<T, V> in[U], next[U];
+    int t = from;
+    if (t + U <= to)
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) {
-          Pack<T, V> v;
+      for (int u = 0; u < U; u++) c.load_x(in[u], t + u);
+    for (; t + U <= to; t += U) {      // the next rows are under way while these are worked on
+      if (t + 2 * U <= to)
 #pragma unroll
-          for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(win[j][i]);
-          store_some<T, V>(static_cast<T*>(p.a.final_state) + s.s * c.state_row + (long long)j * p.a.D + channel, v, c.valid, c.wide);
-        }
+        for (int u = 0; u < U; u++) c.load_x(next[u], t + U + u);
+#pragma unroll
+      for (int u = 0; u < U; u++) token(t + u, in[u]);
+#pragma unroll
+      for (int u = 0; u < U; u++) in[u] = next[u];
+    }
+    for (; t < to; t++) {
+      c.load_x(in[0], t);
+      token(t, in[0]);
+    }
+    if (p.a.final_state != nullptr && to == s.end) {
+#pragma unroll
+      for (int j = 0; j < W - 1; j++) {
+        Pack<T, V> v;
+#pragma unroll
+        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(win[j][i]);
+        store_some<T, V>(static_cast<T*>(p.a.final_state) + s.s * c.state_row + (long long)j * p.a.D + channel, v, c.valid, c.wide);
       }
     }
+    from = to;
+    if (from < t1) s = span_after(p.a, s);
   }
 }
 
 template <class T, int W, int V>
-__global__ void __launch_bounds__(WARPS * 32) conv_bwd_kernel(const __grid_constant__ ConvParams p, float* __restrict__ partial) {
+__global__ void __launch_bounds__(WARPS * 32, 3) conv_bwd_kernel(const __grid_constant__ ConvParams p, float* __restrict__ partial) {
   constexpr int U = 4;
   __shared__ float sums[WARPS][W + 1][32 * V];
   const RewyConvArgs& a = p.a;
@@ -147,69 +159,102 @@ __global__ void __launch_bounds__(WARPS * 32) conv_bwd_kernel(const __grid_const
       const int to = min(t1, s.end);
       float win[W - 1][V], g[W - 1][V] = {};
       c.window(win, s, from);
-      const int stop = to + W - 1, real = min(stop, s.end);   // beyond the sequence there is no g
-      for (int t = from; t < stop; t += U) {
-        Pack<T, V> in[U], d[U];
+      auto load = [&](Pack<T, V>& x, Pack<T, V>& d, int t) {
+        c.load_x(x, t);
+        load_some<T, V>(d, dy + (long long)t * a.D, c.valid, c.wide);
+      };
+      // Token t of the sequence: its g, and out, the complete gradient W-1 tokens before it.  OWN: it counts for dweight.
+      auto step = [&](auto own, const Pack<T, V>& in, const Pack<T, V>& d, float (&out)[V]) {
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (t + u < real) {
-            c.load_x(in[u], t + u);
-            load_some<T, V>(d[u], dy + (long long)(t + u) * a.D, c.valid, c.wide);
+        for (int i = 0; i < V; i++) {
+          const float x = to_f32(in.v[i]);
+          float gi = to_f32(d.v[i]);
+          if (a.activation) {
+            float pre = fmaf(c.weight[W - 1][i], x, c.bias[i]);
+#pragma unroll
+            for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
+            const float sig = sigmoid_fast(pre);
+            gi *= sig * fmaf(pre, 1.f - sig, 1.f);
           }
+          if (own.value) {
+#pragma unroll
+            for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi, win[w][i], dw[w][i]);
+            dw[W - 1][i] = fmaf(gi, x, dw[W - 1][i]);
+            db[i] += gi;
+          }
+#pragma unroll
+          for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
+          win[W - 2][i] = x;
+          out[i] = c.weight[0][i] * gi;
+#pragma unroll
+          for (int w = 1; w < W; w++) out[i] = fmaf(c.weight[w][i], g[W - 1 - w][i], out[i]);
+#pragma unroll
+          for (int j = 0; j < W - 2; j++) g[j][i] = g[j + 1][i];
+          g[W - 2][i] = gi;
+        }
+      };
+      auto put = [&](int pos, float (&out)[V]) {
+        Pack<T, V> v;
+#pragma unroll
+        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
+        store_some<T, V>(dx + (long long)pos * a.D, v, c.valid, c.wide);
+      };
+      // At the edges: rows before the sequence are its initial state's, the last ones get the final state's gradient too.
+      auto put_edge = [&](int pos, float (&out)[V]) {
+        const bool before = pos < from;
+        if (before && (from != s.begin || a.dinitial_state == nullptr)) return;
+        if (a.dfinal_state != nullptr && pos >= s.end - (W - 1)) {
+          Pack<T, V> v;
+          load_some<T, V>(v, static_cast<const T*>(a.dfinal_state) + s.s * c.state_row + (long long)(pos - (s.end - (W - 1))) * a.D + channel,
+                          c.valid, c.wide);
+#pragma unroll
+          for (int i = 0; i < V; i++) out[i] += to_f32(v.v[i]);
+        }
+        if (!before) {
+          put(pos, out);
+          return;
+        }
+        Pack<T, V> v;
+#pragma unroll
+        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
+        store_some<T, V>(static_cast<T*>(a.dinitial_state) + s.s * c.state_row + (long long)(W - 1 + pos - s.begin) * a.D + channel, v, c.valid, c.wide);
+      };
+      float out[V];
+      int t = from;
+      Pack<T, V> in[U], d[U], next[U], nd[U];
+#pragma unroll 1
+      for (; t < min(from + W - 1, to); t++) {
+        load(in[0], d[0], t);
+        step(std::true_type(), in[0], d[0], out);
+        put_edge(t - (W - 1), out);
+      }
+      if (t + U <= to)
+#pragma unroll
+        for (int u = 0; u < U; u++) load(in[u], d[u], t + u);
+      for (; t + U <= to; t += U) {   // the next rows are under way while these are worked on
+        if (t + 2 * U <= to)
+#pragma unroll
+          for (int u = 0; u < U; u++) load(next[u], nd[u], t + U + u);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          const int now = t + u;
-          if (now >= stop) break;
-          float fresh[V], out[V];
-#pragma unroll
-          for (int i = 0; i < V; i++) {
-            fresh[i] = 0.f;
-            if (now < real) {
-              const float x = to_f32(in[u].v[i]);
-              float gi = to_f32(d[u].v[i]);
-              if (a.activation) {
-                float pre = fmaf(c.weight[W - 1][i], x, c.bias[i]);
-#pragma unroll
-                for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
-                const float sig = sigmoid_fast(pre);
-                gi *= sig * fmaf(pre, 1.f - sig, 1.f);
-              }
-              if (now < to) {
-#pragma unroll
-                for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi, win[w][i], dw[w][i]);
-                dw[W - 1][i] = fmaf(gi, x, dw[W - 1][i]);
-                db[i] += gi;
-              }
-#pragma unroll
-              for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
-              win[W - 2][i] = x;
-              fresh[i] = gi;
-            }
-            out[i] = c.weight[0][i] * fresh[i];
-#pragma unroll
-            for (int w = 1; w < W; w++) out[i] = fmaf(c.weight[w][i], g[W - 1 - w][i], out[i]);
-#pragma unroll
-            for (int j = 0; j < W - 2; j++) g[j][i] = g[j + 1][i];
-            g[W - 2][i] = fresh[i];
-          }
-          const int pos = now - (W - 1);       // its gradient is complete
-          const bool before = pos < from;      // a row of the initial state, or a token of the block before
-          if (before && from != s.begin) continue;
-          if (before && a.dinitial_state == nullptr) continue;
-          if (a.dfinal_state != nullptr && pos >= s.end - (W - 1)) {
-            Pack<T, V> v;
-            load_some<T, V>(v, static_cast<const T*>(a.dfinal_state) + s.s * c.state_row + (long long)(pos - (s.end - (W - 1))) * a.D + channel,
-                            c.valid, c.wide);
-#pragma unroll
-            for (int i = 0; i < V; i++) out[i] += to_f32(v.v[i]);
-          }
-          Pack<T, V> v;
-#pragma unroll
-          for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
-          T* to_row = before ? static_cast<T*>(a.dinitial_state) + s.s * c.state_row + (long long)(W - 1 + pos - s.begin) * a.D + channel
-                             : dx + (long long)pos * a.D;
-          store_some<T, V>(to_row, v, c.valid, c.wide);
+          step(std::true_type(), in[u], d[u], out);
+          put(t + u - (W - 1), out);
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) { in[u] = next[u]; d[u] = nd[u]; }
+      }
+#pragma unroll 1
+      for (; t < to; t++) {
+        load(in[0], d[0], t);
+        step(std::true_type(), in[0], d[0], out);
+        put(t - (W - 1), out);
+      }
+#pragma unroll 1
+      for (; t < to + W - 1; t++) {   // tokens of the next block, and beyond the sequence, where there is no g
+        if (t < s.end) load(in[0], d[0], t);
+        else { zero_pack(in[0]); zero_pack(d[0]); }
+        step(std::false_type(), in[0], d[0], out);
+        put_edge(t - (W - 1), out);
       }
       from = to;
       if (from < t1) s = span_after(a, s);
@@ -293,7 +338,7 @@ int check_conv(const RewyConvArgs* a) {
   LAYER_REQUIRE(a->W >= 2 && a->W <= 4, REWY_ERR_UNSUPPORTED, "the convolution takes 2 to 4 taps");
   LAYER_REQUIRE(a->B > 0 && a->T > 0 && a->D > 0, REWY_ERR_SHAPE, "B, T and D must be positive");
   LAYER_REQUIRE((long long)a->B * a->T <= (1LL << 30) && a->D <= (1 << 24), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or D 2^24 channels");
-  LAYER_REQUIRE(((long long)a->B * a->T / 64 + a->B) * (a->D / 128 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more tokens and channels than one grid holds");
+  LAYER_REQUIRE(((long long)a->B * a->T / 64 + a->B) * (a->D / 64 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more tokens and channels than one grid holds");
   LAYER_REQUIRE(a->x != nullptr && a->weight != nullptr, REWY_ERR_NULL, "x or weight is NULL");
   LAYER_REQUIRE(a->cu_seqlens == nullptr || (a->B == 1 && a->num_seqs > 0), REWY_ERR_SHAPE, "packed sequences need B = 1 and num_seqs > 0");
   return REWY_OK;
@@ -336,7 +381,7 @@ extern "C" int rewy_conv_fwd(const RewyConvArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->y != nullptr, REWY_ERR_NULL, "y is NULL");
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = FWD_V;
     const ConvParams p = conv_params(*a, V, true);
     const unsigned grid = (unsigned)((long long)p.channel_blocks * p.token_blocks * a->B);
     with_taps(a->W, [&](auto w) { conv_fwd_kernel<T, w.value, V><<<grid, WARPS * 32, 0, (cudaStream_t)st>>>(p); });
@@ -348,7 +393,7 @@ extern "C" size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D,
   if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4) return 0;
   RewyConvArgs a{};
   a.B = B; a.T = T; a.D = D; a.W = W;
-  const ConvParams p = conv_params(a, 4, true);
+  const ConvParams p = conv_params(a, BWD_V, true);
   return (size_t)p.token_blocks * B * (W + 1) * D * sizeof(float);
 }
 
@@ -357,7 +402,7 @@ extern "C" int rewy_conv_bwd(const RewyConvArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->dy != nullptr && a->dx != nullptr && a->dweight != nullptr, REWY_ERR_NULL, "dy, dx or dweight is NULL");
   LAYER_REQUIRE(a->workspace != nullptr && a->workspace_bytes >= rewy_conv_bwd_workspace_bytes(a->B, a->T, a->D, a->W), REWY_ERR_WORKSPACE,
                 "the workspace of the convolution backward is too small");
-  constexpr int V = 4;
+  constexpr int V = BWD_V;
   const ConvParams p = conv_params(*a, V, true);
   const int parts = p.token_blocks * a->B;
   float* partial = static_cast<float*>(a->workspace);

@@ -14,13 +14,15 @@ namespace {
 
 constexpr int NT = 128, SLICE = 32, ROWS = 8;  // threads, value channels per CTA, state vectors per thread
 
-__device__ __forceinline__ float4 load_state(const float* p, int valid, bool wide) {
-  if (wide && valid >= 4) return *reinterpret_cast<const float4*>(p);
+template <bool WIDE>
+__device__ __forceinline__ float4 load_state(const float* p, int valid) {
+  if constexpr (WIDE) return valid > 0 ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
   return make_float4(valid > 0 ? p[0] : 0.f, valid > 1 ? p[1] : 0.f, valid > 2 ? p[2] : 0.f, valid > 3 ? p[3] : 0.f);
 }
-__device__ __forceinline__ void store_state(float* p, float4 x, int valid, bool wide) {
-  if (wide && valid >= 4) {
-    *reinterpret_cast<float4*>(p) = x;
+template <bool WIDE>
+__device__ __forceinline__ void store_state(float* p, float4 x, int valid) {
+  if constexpr (WIDE) {
+    if (valid > 0) *reinterpret_cast<float4*>(p) = x;
     return;
   }
   if (valid > 0) p[0] = x.x;
@@ -29,8 +31,9 @@ __device__ __forceinline__ void store_state(float* p, float4 x, int valid, bool 
   if (valid > 3) p[3] = x.w;
 }
 
-template <class T, bool V_FIRST>
-__global__ void __launch_bounds__(NT) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices, bool wide) {
+// WIDE: every row of the state starts on 16 bytes and holds whole groups of four
+template <class T, bool V_FIRST, bool WIDE>
+__global__ void __launch_bounds__(NT, 6) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices) {
   __shared__ float sk[NT], sq[NT], serase[NT], sdecay[NT], red[4][3], part[4][2][SLICE];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x % slices;
@@ -50,7 +53,7 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const __grid_constant__ 
   for (int i = 0; i < ROWS; i++) {
     const int r = V_FIRST ? v0 + r0 + 4 * i : r0 + 16 * i, c = V_FIRST ? c4 : v0 + c4;
     const int rows = V_FIRST ? a.V : a.K, cols = V_FIRST ? a.K : a.V;
-    S[i] = load_state(state + (long long)r * cols + c, r < rows ? cols - c : 0, wide);
+    S[i] = load_state<WIDE>(state + (long long)r * cols + c, r < rows ? cols - c : 0);
   }
   const long long qk = ((long long)b * a.H + hv / (a.HV / a.H)) * a.K;
   float q = 0.f, k = 0.f, erase = 1.f, decay = 1.f;
@@ -132,7 +135,7 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const __grid_constant__ 
       const int r = r0 + 16 * i;
       const float x = sk[r];
       S[i].x = fmaf(x, r4[0], S[i].x); S[i].y = fmaf(x, r4[1], S[i].y); S[i].z = fmaf(x, r4[2], S[i].z); S[i].w = fmaf(x, r4[3], S[i].w);
-      store_state(state + (long long)r * a.V + v0 + c4, S[i], r < a.K ? a.V - v0 - c4 : 0, wide);
+      store_state<WIDE>(state + (long long)r * a.V + v0 + c4, S[i], r < a.K ? a.V - v0 - c4 : 0);
     }
   } else {
     const float4 d = *reinterpret_cast<const float4*>(sdecay + c4), x = *reinterpret_cast<const float4*>(serase + c4),
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(NT) delta_step_kernel(const __grid_constant__ 
       const float r = beta * (target(v) - e);
       if (lane == 0 && v < a.V) o[v] = from_f32<T>(a.scale * fmaf(dot, r, p));
       S[i].x = fmaf(kx.x, r, S[i].x); S[i].y = fmaf(kx.y, r, S[i].y); S[i].z = fmaf(kx.z, r, S[i].z); S[i].w = fmaf(kx.w, r, S[i].w);
-      store_state(state + (long long)v * a.K + c4, S[i], v < a.V ? a.K - c4 : 0, wide);
+      store_state<WIDE>(state + (long long)v * a.K + c4, S[i], v < a.V ? a.K - c4 : 0);
     }
   }
 }
@@ -178,8 +181,11 @@ extern "C" int rewy_delta_step(const RewyDeltaStepArgs* a, rewy_stream_t st) {
   const unsigned grid = (unsigned)((long long)a->B * a->HV * slices);
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a->state_v_first) delta_step_kernel<T, true><<<grid, NT, 0, (cudaStream_t)st>>>(*a, slices, wide);
-    else delta_step_kernel<T, false><<<grid, NT, 0, (cudaStream_t)st>>>(*a, slices, wide);
+    const cudaStream_t s = (cudaStream_t)st;
+    if (a->state_v_first && wide) delta_step_kernel<T, true, true><<<grid, NT, 0, s>>>(*a, slices);
+    else if (a->state_v_first) delta_step_kernel<T, true, false><<<grid, NT, 0, s>>>(*a, slices);
+    else if (wide) delta_step_kernel<T, false, true><<<grid, NT, 0, s>>>(*a, slices);
+    else delta_step_kernel<T, false, false><<<grid, NT, 0, s>>>(*a, slices);
   });
   return launched("delta-rule step");
 }

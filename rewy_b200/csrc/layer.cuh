@@ -104,6 +104,48 @@ __device__ __forceinline__ float rcp_fast(float x) {  // 1 ulp
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two FP32 values in a register pair: one instruction for both
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ F2 both(float x) { return pair(x, x); }
+__device__ __forceinline__ float2 halves(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 neg2(F2 a) {
+  const float2 h = halves(a);
+  return pair(-h.x, -h.y);
+}
+__device__ __forceinline__ float sum_halves(F2 a) {
+  const float2 h = halves(a);
+  return h.x + h.y;
+}
+__device__ __forceinline__ F2 ex2_2(F2 a) {
+  const float2 h = halves(a);
+  return pair(ex2(h.x), ex2(h.y));
+}
 constexpr float LOG2E = 1.4426950408889634f;
 // 1 / (1 + e^-x): e^-x overflows to infinity and its reciprocal to 0 for very negative x, as the sigmoid does
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + ex2(-LOG2E * x)); }

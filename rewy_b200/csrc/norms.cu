@@ -55,9 +55,115 @@ __device__ __forceinline__ void row_sums(float (&x)[N], float* red, int parity) 
 
 template <int TPR, int NV>
 struct Layout {
-  static constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, RED = TPR > 32 ? 2 * THREADS / 32 * 2 : 1;
+  static constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, COLS = TPR * NV * E, RED = TPR > 32 ? 2 * THREADS / 32 * 2 : 1;
   __device__ static __forceinline__ int column(int v) { return (v * TPR + threadIdx.x % TPR) * E; }
 };
+
+// The rows that a CTA works on next, on their way through shared memory: every thread copies the elements that it will read
+// itself, so that no barrier stands between, and no registers hold what is under way.  Rows that do not fit twice are loaded
+// when they are needed.  Elements of TA stand in the first NA of the inputs, of TB in the others.
+template <class TA, int NA, class TB, int NB, int TPR, int NV>
+struct Stream {
+  using Y = Layout<TPR, NV>;
+  static constexpr int BYTES_A = NV * E * sizeof(TA), BYTES_B = NV * E * sizeof(TB), STAGE = Y::THREADS * (NA * BYTES_A + NB * BYTES_B);
+  static constexpr int ROOM = (220 * 1024 - Y::COLS * 8) / STAGE, WANT = STAGE <= 32 * 1024 ? 3 : 2, STAGES = ROOM >= WANT ? WANT : ROOM >= 2 ? 2 : 0;
+  static constexpr int BYTES = STAGES * STAGE;
+  const TA* a[NA];
+  const TB* b[NB > 0 ? NB : 1];
+  Pack<TA, E> pa[NA][NV];
+  Pack<TB, E> pb[NB > 0 ? NB : 1][NV];
+  unsigned char* smem;
+  bool wide;
+
+  template <class T>
+  __device__ __forceinline__ T* slot(int stage, int i, int v) const {
+    const int before = sizeof(T) == sizeof(TA) && i < NA ? i * BYTES_A : NA * BYTES_A + (i - NA) * BYTES_B;
+    return reinterpret_cast<T*>(smem + stage * STAGE + Y::THREADS * before) + (v * Y::THREADS + threadIdx.x) * E;
+  }
+  template <class T>
+  __device__ __forceinline__ void copy(T* to, const T* from, int valid) {
+    if (wide && valid >= E) {
+#pragma unroll
+      for (int i = 0; i < E * (int)sizeof(T) / 16; i++) {
+        const unsigned dst = (unsigned)__cvta_generic_to_shared(reinterpret_cast<uint4*>(to) + i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<const uint4*>(from) + i) : "memory");
+      }
+      return;
+    }
+    Pack<T, E> x;
+    load_some<T, E>(x, from, valid, false);
+    *reinterpret_cast<Pack<T, E>*>(to) = x;
+  }
+  // a[] and b[] point at the row; valid(v, i): how many elements of input i there are from column(v) on
+  template <class F>
+  __device__ __forceinline__ void ask(int stage, F&& valid) {
+    if constexpr (STAGES > 0) {
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int i = 0; i < NA; i++) copy(slot<TA>(stage, i, v), a[i] + Y::column(v), valid(v, i));
+#pragma unroll
+        for (int i = 0; i < NB; i++) copy(slot<TB>(stage, NA + i, v), b[i] + Y::column(v), valid(v, NA + i));
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void take(int stage, F&& valid) {
+    if constexpr (STAGES > 0) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int i = 0; i < NA; i++) pa[i][v] = *reinterpret_cast<const Pack<TA, E>*>(slot<TA>(stage, i, v));
+#pragma unroll
+        for (int i = 0; i < NB; i++) pb[i][v] = *reinterpret_cast<const Pack<TB, E>*>(slot<TB>(stage, NA + i, v));
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int i = 0; i < NA; i++) load_some<TA, E>(pa[i][v], a[i] + Y::column(v), valid(v, i), wide);
+#pragma unroll
+        for (int i = 0; i < NB; i++) load_some<TB, E>(pb[i][v], b[i] + Y::column(v), valid(v, NA + i), wide);
+      }
+    }
+  }
+};
+
+// Calls work(r, real, parity) for each row of this thread's, its elements in `in`; point(r) sets the inputs' addresses, with(i)
+// says whether there is an input i at all.
+template <int TPR, int NV, class In, class Point, class With, class Work>
+__device__ __forceinline__ void for_rows(In& in, long long rows, int D, Point&& point, With&& with, Work&& work) {
+  using Y = Layout<TPR, NV>;
+  const long long stride = (long long)gridDim.x * Y::ROWS, first = (long long)blockIdx.x * Y::ROWS;
+  const int mine = threadIdx.x / TPR;
+  auto ask = [&](long long base, int stage) {
+    const long long r = base + mine;
+    const bool real = r < rows;
+    point(real ? r : 0);
+    in.ask(stage, [&](int v, int i) { return real && with(i) ? D - Y::column(v) : 0; });
+  };
+  if constexpr (In::STAGES > 0)
+#pragma unroll
+    for (int k = 0; k < In::STAGES - 1; k++) ask(first + k * stride, k);
+  int stage = 0, parity = 0;
+  for (long long base = first; base < rows; base += stride, parity ^= 1) {
+    const long long r = base + mine;
+    const bool real = r < rows;
+    if constexpr (In::STAGES > 0) {
+      const int ahead = stage == 0 ? In::STAGES - 1 : stage - 1;
+      ask(base + (In::STAGES - 1) * stride, ahead);
+    } else {
+      point(real ? r : 0);
+    }
+    in.take(stage, [&](int v, int i) { return real && with(i) ? D - Y::column(v) : 0; });
+    work(r, real, parity);
+    if constexpr (In::STAGES > 0) stage = stage == In::STAGES - 1 ? 0 : stage + 1;
+  }
+  if constexpr (In::STAGES > 0) asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // The CTA's sums per column: over its rows' threads in shared memory, then to `to`.
 template <int TPR, int NV>
 __device__ __forceinline__ void store_column_sums(float (&x)[NV][E], float* sums, float* to, int D) {
@@ -73,262 +179,272 @@ __device__ __forceinline__ void store_column_sums(float (&x)[NV][E], float* sums
 #pragma unroll
     for (int v = 0; v < NV; v++)
 #pragma unroll
-      for (int e = 0; e < E; e++) sums[threadIdx.x / TPR * (TPR * NV * E) + Y::column(v) + e] = x[v][e];
+      for (int e = 0; e < E; e++) sums[threadIdx.x / TPR * Y::COLS + Y::column(v) + e] = x[v][e];
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += Y::THREADS) {
       float s = 0.f;
 #pragma unroll
-      for (int r = 0; r < Y::ROWS; r++) s += sums[r * (TPR * NV * E) + c];
+      for (int r = 0; r < Y::ROWS; r++) s += sums[r * Y::COLS + c];
       to[c] = s;
     }
   }
 }
+// A parameter per column as FP32 in shared memory
 template <int TPR, int NV>
-__device__ __forceinline__ void load_params(float (&w)[NV][E], const void* p, int dtype, int D, float otherwise) {
-#pragma unroll
-  for (int v = 0; v < NV; v++)
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int c = Layout<TPR, NV>::column(v) + e;
-      w[v][e] = c >= D ? 0.f : p == nullptr ? otherwise : param_at(p, dtype, c);
-    }
+__device__ __forceinline__ void load_params(float* w, const void* p, int dtype, int D, float otherwise) {
+  for (int c = threadIdx.x; c < Layout<TPR, NV>::COLS; c += Layout<TPR, NV>::THREADS) w[c] = c >= D ? 0.f : p == nullptr ? otherwise : param_at(p, dtype, c);
+}
+__device__ __forceinline__ void read8(float (&x)[E], const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <int N>
+__device__ __forceinline__ float act_of(float g, int activation, float& slope) {
+  const float sig = sigmoid_fast(g);
+  if constexpr (N > 0) slope = activation == 0 ? sig * fmaf(g, 1.f - sig, 1.f) : sig * (1.f - sig);
+  return activation == 0 ? g * sig : sig;
 }
 
+// CTAs on an SM that the registers are cut for
+template <class T, int TPR, int NV, bool BACKWARD>
+constexpr int resident() {
+  constexpr int threads = Layout<TPR, NV>::THREADS, most = sizeof(T) == 4 ? 512 : BACKWARD ? 768 : 1024;
+  return most > threads ? most / threads : 1;
+}
 template <class T, int TPR, int NV>
-__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS) gated_fwd_kernel(const __grid_constant__ NormParams p) {
+using GatedFwd = Stream<T, 2, T, 0, TPR, NV>;
+template <class T, int TPR, int NV>
+using GatedBwd = Stream<T, 3, T, 0, TPR, NV>;
+template <class T, class TR, int TPR, int NV>
+using ResidualFwd = Stream<T, 1, TR, 1, TPR, NV>;
+template <class T, class TR, int TPR, int NV>
+using ResidualBwd = Stream<T, 2, TR, 2, TPR, NV>;
+
+template <class T, int TPR, int NV>
+__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV, false>()) gated_fwd_kernel(const __grid_constant__ NormParams p) {
   using Y = Layout<TPR, NV>;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float red[Y::RED];
   const RewyNormArgs& a = p.a;
-  float w[NV][E];
+  float* const w = reinterpret_cast<float*>(smem + GatedFwd<T, TPR, NV>::BYTES);
   load_params<TPR, NV>(w, a.weight, a.param_dtype, a.D, 1.f);
-  int parity = 0;
-  for (long long base = (long long)blockIdx.x * Y::ROWS; base < a.rows; base += (long long)gridDim.x * Y::ROWS, parity ^= 1) {
-    const long long r = base + threadIdx.x / TPR;
-    const bool real = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (real ? row_start(r, a.x_inner, a.x_stride) : 0);
-    const T* g = static_cast<const T*>(a.gate) + (real ? row_start(r, a.other_inner, a.other_stride) : 0);
-    Pack<T, E> px[NV], pg[NV];
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v), valid = real ? a.D - c : 0;
-      load_some<T, E>(px[v], x + c, valid, p.wide);
-      load_some<T, E>(pg[v], g + c, valid, p.wide);
-    }
-    float sum[1] = {0.f};
+  __syncthreads();
+  GatedFwd<T, TPR, NV> in;
+  in.smem = smem; in.wide = p.wide;
+  auto point = [&](long long r) {
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
+    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.other_stride);
+  };
+  for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
+    float t[NV][E], sum[1] = {0.f}, slope;   // what is normalised, times what stands behind the norm
 #pragma unroll
     for (int v = 0; v < NV; v++)
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        float t = to_f32(px[v].v[e]);
-        if (a.gate_first && Y::column(v) + e < a.D) {
-          const float gv = to_f32(pg[v].v[e]), sig = sigmoid_fast(gv);
-          t *= a.activation == 0 ? gv * sig : sig;
-        }
-        sum[0] = fmaf(t, t, sum[0]);
+        const float x = to_f32(in.pa[0][v].v[e]), act = act_of<0>(to_f32(in.pa[1][v].v[e]), a.activation, slope);
+        t[v][e] = x * act;
+        const float n = a.gate_first ? t[v][e] : x;
+        sum[0] = fmaf(n, n, sum[0]);       // elements that do not exist are zero
       }
     row_sums<TPR>(sum, red, parity);
     const float rs = rsqrtf(sum[0] / a.D + a.eps);
-    if (!real) continue;
+    if (!real) return;
     T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
+      if (c >= a.D) continue;
+      float wv[E];
+      read8(wv, w + c);
       Pack<T, E> out;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float gv = to_f32(pg[v].v[e]), sig = sigmoid_fast(gv);
-        out.v[e] = from_f32<T>(to_f32(px[v].v[e]) * rs * w[v][e] * (a.activation == 0 ? gv * sig : sig));
-      }
-      if (c < a.D) store_some<T, E>(y + c, out, a.D - c, p.wide);
+      for (int e = 0; e < E; e++) out.v[e] = from_f32<T>(t[v][e] * rs * wv[e]);
+      store_some<T, E>(y + c, out, a.D - c, p.wide);
     }
-  }
+  });
 }
 
 template <class T, int TPR, int NV>
-__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS) gated_bwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV, true>()) gated_bwd_kernel(const __grid_constant__ NormParams p) {
   using Y = Layout<TPR, NV>;
-  __shared__ float red[Y::RED], sums[Y::ROWS > 1 ? Y::ROWS * TPR * NV * E : 1];
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float red[Y::RED];
   const RewyNormArgs& a = p.a;
-  float w[NV][E], dw[NV][E] = {};
+  float* const w = reinterpret_cast<float*>(smem + GatedBwd<T, TPR, NV>::BYTES);
   load_params<TPR, NV>(w, a.weight, a.param_dtype, a.D, 1.f);
-  int parity = 0;
-  for (long long base = (long long)blockIdx.x * Y::ROWS; base < a.rows; base += (long long)gridDim.x * Y::ROWS, parity ^= 1) {
-    const long long r = base + threadIdx.x / TPR;
-    const bool real = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (real ? row_start(r, a.x_inner, a.x_stride) : 0);
-    const T* g = static_cast<const T*>(a.gate) + (real ? row_start(r, a.other_inner, a.other_stride) : 0);
-    const T* dy = static_cast<const T*>(a.dy) + (real ? r * a.D : 0);
-    Pack<T, E> px[NV], pg[NV], pd[NV];
+  __syncthreads();
+  float dw[NV][E] = {};
+  GatedBwd<T, TPR, NV> in;
+  in.smem = smem; in.wide = p.wide;
+  auto point = [&](long long r) {
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
+    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.other_stride);
+    in.a[2] = static_cast<const T*>(a.dy) + r * a.D;
+  };
+  for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
+    float sum[2] = {0.f, 0.f}, slope;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v), valid = real ? a.D - c : 0;
-      load_some<T, E>(px[v], x + c, valid, p.wide);
-      load_some<T, E>(pg[v], g + c, valid, p.wide);
-      load_some<T, E>(pd[v], dy + c, valid, p.wide);
-    }
-    auto gate = [&](int v, int e, float& act, float& slope) {
-      const float gv = to_f32(pg[v].v[e]), sig = sigmoid_fast(gv);
-      act = a.activation == 0 ? gv * sig : sig;
-      slope = a.activation == 0 ? sig * fmaf(gv, 1.f - sig, 1.f) : sig * (1.f - sig);
-    };
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int v = 0; v < NV; v++)
+      float wv[E];
+      read8(wv, w + Y::column(v));
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (Y::column(v) + e >= a.D) continue;
-        float act, slope;
-        gate(v, e, act, slope);
-        const float xv = to_f32(px[v].v[e]), t = a.gate_first ? xv * act : xv;
-        const float dn = to_f32(pd[v].v[e]) * w[v][e] * (a.gate_first ? 1.f : act);
+        const float x = to_f32(in.pa[0][v].v[e]), act = act_of<0>(to_f32(in.pa[1][v].v[e]), a.activation, slope), dn = to_f32(in.pa[2][v].v[e]) * wv[e];
+        const float t = a.gate_first ? x * act : x;
         sum[0] = fmaf(t, t, sum[0]);
-        sum[1] = fmaf(dn, t, sum[1]);
+        sum[1] = fmaf(dn * act, x, sum[1]);    // dn t either way
       }
+    }
     row_sums<TPR>(sum, red, parity);
-    if (!real) continue;
+    if (!real) return;
     const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
       if (c >= a.D) continue;
+      float wv[E];
+      read8(wv, w + c);
       Pack<T, E> ox, og;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        float act, slope;
-        gate(v, e, act, slope);
-        const float xv = to_f32(px[v].v[e]), d = to_f32(pd[v].v[e]);
-        if (c + e >= a.D) continue;
-        if (a.gate_first) {
-          const float t = xv * act, dv = fmaf(rs, d * w[v][e], -back * t);
-          ox.v[e] = from_f32<T>(dv * act);
-          og.v[e] = from_f32<T>(dv * xv * slope);
-          dw[v][e] = fmaf(d, t * rs, dw[v][e]);
-        } else {
-          const float n = xv * rs, dn = d * w[v][e];
-          ox.v[e] = from_f32<T>(fmaf(rs, dn * act, -back * xv));
-          og.v[e] = from_f32<T>(dn * n * slope);
-          dw[v][e] = fmaf(d, n * act, dw[v][e]);
-        }
+        const float act = act_of<1>(to_f32(in.pa[1][v].v[e]), a.activation, slope);
+        const float xv = to_f32(in.pa[0][v].v[e]), d = to_f32(in.pa[2][v].v[e]), dn = d * wv[e];
+        // gate first: v = x act, dx = dv act, dgate = dv x act'.  Else dgate = dn n act', dx = r dn act - back x
+        const float dv = a.gate_first ? fmaf(rs, dn, -back * (xv * act)) : rs * dn;
+        ox.v[e] = from_f32<T>(a.gate_first ? dv * act : fmaf(dv, act, -back * xv));
+        og.v[e] = from_f32<T>(dv * xv * slope);
+        dw[v][e] = fmaf(d, xv * act * rs, dw[v][e]);
       }
       store_some<T, E>(static_cast<T*>(a.dx) + r * a.D + c, ox, a.D - c, p.wide);
       store_some<T, E>(static_cast<T*>(a.dgate) + r * a.D + c, og, a.D - c, p.wide);
     }
-  }
-  store_column_sums<TPR, NV>(dw, sums, p.partial + (long long)blockIdx.x * 2 * a.D, a.D);
+  });
+  store_column_sums<TPR, NV>(dw, reinterpret_cast<float*>(smem), p.partial + (long long)blockIdx.x * 2 * a.D, a.D);
 }
 
 template <class T, class TR, int TPR, int NV>
-__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS) residual_fwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV, false>()) residual_fwd_kernel(const __grid_constant__ NormParams p) {
   using Y = Layout<TPR, NV>;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float red[Y::RED];
   const RewyNormArgs& a = p.a;
-  float w[NV][E], s[NV][E];
+  float* const w = reinterpret_cast<float*>(smem + ResidualFwd<T, TR, TPR, NV>::BYTES);
+  float* const s = w + Y::COLS;
   load_params<TPR, NV>(w, a.weight, a.param_dtype, a.D, 1.f);
   load_params<TPR, NV>(s, a.scale_vector, a.scale_dtype, a.D, a.scale);
-  int parity = 0;
-  for (long long base = (long long)blockIdx.x * Y::ROWS; base < a.rows; base += (long long)gridDim.x * Y::ROWS, parity ^= 1) {
-    const long long r = base + threadIdx.x / TPR;
-    const bool real = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (real ? row_start(r, a.x_inner, a.x_stride) : 0);
-    const TR* res = static_cast<const TR*>(a.residual) + (real && a.residual != nullptr ? row_start(r, a.other_inner, a.other_stride) : 0);
+  __syncthreads();
+  ResidualFwd<T, TR, TPR, NV> in;
+  in.smem = smem; in.wide = p.wide;
+  const bool has = a.residual != nullptr;
+  auto point = [&](long long r) {
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
+    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.other_stride) : 0);
+  };
+  for_rows<TPR, NV>(in, a.rows, a.D, point, [&](int i) { return i == 0 || has; }, [&](long long r, bool real, int parity) {
     float t[NV][E], sum[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v), valid = real ? a.D - c : 0;
-      Pack<T, E> px;
-      Pack<TR, E> pr;
-      load_some<T, E>(px, x + c, valid, p.wide);
-      load_some<TR, E>(pr, res + c, a.residual != nullptr ? valid : 0, p.wide);
+      float sv[E];
+      read8(sv, s + Y::column(v));
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        t[v][e] = fmaf(s[v][e], to_f32(px.v[e]), to_f32(pr.v[e]));
-        if (c + e < a.D) sum[0] = fmaf(t[v][e], t[v][e], sum[0]);
+        t[v][e] = fmaf(sv[e], to_f32(in.pa[0][v].v[e]), to_f32(in.pb[0][v].v[e]));
+        sum[0] = fmaf(t[v][e], t[v][e], sum[0]);
       }
     }
     row_sums<TPR>(sum, red, parity);
-    if (!real) continue;
+    if (!real) return;
     const float rs = rsqrtf(sum[0] / a.D + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
       if (c >= a.D) continue;
+      float wv[E];
+      read8(wv, w + c);
       Pack<T, E> oy;
       Pack<TR, E> orr;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        oy.v[e] = from_f32<T>(t[v][e] * rs * w[v][e]);
+        oy.v[e] = from_f32<T>(t[v][e] * rs * wv[e]);
         orr.v[e] = from_f32<TR>(t[v][e]);
       }
       store_some<T, E>(static_cast<T*>(a.y) + r * a.D + c, oy, a.D - c, p.wide);
       store_some<TR, E>(static_cast<TR*>(a.residual_out) + r * a.D + c, orr, a.D - c, p.wide);
     }
-  }
+  });
 }
 
 // SCALE: the scale is a vector that has a gradient
 template <class T, class TR, int TPR, int NV, bool SCALE>
-__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS) residual_bwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV, true>()) residual_bwd_kernel(const __grid_constant__ NormParams p) {
   using Y = Layout<TPR, NV>;
-  __shared__ float red[Y::RED], sums[Y::ROWS > 1 ? Y::ROWS * TPR * NV * E : 1];
+  using In = ResidualBwd<T, TR, TPR, NV>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float red[Y::RED];
   const RewyNormArgs& a = p.a;
-  float w[NV][E], s[SCALE ? NV : 1][E], dw[NV][E] = {}, ds[SCALE ? NV : 1][E] = {};
+  float* const w = reinterpret_cast<float*>(smem + In::BYTES);
+  float* const s = w + Y::COLS;
   load_params<TPR, NV>(w, a.weight, a.param_dtype, a.D, 1.f);
-  if constexpr (SCALE) load_params<TPR, NV>(s, a.scale_vector, a.scale_dtype, a.D, a.scale);
-  int parity = 0;
-  for (long long base = (long long)blockIdx.x * Y::ROWS; base < a.rows; base += (long long)gridDim.x * Y::ROWS, parity ^= 1) {
-    const long long r = base + threadIdx.x / TPR;
-    const bool real = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (real ? row_start(r, a.x_inner, a.x_stride) : 0);
-    const TR* res = static_cast<const TR*>(a.residual) + (real && a.residual != nullptr ? row_start(r, a.other_inner, a.other_stride) : 0);
-    const T* dy = static_cast<const T*>(a.dy) + (real ? r * a.D : 0);
-    const TR* dro = static_cast<const TR*>(a.dresidual_out) + (real && a.dresidual_out != nullptr ? r * a.D : 0);
-    Pack<T, E> px[NV], pd[NV];
-    Pack<TR, E> pr[NV], po[NV];
+  if (SCALE) load_params<TPR, NV>(s, a.scale_vector, a.scale_dtype, a.D, a.scale);
+  __syncthreads();
+  float dw[NV][E] = {}, ds[SCALE ? NV : 1][E] = {};
+  In in;
+  in.smem = smem; in.wide = p.wide;
+  const bool has = a.residual != nullptr, back_too = a.dresidual_out != nullptr;
+  auto point = [&](long long r) {
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
+    in.a[1] = static_cast<const T*>(a.dy) + r * a.D;
+    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.other_stride) : 0);
+    in.b[1] = static_cast<const TR*>(a.dresidual_out) + (back_too ? r * a.D : 0);
+  };
+  auto scales = [&](float(&sv)[E], int v) {
+    if constexpr (SCALE) read8(sv, s + Y::column(v));
+    else
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v), valid = real ? a.D - c : 0;
-      load_some<T, E>(px[v], x + c, valid, p.wide);
-      load_some<TR, E>(pr[v], res + c, a.residual != nullptr ? valid : 0, p.wide);
-      load_some<T, E>(pd[v], dy + c, valid, p.wide);
-      load_some<TR, E>(po[v], dro + c, a.dresidual_out != nullptr ? valid : 0, p.wide);
-    }
-    auto scale = [&](int v, int e) { return SCALE ? s[SCALE ? v : 0][e] : a.scale; };
+      for (int e = 0; e < E; e++) sv[e] = a.scale;
+  };
+  for_rows<TPR, NV>(in, a.rows, a.D, point, [&](int i) { return i < 2 || (i == 2 ? has : back_too); }, [&](long long r, bool real, int parity) {
     float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+    for (int v = 0; v < NV; v++) {
+      float wv[E], sv[E];
+      read8(wv, w + Y::column(v));
+      scales(sv, v);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (Y::column(v) + e >= a.D) continue;
-        const float t = fmaf(scale(v, e), to_f32(px[v].v[e]), to_f32(pr[v].v[e]));
+        const float t = fmaf(sv[e], to_f32(in.pa[0][v].v[e]), to_f32(in.pb[0][v].v[e]));
         sum[0] = fmaf(t, t, sum[0]);
-        sum[1] = fmaf(to_f32(pd[v].v[e]) * w[v][e], t, sum[1]);
+        sum[1] = fmaf(to_f32(in.pa[1][v].v[e]) * wv[e], t, sum[1]);
       }
+    }
     row_sums<TPR>(sum, red, parity);
-    if (!real) continue;
+    if (!real) return;
     const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
       if (c >= a.D) continue;
+      float wv[E], sv[E];
+      read8(wv, w + c);
+      scales(sv, v);
       Pack<T, E> ox;
       Pack<TR, E> orr;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (c + e >= a.D) continue;
-        const float xv = to_f32(px[v].v[e]), t = fmaf(scale(v, e), xv, to_f32(pr[v].v[e])), d = to_f32(pd[v].v[e]);
-        const float dt = to_f32(po[v].v[e]) + fmaf(rs, d * w[v][e], -back * t);
-        ox.v[e] = from_f32<T>(scale(v, e) * dt);
+        const float xv = to_f32(in.pa[0][v].v[e]), t = fmaf(sv[e], xv, to_f32(in.pb[0][v].v[e])), d = to_f32(in.pa[1][v].v[e]);
+        const float dt = to_f32(in.pb[1][v].v[e]) + fmaf(rs, d * wv[e], -back * t);
+        ox.v[e] = from_f32<T>(sv[e] * dt);
         orr.v[e] = from_f32<TR>(dt);
         dw[v][e] = fmaf(d, t * rs, dw[v][e]);
         if constexpr (SCALE) ds[v][e] = fmaf(xv, dt, ds[v][e]);
       }
       store_some<T, E>(static_cast<T*>(a.dx) + r * a.D + c, ox, a.D - c, p.wide);
-      if (a.dresidual != nullptr) store_some<TR, E>(static_cast<TR*>(a.dresidual) + r * a.D + c, orr, a.D - c, p.wide);
+      if (has) store_some<TR, E>(static_cast<TR*>(a.dresidual) + r * a.D + c, orr, a.D - c, p.wide);
     }
-  }
+  });
   float* to = p.partial + (long long)blockIdx.x * 2 * a.D;
-  store_column_sums<TPR, NV>(dw, sums, to, a.D);
-  if constexpr (SCALE) store_column_sums<TPR, NV>(ds, sums, to + a.D, a.D);
+  store_column_sums<TPR, NV>(dw, reinterpret_cast<float*>(smem), to, a.D);
+  if constexpr (SCALE) store_column_sums<TPR, NV>(ds, reinterpret_cast<float*>(smem), to + a.D, a.D);
 }
 
 // Gradients per column from the CTAs' sums [parts][2][D]: 32 threads per column, blockIdx.y chooses the first or second sum.
@@ -360,8 +476,9 @@ void with_layout(int D, F&& f) {
   if (D <= 128) f(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (D <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
   else if (D <= 1024) f(integral_constant<int, 128>(), integral_constant<int, 1>());
-  else if (D <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
-  else if (D <= 8192) f(integral_constant<int, 512>(), integral_constant<int, 2>());
+  else if (D <= 2048) f(integral_constant<int, 256>(), integral_constant<int, 1>());
+  else if (D <= 4096) f(integral_constant<int, 512>(), integral_constant<int, 1>());
+  else if (D <= 8192) f(integral_constant<int, 1024>(), integral_constant<int, 1>());
   else f(integral_constant<int, 1024>(), integral_constant<int, 2>());
 }
 template <class F>
@@ -371,12 +488,13 @@ void with_residual_type(int dtype, int residual_dtype, F&& f) {
     else f(t, float());
   });
 }
-int rows_per_cta(int D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 1024 ? 2 : 1; }
-int grid_of(int64_t rows, int D, int per_sm) {
-  const int64_t ctas = (rows + rows_per_cta(D) - 1) / rows_per_cta(D), most = 148ll * per_sm;
+int rows_per_cta(int D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 1024 ? 2 : 1; }  // as with_layout chooses
+int threads_per_cta(int D) { return D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+int grid_of(int64_t rows, int D, int threads_per_sm) {
+  const int64_t ctas = (rows + rows_per_cta(D) - 1) / rows_per_cta(D), each = threads_per_sm / threads_per_cta(D), most = 148 * (each > 0 ? each : 1);
   return (int)(ctas < most ? ctas : most);
 }
-constexpr int FWD_PER_SM = 8, BWD_PER_SM = 3;
+constexpr int FWD_PER_SM = 1024, BWD_PER_SM = 768;  // threads
 
 int check_norm(const RewyNormArgs* a) {
   LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
@@ -400,6 +518,13 @@ NormParams norm_params(const RewyNormArgs& a) {
   p.wide = w;
   return p;
 }
+template <auto Kern>
+cudaError_t launch(const NormParams& p, int grid, int threads, int smem, rewy_stream_t st) {
+  const cudaError_t e = ensure_dynamic_smem<Kern>(smem);
+  if (e == cudaSuccess) Kern<<<grid, threads, smem, (cudaStream_t)st>>>(p);
+  return e;
+}
+int done(cudaError_t e, const char* what, int launches) { return e == cudaSuccess ? launched(what, launches) : report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e)); }
 int check_backward(const RewyNormArgs* a) {
   LAYER_REQUIRE(a->dy != nullptr && a->dx != nullptr && a->dweight != nullptr, REWY_ERR_NULL, "dy, dx or dweight is NULL");
   LAYER_REQUIRE(a->workspace != nullptr && a->workspace_bytes >= rewy_norm_bwd_workspace_bytes(a->rows, a->D), REWY_ERR_WORKSPACE,
@@ -426,13 +551,15 @@ extern "C" int rewy_gated_norm_fwd(const RewyNormArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->gate != nullptr && a->y != nullptr, REWY_ERR_NULL, "gate or y is NULL");
   const NormParams p = norm_params(*a);
   const int grid = grid_of(a->rows, a->D, FWD_PER_SM);
+  cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     with_layout(a->D, [&](auto tpr, auto nv) {
+      using T = decltype(t);
       using Y = Layout<tpr.value, nv.value>;
-      gated_fwd_kernel<decltype(t), tpr.value, nv.value><<<grid, Y::THREADS, 0, (cudaStream_t)st>>>(p);
+      e = launch<gated_fwd_kernel<T, tpr.value, nv.value>>(p, grid, Y::THREADS, GatedFwd<T, tpr.value, nv.value>::BYTES + Y::COLS * 4, st);
     });
   });
-  return launched("gated norm forward");
+  return done(e, "gated norm forward", 1);
 }
 
 extern "C" int rewy_gated_norm_bwd(const RewyNormArgs* a, rewy_stream_t st) {
@@ -441,14 +568,16 @@ extern "C" int rewy_gated_norm_bwd(const RewyNormArgs* a, rewy_stream_t st) {
   if (const int rc = check_backward(a)) return rc;
   const NormParams p = norm_params(*a);
   const int grid = grid_of(a->rows, a->D, BWD_PER_SM);
+  cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     with_layout(a->D, [&](auto tpr, auto nv) {
+      using T = decltype(t);
       using Y = Layout<tpr.value, nv.value>;
-      gated_bwd_kernel<decltype(t), tpr.value, nv.value><<<grid, Y::THREADS, 0, (cudaStream_t)st>>>(p);
+      e = launch<gated_bwd_kernel<T, tpr.value, nv.value>>(p, grid, Y::THREADS, GatedBwd<T, tpr.value, nv.value>::BYTES + Y::COLS * 4, st);
     });
   });
-  sum_columns(p, grid, false, (cudaStream_t)st);
-  return launched("gated norm backward", 2);
+  if (e == cudaSuccess) sum_columns(p, grid, false, (cudaStream_t)st);
+  return done(e, "gated norm backward", 2);
 }
 
 extern "C" int rewy_residual_norm_fwd(const RewyNormArgs* a, rewy_stream_t st) {
@@ -456,13 +585,16 @@ extern "C" int rewy_residual_norm_fwd(const RewyNormArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->residual_out != nullptr && a->y != nullptr, REWY_ERR_NULL, "residual_out or y is NULL");
   const NormParams p = norm_params(*a);
   const int grid = grid_of(a->rows, a->D, FWD_PER_SM);
+  cudaError_t e = cudaSuccess;
   with_residual_type(a->dtype, a->residual_dtype, [&](auto t, auto tr) {
     with_layout(a->D, [&](auto tpr, auto nv) {
+      using T = decltype(t);
+      using TR = decltype(tr);
       using Y = Layout<tpr.value, nv.value>;
-      residual_fwd_kernel<decltype(t), decltype(tr), tpr.value, nv.value><<<grid, Y::THREADS, 0, (cudaStream_t)st>>>(p);
+      e = launch<residual_fwd_kernel<T, TR, tpr.value, nv.value>>(p, grid, Y::THREADS, ResidualFwd<T, TR, tpr.value, nv.value>::BYTES + Y::COLS * 8, st);
     });
   });
-  return launched("residual norm forward");
+  return done(e, "residual norm forward", 1);
 }
 
 extern "C" int rewy_residual_norm_bwd(const RewyNormArgs* a, rewy_stream_t st) {
@@ -472,15 +604,17 @@ extern "C" int rewy_residual_norm_bwd(const RewyNormArgs* a, rewy_stream_t st) {
   if (const int rc = check_backward(a)) return rc;
   const NormParams p = norm_params(*a);
   const int grid = grid_of(a->rows, a->D, BWD_PER_SM);
+  cudaError_t e = cudaSuccess;
   with_residual_type(a->dtype, a->residual_dtype, [&](auto t, auto tr) {
     with_layout(a->D, [&](auto tpr, auto nv) {
+      using T = decltype(t);
+      using TR = decltype(tr);
       using Y = Layout<tpr.value, nv.value>;
-      if (a->scale_vector != nullptr)
-        residual_bwd_kernel<decltype(t), decltype(tr), tpr.value, nv.value, true><<<grid, Y::THREADS, 0, (cudaStream_t)st>>>(p);
-      else
-        residual_bwd_kernel<decltype(t), decltype(tr), tpr.value, nv.value, false><<<grid, Y::THREADS, 0, (cudaStream_t)st>>>(p);
+      constexpr int bytes = ResidualBwd<T, TR, tpr.value, nv.value>::BYTES + Y::COLS * 8;
+      if (a->scale_vector != nullptr) e = launch<residual_bwd_kernel<T, TR, tpr.value, nv.value, true>>(p, grid, Y::THREADS, bytes, st);
+      else e = launch<residual_bwd_kernel<T, TR, tpr.value, nv.value, false>>(p, grid, Y::THREADS, bytes, st);
     });
   });
-  sum_columns(p, grid, a->scale_vector != nullptr, (cudaStream_t)st);
-  return launched("residual norm backward", 2);
+  if (e == cudaSuccess) sum_columns(p, grid, a->scale_vector != nullptr, (cudaStream_t)st);
+  return done(e, "residual norm backward", 2);
 }

@@ -124,11 +124,22 @@ __device__ __forceinline__ void put_sums(float* at, int stride, const float (&x)
   }
 }
 
-// Sums of v over the warp's 32 / L channels (lanes that differ in the bits from L up); values are handed out on the way.  Calls
-// put(value index, sum) for those the lane ends with.
+// Sums of v (dB and dC of a thread's four states) over the warp's 32 / L channels, the lanes that differ in the bits from L up.
+// Each exchange halves the values that a lane is left with; it puts them at places i of a row of [dB | dC] counted from
+// sum_place, where `put` gets them.
+template <int L>
+__device__ __forceinline__ int sum_place(int lane, int n0) {
+  constexpr int NP = S * L;
+  int base = 0, n = 8;
+#pragma unroll
+  for (int m = 16; m >= L && n > 1; m >>= 1) {
+    n >>= 1;
+    base += lane & m ? n : 0;
+  }
+  return (base >> 2) * NP + n0 + (base & 3);
+}
 template <int L, class F>
 __device__ __forceinline__ void sum_channels(float (&v)[8], int lane, F&& put) {
-  int base = 0;
   int n = 8;
 #pragma unroll
   for (int m = 16; m >= L; m >>= 1) {
@@ -141,14 +152,13 @@ __device__ __forceinline__ void sum_channels(float (&v)[8], int lane, F&& put) {
           const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
           v[i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
         }
-      base += up ? n : 0;
     } else {
       v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (i < n) put(base + i, v[i]);
+  for (int i = 0; i < 4; i++)   // n <= 4: the values lie in one half of the row
+    if (i < n) put(i, v[i]);
 }
 
 // A tile's rows of one [B,T,M] tensor: 8 channels per access.
@@ -236,6 +246,7 @@ __global__ void __launch_bounds__(NT) scan_fwd_kernel(const __grid_constant__ Sc
   load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
+  const F2 A01 = pair(A2[0], A2[1]), A23 = pair(A2[2], A2[3]);
 
   Sequence q;
   q.at(a, at.b, at.t0);
@@ -283,43 +294,43 @@ __global__ void __launch_bounds__(NT) scan_fwd_kernel(const __grid_constant__ Sc
     const bool more = t0 + TT < at.t1;
     if (more) fetch(nu, nd, nz, t0 + TT);
     __syncthreads();
-#pragma unroll 2
-    for (int k = 0; k < TT; k += 4) {
+    // CHECK: a sequence may begin inside the tile
+    auto tokens = [&](auto check, int k) {
       if (!STATE_ONLY && k % CK == 0 && a.checkpoints != nullptr && t0 + k < a.T)
         store4(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + k) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
       float y[4];
-      auto token = [&](int j) {
-        const float d = sdt[(k + j) * CH + ch], x = sdu[(k + j) * CH + ch];
-        const float4 Bv = *reinterpret_cast<const float4*>(sB + (k + j) * NP + n0);
-        h[0] = fmaf(ex2(d * A2[0]), h[0], x * Bv.x);
-        h[1] = fmaf(ex2(d * A2[1]), h[1], x * Bv.y);
-        h[2] = fmaf(ex2(d * A2[2]), h[2], x * Bv.z);
-        h[3] = fmaf(ex2(d * A2[3]), h[3], x * Bv.w);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (check.value && t0 + k + j == q.next && t0 + k + j < at.t1) {
+          finish(q.s);
+          q.advance(a);
+          start(q.s);
+        }
+        const float d = sdt[(k + j) * CH + ch];
+        const F2 dd = both(d), x = both(sdu[(k + j) * CH + ch]);
+        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k + j) * NP + n0);
+        const F2 h01 = fma2(ex2_2(mul2(dd, A01)), pair(h[0], h[1]), mul2(x, F2{Bv.x}));
+        const F2 h23 = fma2(ex2_2(mul2(dd, A23)), pair(h[2], h[3]), mul2(x, F2{Bv.y}));
+        const float2 u01 = halves(h01), u23 = halves(h23);
+        h[0] = u01.x; h[1] = u01.y; h[2] = u23.x; h[3] = u23.y;
         if constexpr (STATE_ONLY) {
           total += d;
         } else {
-          const float4 Cv = *reinterpret_cast<const float4*>(sC + (k + j) * NP + n0);
-          y[j] = fmaf(Cv.x, h[0], Cv.y * h[1]) + fmaf(Cv.z, h[2], Cv.w * h[3]);
-        }
-      };
-      if (t0 + k + 3 < q.next) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) token(j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (t0 + k + j == q.next && t0 + k + j < at.t1) {
-            finish(q.s);
-            q.advance(a);
-            start(q.s);
-          }
-          token(j);
+          const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(sC + (k + j) * NP + n0);
+          y[j] = sum_halves(fma2(F2{Cv.x}, h01, mul2(F2{Cv.y}, h23)));
         }
       }
       if constexpr (!STATE_ONLY) {
         sum_states<L>(y, sl);
         put_sums<L>(sy + k * YS + ch, YS, y, sl);
       }
+    };
+    if (t0 + TT <= q.next) {
+#pragma unroll 4
+      for (int k = 0; k < TT; k += 4) tokens(std::false_type(), k);
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < TT; k += 4) tokens(std::true_type(), k);
     }
     __syncthreads();
     if constexpr (!STATE_ONLY) {
@@ -483,11 +494,14 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
     sm.D[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
   }
   for (int i = threadIdx.x; i < TT * CH; i += NT) sm.dD[i] = sm.dbias[i] = 0.f;
-  float A2[S], carry[S] = {}, dA[S] = {};
+  float A2[S], carry4[S] = {};
   load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
-  join_backward<L>(carry, p, at, m, A2, n0, ok);
+  join_backward<L>(carry4, p, at, m, A2, n0, ok);
+  const F2 A2p[2] = {pair(A2[0], A2[1]), pair(A2[2], A2[3])};
+  F2 carry[2] = {pair(carry4[0], carry4[1]), pair(carry4[2], carry4[3])}, dA[2] = {both(0.f), both(0.f)}, dA_lost[2] = {both(0.f), both(0.f)};
+  float* const bc_to = &sm.bc[warp][0][sum_place<L>(lane, n0)];
 
   const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
   for (int tile = tiles - 1; tile >= 0; tile--) {
@@ -541,79 +555,98 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
         }
         s_last = q.s;
       }
-      float before[S], h[CK][S], dec[CK][S];
-      load4(before, a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + ts / CK) * a.M + m) * a.N, n0, a.N, ok, p.wide_state);
-      auto initial = [&](float(&x)[S], int s) {
-        load4(x, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
+      auto initial = [&](F2(&x)[2], int s) {
+        float v[S];
+        load4(v, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
+        x[0] = pair(v[0], v[1]);
+        x[1] = pair(v[2], v[3]);
       };
+      // The gradient that leaves a sequence's first token is its initial state's; the token before belongs to another one.
+      auto leave = [&](int s) {
+        const float2 c01 = halves(carry[0]), c23 = halves(carry[1]);
+        const float out[S] = {c01.x, c01.y, c23.x, c23.y};
+        if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s * a.M + m) * a.N, out, n0, a.N, ok, p.wide_state);
+        const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s > 0;
+        float v[S];
+        load4(v, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
+        carry[0] = pair(v[0], v[1]);
+        carry[1] = pair(v[2], v[3]);
+      };
+      F2 before[2], local[2] = {both(0.f), both(0.f)};
       {
-        float x[S];
+        float v[S];
+        load4(v, a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + ts / CK) * a.M + m) * a.N, n0, a.N, ok, p.wide_state);
+        before[0] = pair(v[0], v[1]);
+        before[1] = pair(v[2], v[3]);
+      }
+      if (starts & 1u) initial(before, s_low);
+      // INSIDE: sequences begin behind the first of the 16 tokens
+      auto walk = [&](auto inside) {
+        F2 h[CK][2], dec[CK][2], x[2] = {before[0], before[1]};
         int s = s_low;
 #pragma unroll
-        for (int i = 0; i < S; i++) x[i] = before[i];
-        if (starts & 1u) {
-          initial(before, s);
-#pragma unroll
-          for (int i = 0; i < S; i++) x[i] = before[i];
-        }
-#pragma unroll
         for (int j = 0; j < CK; j++) {
-          if (j > 0 && (starts >> j & 1u)) initial(x, ++s);
-          const float d = sm.dt[(k0 + j) * CH + ch], w = sm.du[(k0 + j) * CH + ch];
-          const float4 Bv = *reinterpret_cast<const float4*>(sm.B + (k0 + j) * NP + n0);
-          const float b4[S] = {Bv.x, Bv.y, Bv.z, Bv.w};
+          if (inside.value && j > 0 && (starts >> j & 1u)) initial(x, ++s);
+          const F2 d = both(sm.dt[(k0 + j) * CH + ch]), w = both(sm.du[(k0 + j) * CH + ch]);
+          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sm.B + (k0 + j) * NP + n0);
+          const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}};
 #pragma unroll
-          for (int i = 0; i < S; i++) {
-            dec[j][i] = ex2(d * A2[i]);
-            x[i] = fmaf(dec[j][i], x[i], w * b4[i]);
+          for (int i = 0; i < 2; i++) {
+            dec[j][i] = ex2_2(mul2(d, A2p[i]));
+            x[i] = fma2(dec[j][i], x[i], mul2(w, b2[i]));
             h[j][i] = x[i];
           }
         }
-      }
+        s = s_last;
 #pragma unroll
-      for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
-        float drive[4], decay[4], y[4];
+        for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
+          float drive[4], decay[4], y[4];
 #pragma unroll
-        for (int jj = 3; jj >= 0; jj--) {
-          const int j = j4 + jj;
-          const float d = sm.dt[(k0 + j) * CH + ch], w = sm.du[(k0 + j) * CH + ch], g = sm.dy[(k0 + j) * CH + ch];
-          const float4 Bv = *reinterpret_cast<const float4*>(sm.B + (k0 + j) * NP + n0), Cv = *reinterpret_cast<const float4*>(sm.C + (k0 + j) * NP + n0);
-          const float b4[S] = {Bv.x, Bv.y, Bv.z, Bv.w}, c4[S] = {Cv.x, Cv.y, Cv.z, Cv.w};
-          const bool first = starts >> j & 1u;
-          float old[S];
+          for (int jj = 3; jj >= 0; jj--) {
+            const int j = j4 + jj;
+            const F2 d = both(sm.dt[(k0 + j) * CH + ch]), w = both(sm.du[(k0 + j) * CH + ch]), g = both(sm.dy[(k0 + j) * CH + ch]);
+            const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sm.B + (k0 + j) * NP + n0), Cv = *reinterpret_cast<const ulonglong2*>(sm.C + (k0 + j) * NP + n0);
+            const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}}, c2[2] = {F2{Cv.x}, F2{Cv.y}};
+            F2 old[2] = {j == 0 ? before[0] : h[j > 0 ? j - 1 : 0][0], j == 0 ? before[1] : h[j > 0 ? j - 1 : 0][1]};
+            const bool first = inside.value && j > 0 && (starts >> j & 1u);
+            if (first) initial(old, s);
+            float v[8];
+            F2 dr, de, yy;
 #pragma unroll
-          for (int i = 0; i < S; i++) old[i] = j == 0 ? before[i] : h[j > 0 ? j - 1 : 0][i];
-          if (j > 0 && first) initial(old, s_last);
-          float v[8], dr = 0.f, de = 0.f, yy = 0.f;
-#pragma unroll
-          for (int i = 0; i < S; i++) {
-            const float gh = fmaf(c4[i], g, carry[i]);
-            carry[i] = dec[j][i] * gh;
-            const float qv = carry[i] * old[i];
-            dr = fmaf(gh, b4[i], dr);
-            de = fmaf(qv, A2[i], de);
-            yy = fmaf(c4[i], h[j][i], yy);
-            dA[i] = fmaf(qv, d, dA[i]);
-            v[i] = gh * w;
-            v[4 + i] = g * h[j][i];
+            for (int i = 0; i < 2; i++) {
+              const F2 gh = fma2(c2[i], g, carry[i]);
+              carry[i] = mul2(dec[j][i], gh);
+              const F2 qv = mul2(carry[i], old[i]);
+              dr = i ? fma2(gh, b2[i], dr) : mul2(gh, b2[i]);
+              de = i ? fma2(qv, A2p[i], de) : mul2(qv, A2p[i]);
+              yy = i ? fma2(c2[i], h[j][i], yy) : mul2(c2[i], h[j][i]);
+              local[i] = fma2(qv, d, local[i]);
+              const float2 vb = halves(mul2(gh, w)), vc = halves(mul2(g, h[j][i]));
+              v[2 * i] = vb.x; v[2 * i + 1] = vb.y; v[4 + 2 * i] = vc.x; v[5 + 2 * i] = vc.y;
+            }
+            drive[jj] = sum_halves(dr); decay[jj] = sum_halves(de); y[jj] = sum_halves(yy);
+            sum_channels<L>(v, lane, [&](int i, float e) { bc_to[(k0 + j) * 2 * NP + i] = e; });
+            if (first) leave(s--);
           }
-          drive[jj] = dr; decay[jj] = de; y[jj] = yy;
-          sum_channels<L>(v, lane, [&](int i, float x) { sm.bc[warp][k0 + j][(i >> 2) * NP + n0 + (i & 3)] = x; });
-          if (first) {
-            if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s_last * a.M + m) * a.N, carry, n0, a.N, ok, p.wide_state);
-            s_last--;
-            const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s_last >= 0;
-            load4(carry, a.dfinal_state + ((long long)(has ? s_last : 0) * a.M + m) * a.N, n0, a.N, ok && has, p.wide_state);
+          sum_states<L>(drive, sl);
+          put_sums<L>(sm.drive + (k0 + j4) * YS + ch, YS, drive, sl);
+          sum_states<L>(decay, sl);
+          put_sums<L>(sm.decay + (k0 + j4) * YS + ch, YS, decay, sl);
+          if (gated) {
+            sum_states<L>(y, sl);
+            put_sums<L>(sm.y + (k0 + j4) * YS + ch, YS, y, sl);
           }
         }
-        sum_states<L>(drive, sl);
-        put_sums<L>(sm.drive + (k0 + j4) * YS + ch, YS, drive, sl);
-        sum_states<L>(decay, sl);
-        put_sums<L>(sm.decay + (k0 + j4) * YS + ch, YS, decay, sl);
-        if (gated) {
-          sum_states<L>(y, sl);
-          put_sums<L>(sm.y + (k0 + j4) * YS + ch, YS, y, sl);
-        }
+      };
+      if (starts >> 1) walk(std::true_type());
+      else walk(std::false_type());
+      if (starts & 1u) leave(s_low);
+      // dA over thousands of tokens: sums of 16, joined with what each addition rounds off
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const F2 add = add2(local[i], dA_lost[i]), sum = add2(dA[i], add);
+        dA_lost[i] = add2(add, neg2(add2(sum, neg2(dA[i]))));
+        dA[i] = sum;
       }
     }
     __syncthreads();
@@ -658,7 +691,11 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
     }
   }
   float* part = p.part_m + ((long long)at.b * p.segments + at.seg) * ((long long)a.M * (a.N + 2));
-  store4(part + m * a.N, dA, n0, a.N, ok, false);
+  {
+    const float2 x = halves(dA[0]), y = halves(dA[1]);
+    const float out[S] = {x.x, x.y, y.x, y.y};
+    store4(part + m * a.N, out, n0, a.N, ok, false);
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < at.valid; c += NT) {
     float x = 0.f, y = 0.f;
