@@ -27,7 +27,7 @@ namespace rewy {
 namespace {
 
 constexpr int TT = 32;    // tokens per tile
-constexpr int NT = 128;   // threads per CTA
+constexpr int NT = 128;   // threads that run the recurrence
 constexpr int S = 4;      // states per thread
 constexpr int CK = 16;    // tokens between checkpoints
 constexpr float LN2 = 0.6931471805599453f;
@@ -95,22 +95,31 @@ __device__ __forceinline__ void store4(float* p, const float (&x)[S], int n0, in
     if (n0 + i < N) p[n0 + i] = x[i];
 }
 
-// Sums of x over the L lanes of a channel.  Afterwards lane l of them holds in x[0] (L = 2: x[0], x[1]) the sum of value
-// sum_owner(l) (L = 2: and the next one); lanes of the same l % 4 hold the same.
-template <int L>
-__device__ __forceinline__ void sum_states(float (&x)[4], int l) {
+// Sums over the L lanes of a channel, for G sets of four values.  Afterwards lane l of them holds in x[.][0] (L = 2: x[.][0], x[.][1])
+// the sum of the value that put_sums writes.  Exchanges keep the order in which they are written, so all sets take a step
+// together: one latency per step instead of one per set.
+template <int L, int G>
+__device__ __forceinline__ void sum_states(float (&x)[G][4], int l) {
 #pragma unroll
   for (int m = L / 2; m >= 4; m >>= 1)
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], m);
-  const bool odd = l & 1;
-  const float k0 = odd ? x[2] : x[0], k1 = odd ? x[3] : x[1], s0 = odd ? x[0] : x[2], s1 = odd ? x[1] : x[3];
-  x[0] = k0 + __shfl_xor_sync(0xffffffffu, s0, 1);
-  x[1] = k1 + __shfl_xor_sync(0xffffffffu, s1, 1);
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[g][i] += __shfl_xor_sync(0xffffffffu, x[g][i], m);
+  const bool odd = l & 1, up = l & 2;
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float keep = odd ? x[g][2 + i] : x[g][i], give = odd ? x[g][i] : x[g][2 + i];
+      x[g][i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+    }
   if constexpr (L >= 4) {
-    const bool up = l & 2;
-    const float k = up ? x[1] : x[0], s = up ? x[0] : x[1];
-    x[0] = k + __shfl_xor_sync(0xffffffffu, s, 2);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const float keep = up ? x[g][1] : x[g][0], give = up ? x[g][0] : x[g][1];
+      x[g][0] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+    }
   }
 }
 template <int L>
@@ -120,7 +129,7 @@ __device__ __forceinline__ void put_sums(float* at, int stride, const float (&x)
     at[first * stride] = x[0];
     at[(first + 1) * stride] = x[1];
   } else {
-    if (l < 4) at[(first + ((l >> 1) & 1)) * stride] = x[0];
+    if (L == 4 || l < 4) at[(first + ((l >> 1) & 1)) * stride] = x[0];
   }
 }
 
@@ -138,27 +147,41 @@ __device__ __forceinline__ int sum_place(int lane, int n0) {
   }
   return (base >> 2) * NP + n0 + (base & 3);
 }
-template <int L, class F>
-__device__ __forceinline__ void sum_channels(float (&v)[8], int lane, F&& put) {
+template <int L, int G, class F>
+__device__ __forceinline__ void sum_channels(float (&v)[G][8], int lane, F&& put) {  // G tokens step by step together
   int n = 8;
 #pragma unroll
   for (int m = 16; m >= L; m >>= 1) {
+    const bool up = lane & m;
     if (n > 1) {
       n >>= 1;
-      const bool up = lane & m;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (i < n) {
-          const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
-        }
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (i < n) {
+            const float keep = up ? v[g][i + n] : v[g][i], give = up ? v[g][i] : v[g][i + n];
+            v[g][i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+          }
     } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+#pragma unroll
+      for (int g = 0; g < G; g++) v[g][0] += __shfl_xor_sync(0xffffffffu, v[g][0], m);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++)   // n <= 4: the values lie in one half of the row
-    if (i < n) put(i, v[i]);
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)   // n <= 4: the values lie in one half of the row
+      if (i < n) put(g, i, v[g][i]);
+}
+
+__device__ __forceinline__ void read8(float (&x)[8], const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void write8(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
 // A tile's rows of one [B,T,M] tensor: 8 channels per access.
@@ -166,7 +189,7 @@ template <class T, int L>
 struct Rows {
   static constexpr int CH = NT / L, PER_TOKEN = CH / 8, COUNT = TT * PER_TOKEN, EACH = (COUNT + NT - 1) / NT;
   __device__ static __forceinline__ bool mine(int k, int& tok, int& c) {
-    const int i = threadIdx.x + k * NT;
+    const int i = threadIdx.x % NT + k * NT;
     tok = i / PER_TOKEN;
     c = i % PER_TOKEN * 8;
     return i < COUNT;
@@ -184,7 +207,7 @@ struct Shared {
   __device__ __forceinline__ void fetch(const ScanParams& p, const T* B, const T* C, int t0, int t1) {
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
-      const int i = threadIdx.x + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      const int i = threadIdx.x % NT + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
       const int t = t0 + j / PER_TOKEN, n = j % PER_TOKEN * 8;
       if (i < COUNT)
         load_some<T, 8>(v[k], (which ? C + t * p.a.C_stride[1] : B + t * p.a.B_stride[1]) + n, t < t1 ? p.a.N - n : 0, p.wide_bc);
@@ -193,7 +216,7 @@ struct Shared {
   __device__ __forceinline__ void publish(float* sB, float* sC) const {
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
-      const int i = threadIdx.x + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      const int i = threadIdx.x % NT + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
       if (i < COUNT) {
         float* to = (which ? sC : sB) + j * 8;
 #pragma unroll
@@ -204,9 +227,17 @@ struct Shared {
   }
 };
 
-__device__ __forceinline__ float step_of(float raw, float bias, bool softplus) {
-  float sig;
-  return softplus ? softplus_fast(raw + bias, sig) : raw + bias;
+// Eight elements at a time: what is asked once stands outside the loops, whose chains then run side by side.
+// dt of raw inputs, and what a gradient of dt is multiplied by for them
+template <bool SLOPE>
+__device__ __forceinline__ void steps_of(float (&d)[8], float (&slope)[8], bool softplus) {
+  if (softplus) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) d[e] = softplus_fast(d[e], slope[e]);
+  } else if (SLOPE) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) slope[e] = 1.f;
+  }
 }
 
 // State at the first token of segment `seg` of a sequence that began before it, from the ends of the segments between.
@@ -222,26 +253,128 @@ __device__ __forceinline__ void join_forward(float (&h)[S], const ScanParams& p,
   }
 }
 
+template <int L>
+struct FwdShared {
+  static constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
+  float dt[2][TT * CH], du[2][TT * CH], B[2][TT * NP], C[2][TT * NP], y[2][TT * YS];  // du: dt u
+};
+
 // STATE_ONLY: the first pass of a scan in segments (all but the last one).
+// Two groups of four warps: the first runs the recurrence of a tile, the second meanwhile writes what came of the tile before
+// and prepares the tile behind.
 template <class T, int L, bool STATE_ONLY>
-__global__ void __launch_bounds__(NT) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
   using R = Rows<T, L>;
-  __shared__ __align__(16) float sdt[TT * CH], sdu[TT * CH], sB[TT * NP], sC[STATE_ONLY ? 4 : TT * NP], sy[STATE_ONLY ? 4 : TT * YS], sbias[CH], sD[CH];
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  FwdShared<L>& sm = *reinterpret_cast<FwdShared<L>*>(raw_smem);
   const RewyScanArgs& a = p.a;
   const Place<L> at(p, 0, STATE_ONLY ? p.segments - 1 : p.segments);
+  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  const bool gated = !STATE_ONLY && a.z != nullptr;
+  if (threadIdx.x >= NT) {
+    const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
+    const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+    const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
+    const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
+    const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+    float bias[R::EACH][8], Dv[R::EACH][8];
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      R::mine(k, tok, c);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        bias[k][e] = a.dt_bias != nullptr && c + e < at.valid ? a.dt_bias[at.m0 + c + e] : 0.f;
+        Dv[k][e] = !STATE_ONLY && a.D != nullptr && c + e < at.valid ? a.D[at.m0 + c + e] : 0.f;
+      }
+    }
+    Pack<T, 8> ru[R::EACH], rd[R::EACH], xu[R::EACH], xz[R::EACH];
+    Shared<T, L, STATE_ONLY ? 1 : 3> bc;
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        fetch8(ru[k], u, a.u_stride[1], t + tok, at.t1, c, at.valid, p.wide);
+        fetch8(rd[k], dt, a.dt_stride[1], t + tok, at.t1, c, at.valid, p.wide);
+      }
+      bc.fetch(p, Bm, C, t, at.t1);
+    };
+    auto publish = [&](int t, int buf) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        float d[8], w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] = to_f32(rd[k].v[e]) + bias[k][e];
+        steps_of<false>(d, w, a.softplus);
+        const int real = t + tok < at.t1 ? at.valid - c : 0;   // a token that does not exist: no decay, no input
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          d[e] = e < real ? d[e] : 0.f;
+          w[e] = d[e] * to_f32(ru[k].v[e]);
+        }
+        write8(&sm.dt[buf][tok * CH + c], d);
+        write8(&sm.du[buf][tok * CH + c], w);
+      }
+      bc.publish(sm.B[buf], sm.C[buf]);
+    };
+    auto fetch_again = [&](int t0) {   // u and z of the tile whose recurrence has been run
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        if (a.D != nullptr) fetch8(xu[k], u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+        else zero_pack(xu[k]);
+        if (gated) fetch8(xz[k], z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      }
+    };
+    auto finish_tile = [&](int t0, int buf) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
+        float y[8];
+        read8(y, &sm.y[buf][tok * YS + c]);
+        Pack<T, 8> out;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = fmaf(Dv[k][e], to_f32(xu[k].v[e]), y[e]);
+        if (gated)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float g = to_f32(xz[k].v[e]);
+            y[e] *= g * sigmoid_fast(g);
+          }
+#pragma unroll
+        for (int e = 0; e < 8; e++) out.v[e] = from_f32<T>(y[e]);
+        store_some<T, 8>(static_cast<T*>(a.y) + ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c, out, at.valid - c, p.wide);
+      }
+    };
+    // What a step reads has been asked for a step before.
+    fetch(at.t0);
+    publish(at.t0, 0);
+    if (tiles > 1) fetch(at.t0 + TT);
+    if (!STATE_ONLY) fetch_again(at.t0);
+    __syncthreads();
+    for (int i = 0; i < tiles; i++) {
+      const int t0 = at.t0 + i * TT;
+      if (i + 1 < tiles) publish(t0 + TT, (i + 1) & 1);
+      if (i + 2 < tiles) fetch(t0 + 2 * TT);
+      if (!STATE_ONLY && i > 0) {
+        finish_tile(t0 - TT, (i - 1) & 1);
+        fetch_again(t0);
+      }
+      __syncthreads();
+    }
+    if (!STATE_ONLY) finish_tile(at.t0 + (tiles - 1) * TT, (tiles - 1) & 1);
+    return;
+  }
+
   const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
   const bool ok = ch < at.valid;
   const long long m = at.m0 + ch;
-  const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
-  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
-  const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
-  const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  for (int c = threadIdx.x; c < CH; c += NT) {
-    sbias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
-    sD[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
-  }
   float A2[S], h[S] = {};
   load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
@@ -257,105 +390,62 @@ __global__ void __launch_bounds__(NT) scan_fwd_kernel(const __grid_constant__ Sc
   if (q.begin == at.t0) start(q.s);
   else if (!STATE_ONLY) join_forward(h, p, at.b, at.seg, q.begin, m, A2, n0, ok);
 
-  Pack<T, 8> ru[R::EACH], rd[R::EACH], rz[R::EACH], nu[R::EACH], nd[R::EACH], nz[R::EACH];
-  Shared<T, L, STATE_ONLY ? 1 : 3> bc;
-  auto fetch = [&](Pack<T, 8>(&xu)[R::EACH], Pack<T, 8>(&xd)[R::EACH], Pack<T, 8>(&xz)[R::EACH], int t) {
-#pragma unroll
-    for (int k = 0; k < R::EACH; k++) {
-      int tok, c;
-      if (!R::mine(k, tok, c)) continue;
-      fetch8(xu[k], u, a.u_stride[1], t + tok, at.t1, c, at.valid, p.wide);
-      fetch8(xd[k], dt, a.dt_stride[1], t + tok, at.t1, c, at.valid, p.wide);
-      if (!STATE_ONLY && a.z != nullptr) fetch8(xz[k], z, a.z_stride[1], t + tok, at.t1, c, at.valid, p.wide);
-    }
-    bc.fetch(p, Bm, C, t, at.t1);
-  };
-  auto publish = [&](int t) {
-#pragma unroll
-    for (int k = 0; k < R::EACH; k++) {
-      int tok, c;
-      if (!R::mine(k, tok, c)) continue;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const bool real = t + tok < at.t1 && c + e < at.valid;   // a token that does not exist: no decay, no input
-        const float d = real ? step_of(to_f32(rd[k].v[e]), sbias[c + e], a.softplus) : 0.f;
-        sdt[tok * CH + c + e] = d;
-        sdu[tok * CH + c + e] = real ? d * to_f32(ru[k].v[e]) : 0.f;
-      }
-    }
-    bc.publish(sB, sC);
-  };
-  fetch(ru, rd, rz, at.t0);
-  __syncthreads();   // sbias, sD
-  publish(at.t0);
-
   float total = 0.f;
-  for (int t0 = at.t0; t0 < at.t1; t0 += TT) {
-    const bool more = t0 + TT < at.t1;
-    if (more) fetch(nu, nd, nz, t0 + TT);
-    __syncthreads();
-    // CHECK: a sequence may begin inside the tile
+  __syncthreads();
+  for (int i = 0; i < tiles; i++) {
+    const int t0 = at.t0 + i * TT, buf = i & 1;
+    const float *__restrict__ const sdt = sm.dt[buf] + ch, *__restrict__ const sdu = sm.du[buf] + ch;
+    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.C[buf] + n0;
+    float* __restrict__ const sy = sm.y[buf] + ch;
+    // Eight tokens; check: a sequence may begin inside the tile
     auto tokens = [&](auto check, int k) {
-      if (!STATE_ONLY && k % CK == 0 && a.checkpoints != nullptr && t0 + k < a.T)
-        store4(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + k) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
-      float y[4];
+      float y[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (check.value && t0 + k + j == q.next && t0 + k + j < at.t1) {
-          finish(q.s);
-          q.advance(a);
-          start(q.s);
+      for (int half = 0; half < 2; half++) {
+        const int kh = k + 4 * half;
+        if (!STATE_ONLY && kh % CK == 0 && a.checkpoints != nullptr && t0 + kh < a.T)
+          store4(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + kh) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
+        F2 e01[4], e23[4], g01[4], g23[4];
+        ulonglong2 Cv[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float dj = sdt[(kh + j) * CH];
+          const F2 d = both(dj), w = both(sdu[(kh + j) * CH]);
+          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (kh + j) * NP);
+          if (!STATE_ONLY) Cv[j] = *reinterpret_cast<const ulonglong2*>(sC + (kh + j) * NP);
+          else total += dj;
+          e01[j] = ex2_2(mul2(d, A01));
+          e23[j] = ex2_2(mul2(d, A23));
+          g01[j] = mul2(w, F2{Bv.x});
+          g23[j] = mul2(w, F2{Bv.y});
         }
-        const float d = sdt[(k + j) * CH + ch];
-        const F2 dd = both(d), x = both(sdu[(k + j) * CH + ch]);
-        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k + j) * NP + n0);
-        const F2 h01 = fma2(ex2_2(mul2(dd, A01)), pair(h[0], h[1]), mul2(x, F2{Bv.x}));
-        const F2 h23 = fma2(ex2_2(mul2(dd, A23)), pair(h[2], h[3]), mul2(x, F2{Bv.y}));
-        const float2 u01 = halves(h01), u23 = halves(h23);
-        h[0] = u01.x; h[1] = u01.y; h[2] = u23.x; h[3] = u23.y;
-        if constexpr (STATE_ONLY) {
-          total += d;
-        } else {
-          const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(sC + (k + j) * NP + n0);
-          y[j] = sum_halves(fma2(F2{Cv.x}, h01, mul2(F2{Cv.y}, h23)));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (check.value && t0 + kh + j == q.next && t0 + kh + j < at.t1) {
+            finish(q.s);
+            q.advance(a);
+            start(q.s);
+          }
+          const F2 h01 = fma2(e01[j], pair(h[0], h[1]), g01[j]), h23 = fma2(e23[j], pair(h[2], h[3]), g23[j]);
+          const float2 u01 = halves(h01), u23 = halves(h23);
+          h[0] = u01.x; h[1] = u01.y; h[2] = u23.x; h[3] = u23.y;
+          if constexpr (!STATE_ONLY) y[half][j] = sum_halves(fma2(F2{Cv[j].x}, h01, mul2(F2{Cv[j].y}, h23)));
         }
       }
       if constexpr (!STATE_ONLY) {
         sum_states<L>(y, sl);
-        put_sums<L>(sy + k * YS + ch, YS, y, sl);
+        put_sums<L>(sy + k * YS, YS, y[0], sl);
+        put_sums<L>(sy + (k + 4) * YS, YS, y[1], sl);
       }
     };
     if (t0 + TT <= q.next) {
-#pragma unroll 4
-      for (int k = 0; k < TT; k += 4) tokens(std::false_type(), k);
+#pragma unroll
+      for (int k = 0; k < TT; k += 8) tokens(std::false_type(), k);
     } else {
 #pragma unroll 1
-      for (int k = 0; k < TT; k += 4) tokens(std::true_type(), k);
+      for (int k = 0; k < TT; k += 8) tokens(std::true_type(), k);
     }
     __syncthreads();
-    if constexpr (!STATE_ONLY) {
-#pragma unroll
-      for (int k = 0; k < R::EACH; k++) {
-        int tok, c;
-        if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
-        Pack<T, 8> out;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          float v = fmaf(sD[c + e], to_f32(ru[k].v[e]), sy[tok * YS + c + e]);
-          if (a.z != nullptr) {
-            const float g = to_f32(rz[k].v[e]);
-            v *= g * sigmoid_fast(g);
-          }
-          out.v[e] = from_f32<T>(v);
-        }
-        store_some<T, 8>(static_cast<T*>(a.y) + ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c, out, at.valid - c, p.wide);
-      }
-    }
-    if (more) {
-#pragma unroll
-      for (int k = 0; k < R::EACH; k++) { ru[k] = nu[k]; rd[k] = nd[k]; rz[k] = nz[k]; }
-      publish(t0 + TT);
-    }
   }
   if constexpr (STATE_ONLY) {
     const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
@@ -426,17 +516,26 @@ __global__ void __launch_bounds__(NT) scan_bwd_state_kernel(const __grid_constan
       fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
       fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
       if (a.z != nullptr) fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      float d[8], g[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) d[e] = to_f32(xd.v[e]) + sbias[c + e];
+      steps_of<false>(d, g, a.softplus);
+#pragma unroll
+      for (int e = 0; e < 8; e++) g[e] = to_f32(xy.v[e]);
+      if (a.z != nullptr)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float v = to_f32(xz.v[e]);
+          g[e] *= v * sigmoid_fast(v);
+        }
+      const int real = t0 + tok < at.t1 ? at.valid - c : 0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const bool real = t0 + tok < at.t1 && c + e < at.valid;
-        float g = to_f32(xy.v[e]);
-        if (a.z != nullptr) {
-          const float v = to_f32(xz.v[e]);
-          g *= v * sigmoid_fast(v);
-        }
-        sdt[tok * CH + c + e] = real ? step_of(to_f32(xd.v[e]), sbias[c + e], a.softplus) : 0.f;
-        sdy[tok * CH + c + e] = real ? g : 0.f;
+        d[e] = e < real ? d[e] : 0.f;
+        g[e] = e < real ? g[e] : 0.f;
       }
+      write8(sdt + tok * CH + c, d);
+      write8(sdy + tok * CH + c, g);
     }
     Shared<T, L, 2> cc;
     cc.fetch(p, nullptr, C, t0, at.t1);
@@ -465,35 +564,186 @@ __global__ void __launch_bounds__(NT) scan_bwd_state_kernel(const __grid_constan
 template <int L>
 struct BwdShared {
   static constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
-  float dt[TT * CH], du[TT * CH], dy[TT * CH], B[TT * NP], C[TT * NP];
-  float drive[TT * YS], decay[TT * YS], y[TT * YS];   // per token and channel: sum gh B, sum q A2, sum C h
-  float bc[NT / 32][TT][2 * NP];                      // each warp's sums over its channels
-  float dD[TT * CH], dbias[TT * CH];                  // running sums, one entry per token of the tile
+  float4 x[2][TT * CH];                                       // dt, dt u, dy' at place(token, channel)
+  float B[2][TT * NP], C[2][TT * NP];
+  float drive[2][TT * YS], decay[2][TT * YS], y[2][TT * YS];  // per token and channel: sum gh B, sum q A2, sum C h
+  float bc[2][NT / 32][TT][2 * NP];                           // each warp's sums over its channels
   float bias[CH], D[CH];
+  // A thread writes the entries of eight neighbouring channels: turned by what keeps the threads of a quarter warp apart
+  __device__ static __forceinline__ int place(int tok, int c) { return tok * CH + (c & ~7) + ((c ^ ((c >> 3) + CH / 8 * tok)) & 7); }
 };
 
+// Two groups of four warps, as in the forward: the recurrence of a tile beside what stands around the tiles next to it.
 template <class T, int L>
-__global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
   using R = Rows<T, L>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   BwdShared<L>& sm = *reinterpret_cast<BwdShared<L>*>(raw_smem);
   const RewyScanArgs& a = p.a;
   const Place<L> at(p, 0, p.segments);
-  const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool ok = ch < at.valid, gated = a.z != nullptr;
-  const long long m = at.m0 + ch;
-  const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
-  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
-  const T* z = static_cast<const T*>(a.z) + (gated ? at.b * a.z_stride[0] + at.m0 : 0);
-  const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
-  const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  for (int c = threadIdx.x; c < CH; c += NT) {
-    sm.bias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
-    sm.D[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
+  const bool gated = a.z != nullptr;
+  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  float* const part = p.part_m + ((long long)at.b * p.segments + at.seg) * ((long long)a.M * (a.N + 2));
+  if (threadIdx.x >= NT) {
+    const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
+    const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+    const T* z = static_cast<const T*>(a.z) + (gated ? at.b * a.z_stride[0] + at.m0 : 0);
+    const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
+    const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
+    const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+    const int me = threadIdx.x - NT;
+    struct Inputs {
+      Pack<T, 8> u[R::EACH], dt[R::EACH], dy[R::EACH], z[R::EACH];
+    };
+    auto fetch = [&](Inputs& x, int t0) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        fetch8(x.u[k], u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+        fetch8(x.dt[k], dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+        fetch8(x.dy[k], dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+        if (gated) fetch8(x.z[k], z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      }
+    };
+    Inputs ahead, behind;      // of the tile that is prepared next, of the one that is finished next
+    Shared<T, L, 3> bc;
+    auto prepare = [&](int t0, int buf) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        float d[8], g[8];
+        read8(d, sm.bias + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] += to_f32(ahead.dt[k].v[e]);
+        steps_of<false>(d, g, a.softplus);
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[e] = to_f32(ahead.dy[k].v[e]);
+        if (gated)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float v = to_f32(ahead.z[k].v[e]);
+            g[e] *= v * sigmoid_fast(v);
+          }
+        const int real = t0 + tok < at.t1 ? at.valid - c : 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          sm.x[buf][BwdShared<L>::place(tok, c + e)] =
+              e < real ? make_float4(d[e], d[e] * to_f32(ahead.u[k].v[e]), g[e], 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      bc.publish(sm.B[buf], sm.C[buf]);
+    };
+    float sD[R::EACH][8] = {}, sbias[R::EACH][8] = {};   // sums over the tokens that this thread sees
+    auto finish_tile = [&](int t0, int buf) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
+        Pack<T, 8> ou, od, oz;
+        float drive[8], x[8], g[8], d[8], slope[8];
+        const float* const Dv = sm.D + c;
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[e] = to_f32(behind.dy[k].v[e]);
+        if (gated) {
+          read8(x, &sm.y[buf][tok * YS + c]);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float v = to_f32(behind.z[k].v[e]), s = sigmoid_fast(v);
+            oz.v[e] = from_f32<T>(g[e] * fmaf(Dv[e], to_f32(behind.u[k].v[e]), x[e]) * s * fmaf(v, 1.f - s, 1.f));
+            g[e] *= v * s;
+          }
+        }
+        read8(d, sm.bias + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] += to_f32(behind.dt[k].v[e]);
+        steps_of<true>(d, slope, a.softplus);
+        read8(drive, &sm.drive[buf][tok * YS + c]);
+        read8(x, &sm.decay[buf][tok * YS + c]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float uv = to_f32(behind.u[k].v[e]), dd = fmaf(uv, drive[e], LN2 * x[e]) * slope[e];
+          ou.v[e] = from_f32<T>(fmaf(Dv[e], g[e], drive[e] * d[e]));
+          od.v[e] = from_f32<T>(dd);
+          sD[k][e] = fmaf(g[e], uv, sD[k][e]);     // (channels that do not exist are not read)
+          sbias[k][e] += dd;
+        }
+        const long long to = ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c;
+        store_some<T, 8>(static_cast<T*>(a.du) + to, ou, at.valid - c, p.wide);
+        store_some<T, 8>(static_cast<T*>(a.ddt) + to, od, at.valid - c, p.wide);
+        if (gated) store_some<T, 8>(static_cast<T*>(a.dz) + to, oz, at.valid - c, p.wide);
+      }
+      // the warps' sums over their channels: a thread adds one place of the row for every NT / (2 NP)-th token
+      constexpr int EVERY = NT / (2 * NP) > 0 ? NT / (2 * NP) : 1;
+      const int v = me % (2 * NP), n = v % NP;
+      if (n < a.N) {
+        float* to = p.part_bc + ((((long long)at.cb * a.B + at.b) * a.T + t0) * a.G + at.g) * 2 * a.N + v / NP * a.N + n;
+        const int row = a.G * 2 * a.N;
+#pragma unroll 4
+        for (int tok = me / (2 * NP); tok < TT; tok += EVERY) {
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < NT / 32; w++) sum += sm.bc[buf][w][tok][v];
+          if (t0 + tok < at.t1) to[(long long)tok * row] = sum;
+        }
+      }
+    };
+    for (int c = me; c < CH; c += NT) {
+      sm.bias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
+      sm.D[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
+    }
+    __syncthreads();
+    // What a step reads has been asked for a step before.
+    {
+      const int t0 = at.t0 + (tiles - 1) * TT;
+      fetch(ahead, t0);
+      bc.fetch(p, Bm, C, t0, at.t1);
+      prepare(t0, (tiles - 1) & 1);
+      behind = ahead;
+      if (tiles > 1) {
+        fetch(ahead, t0 - TT);
+        bc.fetch(p, Bm, C, t0 - TT, at.t1);
+      }
+    }
+    __syncthreads();
+    for (int tile = tiles - 1; tile >= 0; tile--) {
+      const int t0 = at.t0 + tile * TT;
+      if (tile > 0) prepare(t0 - TT, (tile - 1) & 1);
+      if (tile > 1) {
+        fetch(ahead, t0 - 2 * TT);
+        bc.fetch(p, Bm, C, t0 - 2 * TT, at.t1);
+      }
+      if (tile + 1 < tiles) {
+        finish_tile(t0 + TT, (tile + 1) & 1);
+        fetch(behind, t0);
+      }
+      __syncthreads();
+    }
+    finish_tile(at.t0, 0);
+    // over the tokens of a tile, in the room of the operands, which nothing reads any more
+    float *const all_D = reinterpret_cast<float*>(sm.x[0]), *const all_bias = all_D + TT * CH;
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      if (!R::mine(k, tok, c)) continue;
+      write8(all_D + tok * CH + c, sD[k]);
+      write8(all_bias + tok * CH + c, sbias[k]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");   // this group only
+    for (int c = me; c < at.valid; c += NT) {
+      float x = 0.f, y = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < TT; k++) { x += all_D[k * CH + c]; y += all_bias[k * CH + c]; }
+      part[(long long)a.M * a.N + at.m0 + c] = x;
+      part[(long long)a.M * (a.N + 1) + at.m0 + c] = y;
+    }
+    return;
   }
-  for (int i = threadIdx.x; i < TT * CH; i += NT) sm.dD[i] = sm.dbias[i] = 0.f;
+
+  const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool ok = ch < at.valid;
+  const long long m = at.m0 + ch;
   float A2[S], carry4[S] = {};
   load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
@@ -501,42 +751,35 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
   join_backward<L>(carry4, p, at, m, A2, n0, ok);
   const F2 A2p[2] = {pair(A2[0], A2[1]), pair(A2[2], A2[3])};
   F2 carry[2] = {pair(carry4[0], carry4[1]), pair(carry4[2], carry4[3])}, dA[2] = {both(0.f), both(0.f)}, dA_lost[2] = {both(0.f), both(0.f)};
-  float* const bc_to = &sm.bc[warp][0][sum_place<L>(lane, n0)];
-
-  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  const int place = sum_place<L>(lane, n0);
+  auto initial = [&](F2(&x)[2], int s) {
+    float v[S];
+    load4(v, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
+    x[0] = pair(v[0], v[1]);
+    x[1] = pair(v[2], v[3]);
+  };
+  // The gradient that leaves a sequence's first token is its initial state's; the token before belongs to another one.
+  auto leave = [&](int s) {
+    const float2 c01 = halves(carry[0]), c23 = halves(carry[1]);
+    const float out[S] = {c01.x, c01.y, c23.x, c23.y};
+    if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s * a.M + m) * a.N, out, n0, a.N, ok, p.wide_state);
+    const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s > 0;
+    float v[S];
+    load4(v, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
+    carry[0] = pair(v[0], v[1]);
+    carry[1] = pair(v[2], v[3]);
+  };
+  const float* const kept = a.checkpoints + ((long long)at.b * ((a.T + CK - 1) / CK) * a.M + m) * a.N;
+  float next[S];   // the state before the 16 tokens that come next
+  load4(next, kept + (long long)((at.t1 - 1) / CK) * a.M * a.N, n0, a.N, ok, p.wide_state);
+  __syncthreads();
+  __syncthreads();
   for (int tile = tiles - 1; tile >= 0; tile--) {
-    const int t0 = at.t0 + tile * TT;
-    __syncthreads();   // bias, D and the zeroed sums; the tile behind has been read
-#pragma unroll
-    for (int k = 0; k < R::EACH; k++) {
-      int tok, c;
-      if (!R::mine(k, tok, c)) continue;
-      Pack<T, 8> xu, xd, xy, xz;
-      fetch8(xu, u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
-      if (gated) fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int i = tok * CH + c + e;
-        const bool real = t0 + tok < at.t1 && c + e < at.valid;
-        const float d = real ? step_of(to_f32(xd.v[e]), sm.bias[c + e], a.softplus) : 0.f;
-        float g = to_f32(xy.v[e]);
-        if (gated) {
-          const float v = to_f32(xz.v[e]);
-          g *= v * sigmoid_fast(v);
-        }
-        sm.dt[i] = d;
-        sm.du[i] = real ? d * to_f32(xu.v[e]) : 0.f;
-        sm.dy[i] = real ? g : 0.f;
-      }
-    }
-    {
-      Shared<T, L, 3> bc;
-      bc.fetch(p, Bm, C, t0, at.t1);
-      bc.publish(sm.B, sm.C);
-    }
-    __syncthreads();
+    const int t0 = at.t0 + tile * TT, buf = tile & 1;
+    const float4* __restrict__ const sx = sm.x[buf];
+    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.C[buf] + n0;
+    float *__restrict__ const to_drive = sm.drive[buf] + ch, *__restrict__ const to_decay = sm.decay[buf] + ch, *__restrict__ const to_y = sm.y[buf] + ch;
+    float* __restrict__ const to_bc = &sm.bc[buf][warp][0][place];
 #pragma unroll 1
     for (int sub = TT / CK - 1; sub >= 0; sub--) {
       const int k0 = sub * CK, ts = t0 + k0;
@@ -555,87 +798,61 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
         }
         s_last = q.s;
       }
-      auto initial = [&](F2(&x)[2], int s) {
-        float v[S];
-        load4(v, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
-        x[0] = pair(v[0], v[1]);
-        x[1] = pair(v[2], v[3]);
-      };
-      // The gradient that leaves a sequence's first token is its initial state's; the token before belongs to another one.
-      auto leave = [&](int s) {
-        const float2 c01 = halves(carry[0]), c23 = halves(carry[1]);
-        const float out[S] = {c01.x, c01.y, c23.x, c23.y};
-        if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s * a.M + m) * a.N, out, n0, a.N, ok, p.wide_state);
-        const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s > 0;
-        float v[S];
-        load4(v, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
-        carry[0] = pair(v[0], v[1]);
-        carry[1] = pair(v[2], v[3]);
-      };
-      F2 before[2], local[2] = {both(0.f), both(0.f)};
-      {
-        float v[S];
-        load4(v, a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + ts / CK) * a.M + m) * a.N, n0, a.N, ok, p.wide_state);
-        before[0] = pair(v[0], v[1]);
-        before[1] = pair(v[2], v[3]);
-      }
+      F2 before[2] = {pair(next[0], next[1]), pair(next[2], next[3])}, local[2] = {both(0.f), both(0.f)};
+      if (ts > at.t0) load4(next, kept + (long long)(ts / CK - 1) * a.M * a.N, n0, a.N, ok, p.wide_state);
       if (starts & 1u) initial(before, s_low);
-      // INSIDE: sequences begin behind the first of the 16 tokens
+      // inside: sequences begin behind the first of the 16 tokens
       auto walk = [&](auto inside) {
-        F2 h[CK][2], dec[CK][2], x[2] = {before[0], before[1]};
+        F2 h[CK][2], x[2] = {before[0], before[1]};
         int s = s_low;
 #pragma unroll
         for (int j = 0; j < CK; j++) {
           if (inside.value && j > 0 && (starts >> j & 1u)) initial(x, ++s);
-          const F2 d = both(sm.dt[(k0 + j) * CH + ch]), w = both(sm.du[(k0 + j) * CH + ch]);
-          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sm.B + (k0 + j) * NP + n0);
+          const float2 v = *reinterpret_cast<const float2*>(sx + k0 * CH + BwdShared<L>::place(j, ch));
+          const F2 d = both(v.x), w = both(v.y);
+          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k0 + j) * NP);
           const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}};
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            dec[j][i] = ex2_2(mul2(d, A2p[i]));
-            x[i] = fma2(dec[j][i], x[i], mul2(w, b2[i]));
+            x[i] = fma2(ex2_2(mul2(d, A2p[i])), x[i], mul2(w, b2[i]));
             h[j][i] = x[i];
           }
         }
         s = s_last;
 #pragma unroll
         for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
-          float drive[4], decay[4], y[4];
+          float sums[3][4], v[2][8];   // drive, decay, y of four tokens; dB and dC of this channel of two
 #pragma unroll
           for (int jj = 3; jj >= 0; jj--) {
             const int j = j4 + jj;
-            const F2 d = both(sm.dt[(k0 + j) * CH + ch]), w = both(sm.du[(k0 + j) * CH + ch]), g = both(sm.dy[(k0 + j) * CH + ch]);
-            const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sm.B + (k0 + j) * NP + n0), Cv = *reinterpret_cast<const ulonglong2*>(sm.C + (k0 + j) * NP + n0);
+            const float4 xv = sx[k0 * CH + BwdShared<L>::place(j, ch)];
+            const F2 d = both(xv.x), w = both(xv.y), g = both(xv.z);
+            const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k0 + j) * NP), Cv = *reinterpret_cast<const ulonglong2*>(sC + (k0 + j) * NP);
             const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}}, c2[2] = {F2{Cv.x}, F2{Cv.y}};
             F2 old[2] = {j == 0 ? before[0] : h[j > 0 ? j - 1 : 0][0], j == 0 ? before[1] : h[j > 0 ? j - 1 : 0][1]};
             const bool first = inside.value && j > 0 && (starts >> j & 1u);
             if (first) initial(old, s);
-            float v[8];
             F2 dr, de, yy;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
               const F2 gh = fma2(c2[i], g, carry[i]);
-              carry[i] = mul2(dec[j][i], gh);
+              carry[i] = mul2(ex2_2(mul2(d, A2p[i])), gh);
               const F2 qv = mul2(carry[i], old[i]);
               dr = i ? fma2(gh, b2[i], dr) : mul2(gh, b2[i]);
               de = i ? fma2(qv, A2p[i], de) : mul2(qv, A2p[i]);
               yy = i ? fma2(c2[i], h[j][i], yy) : mul2(c2[i], h[j][i]);
               local[i] = fma2(qv, d, local[i]);
               const float2 vb = halves(mul2(gh, w)), vc = halves(mul2(g, h[j][i]));
-              v[2 * i] = vb.x; v[2 * i + 1] = vb.y; v[4 + 2 * i] = vc.x; v[5 + 2 * i] = vc.y;
+              v[jj & 1][2 * i] = vb.x; v[jj & 1][2 * i + 1] = vb.y; v[jj & 1][4 + 2 * i] = vc.x; v[jj & 1][5 + 2 * i] = vc.y;
             }
-            drive[jj] = sum_halves(dr); decay[jj] = sum_halves(de); y[jj] = sum_halves(yy);
-            sum_channels<L>(v, lane, [&](int i, float e) { bc_to[(k0 + j) * 2 * NP + i] = e; });
+            sums[0][jj] = sum_halves(dr); sums[1][jj] = sum_halves(de); sums[2][jj] = sum_halves(yy);
             if (first) leave(s--);
+            if (jj % 2 == 0) sum_channels<L>(v, lane, [&](int odd, int i, float e) { to_bc[(k0 + j + odd) * 2 * NP + i] = e; });
           }
-          sum_states<L>(drive, sl);
-          put_sums<L>(sm.drive + (k0 + j4) * YS + ch, YS, drive, sl);
-          sum_states<L>(decay, sl);
-          put_sums<L>(sm.decay + (k0 + j4) * YS + ch, YS, decay, sl);
-          if (gated) {
-            sum_states<L>(y, sl);
-            put_sums<L>(sm.y + (k0 + j4) * YS + ch, YS, y, sl);
-          }
+          sum_states<L>(sums, sl);
+          put_sums<L>(to_drive + (k0 + j4) * YS, YS, sums[0], sl);
+          put_sums<L>(to_decay + (k0 + j4) * YS, YS, sums[1], sl);
+          if (gated) put_sums<L>(to_y + (k0 + j4) * YS, YS, sums[2], sl);
         }
       };
       if (starts >> 1) walk(std::true_type());
@@ -650,60 +867,10 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd_kernel(const __grid_constant__
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < R::EACH; k++) {
-      int tok, c;
-      if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
-      Pack<T, 8> xu, xd, xy, xz, ou, od, oz;
-      fetch8(xu, u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      if (gated) {
-        fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
-        fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int i = tok * CH + c + e, iy = tok * YS + c + e;
-        const float uv = to_f32(xu.v[e]), g = sm.dy[i], drive = sm.drive[iy], Dv = sm.D[c + e];
-        float dd = fmaf(uv, drive, LN2 * sm.decay[iy]);
-        if (a.softplus) dd *= sigmoid_fast(to_f32(xd.v[e]) + sm.bias[c + e]);
-        ou.v[e] = from_f32<T>(fmaf(Dv, g, drive * sm.dt[i]));
-        od.v[e] = from_f32<T>(dd);
-        sm.dD[i] = fmaf(g, uv, sm.dD[i]);
-        sm.dbias[i] += dd;
-        if (gated) {
-          const float v = to_f32(xz.v[e]), sig = sigmoid_fast(v);
-          oz.v[e] = from_f32<T>(to_f32(xy.v[e]) * fmaf(Dv, uv, sm.y[iy]) * sig * fmaf(v, 1.f - sig, 1.f));
-        }
-      }
-      const long long to = ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c;
-      store_some<T, 8>(static_cast<T*>(a.du) + to, ou, at.valid - c, p.wide);
-      store_some<T, 8>(static_cast<T*>(a.ddt) + to, od, at.valid - c, p.wide);
-      if (gated) store_some<T, 8>(static_cast<T*>(a.dz) + to, oz, at.valid - c, p.wide);
-    }
-    for (int i = threadIdx.x; i < TT * 2 * NP; i += NT) {
-      const int tok = i / (2 * NP), v = i % (2 * NP), n = v % NP;
-      if (t0 + tok >= at.t1 || n >= a.N) continue;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < NT / 32; w++) sum += sm.bc[w][tok][v];
-      p.part_bc[((((long long)at.cb * a.B + at.b) * a.T + t0 + tok) * a.G + at.g) * 2 * a.N + v / NP * a.N + n] = sum;
-    }
   }
-  float* part = p.part_m + ((long long)at.b * p.segments + at.seg) * ((long long)a.M * (a.N + 2));
-  {
-    const float2 x = halves(dA[0]), y = halves(dA[1]);
-    const float out[S] = {x.x, x.y, y.x, y.y};
-    store4(part + m * a.N, out, n0, a.N, ok, false);
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < at.valid; c += NT) {
-    float x = 0.f, y = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < TT; k++) { x += sm.dD[k * CH + c]; y += sm.dbias[k * CH + c]; }
-    part[(long long)a.M * a.N + at.m0 + c] = x;
-    part[(long long)a.M * (a.N + 1) + at.m0 + c] = y;
-  }
+  const float2 d01 = halves(dA[0]), d23 = halves(dA[1]);
+  const float out[S] = {d01.x, d01.y, d23.x, d23.y};
+  store4(part + m * a.N, out, n0, a.N, ok, false);
 }
 
 // dB, dC [B*T][G][N] from the CTAs' sums [blocks][B*T][G][2][N]
@@ -729,48 +896,60 @@ __global__ void __launch_bounds__(256) scan_sum_m_kernel(const float* __restrict
   if (to != nullptr) *to = sum;
 }
 
-// One token per row: a channel's states over L lanes as above.
+// One token per row: a channel's states over L lanes as above, two channels per thread.  Everything that does not depend on the
+// slot is asked for before the slot is looked at.
 template <class T, int L>
-__global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide) {
-  constexpr int CH = NT / L;
-  const int b = blockIdx.x / blocks, ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
-  const long long m = (long long)(blockIdx.x % blocks) * CH + ch;
-  const bool ok = m < a.M;
+__global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide, bool wide_bc) {
+  constexpr int CH = NT / L, U = 2;
+  const int b = blockIdx.x / blocks, sl = threadIdx.x % L, n0 = sl * S;
+  const long long first = (long long)(blockIdx.x % blocks) * CH * U + threadIdx.x / L;
+  float A2[U][S], u[U], d[U], z[U], D[U];
+  Pack<T, S> Bv[U], Cv[U];
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    const long long m = first + i * CH;
+    const bool ok = m < a.M;
+    const int g = ok ? (int)(m / (a.M / a.G)) : 0;
+    load4(A2[i], a.A + m * a.N, n0, a.N, ok, wide);
+    load_some<T, S>(Bv[i], static_cast<const T*>(a.Bm) + b * a.B_stride[0] + g * a.B_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
+    load_some<T, S>(Cv[i], static_cast<const T*>(a.C) + b * a.C_stride[0] + g * a.C_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
+    u[i] = ok ? to_f32(static_cast<const T*>(a.u)[b * a.u_stride + m]) : 0.f;
+    d[i] = ok ? to_f32(static_cast<const T*>(a.dt)[b * a.dt_stride + m]) + (a.dt_bias != nullptr ? a.dt_bias[m] : 0.f) : 0.f;
+    z[i] = ok && a.z != nullptr ? to_f32(static_cast<const T*>(a.z)[b * a.z_stride + m]) : 0.f;
+    D[i] = ok && a.D != nullptr ? a.D[m] : 0.f;
+  }
   const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
-  T* y = static_cast<T*>(a.y) + (long long)b * a.M + m;
+  T* y = static_cast<T*>(a.y) + (long long)b * a.M;
   if (slot < 0) {
-    if (ok && sl == 0) *y = from_f32<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      if (first + i * CH < a.M && sl == 0) y[first + i * CH] = from_f32<T>(0.f);
     return;
   }
-  float out = 0.f, uv = 0.f;
-  if (ok) {
-    float* state = a.state + (slot * a.M + m) * a.N;
-    const int g = (int)(m / (a.M / a.G));
-    const T* Bm = static_cast<const T*>(a.Bm) + b * a.B_stride[0] + g * a.B_stride[1];
-    const T* C = static_cast<const T*>(a.C) + b * a.C_stride[0] + g * a.C_stride[1];
-    float h[S], A2[S];
-    load4(h, state, n0, a.N, true, wide);
-    load4(A2, a.A + m * a.N, n0, a.N, true, wide);
-    uv = to_f32(static_cast<const T*>(a.u)[b * a.u_stride + m]);
-    const float d = step_of(to_f32(static_cast<const T*>(a.dt)[b * a.dt_stride + m]), a.dt_bias != nullptr ? a.dt_bias[m] : 0.f, a.softplus);
+  float h[U][S], out[U];
 #pragma unroll
-    for (int i = 0; i < S; i++) {
-      const bool real = n0 + i < a.N;
-      const float Bv = real ? to_f32(Bm[n0 + i]) : 0.f, Cv = real ? to_f32(C[n0 + i]) : 0.f;
-      h[i] = fmaf(ex2(d * (A2[i] * LOG2E)), h[i], d * uv * Bv);
-      out = fmaf(Cv, h[i], out);
+  for (int i = 0; i < U; i++) load4(h[i], a.state + (slot * a.M + first + i * CH) * a.N, n0, a.N, first + i * CH < a.M, wide);
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    float sig;
+    if (a.softplus) d[i] = softplus_fast(d[i], sig);
+    out[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      h[i][k] = fmaf(ex2(d[i] * (A2[i][k] * LOG2E)), h[i][k], d[i] * u[i] * to_f32(Bv[i].v[k]));
+      out[i] = fmaf(to_f32(Cv[i].v[k]), h[i][k], out[i]);
     }
-    store4(state, h, n0, a.N, true, wide);
+    store4(a.state + (slot * a.M + first + i * CH) * a.N, h[i], n0, a.N, first + i * CH < a.M, wide);
   }
 #pragma unroll
-  for (int k = L / 2; k > 0; k >>= 1) out += __shfl_xor_sync(0xffffffffu, out, k);
-  if (ok && sl == 0) {
-    if (a.D != nullptr) out = fmaf(a.D[m], uv, out);
-    if (a.z != nullptr) {
-      const float g = to_f32(static_cast<const T*>(a.z)[b * a.z_stride + m]);
-      out *= g * sigmoid_fast(g);
-    }
-    *y = from_f32<T>(out);
+  for (int k = L / 2; k > 0; k >>= 1)
+#pragma unroll
+    for (int i = 0; i < U; i++) out[i] += __shfl_xor_sync(0xffffffffu, out[i], k);
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    out[i] = fmaf(D[i], u[i], out[i]);
+    if (a.z != nullptr) out[i] *= z[i] * sigmoid_fast(z[i]);
+    if (first + i * CH < a.M && sl == 0) y[first + i * CH] = from_f32<T>(out[i]);
   }
 }
 
@@ -875,13 +1054,20 @@ extern "C" int rewy_scan_fwd(const RewyScanArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->y != nullptr, REWY_ERR_NULL, "y is NULL");
   const ScanParams p = scan_params(*a, plan);
   const cudaStream_t s = (cudaStream_t)st;
+  cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     with_lanes(a->N, [&](auto l) {
       using T = decltype(t);
-      if (plan.segments > 1) scan_fwd_kernel<T, l.value, true><<<(unsigned)(plan.ctas * (plan.segments - 1)), NT, 0, s>>>(p);
-      scan_fwd_kernel<T, l.value, false><<<(unsigned)(plan.ctas * plan.segments), NT, 0, s>>>(p);
+      constexpr int L = l.value, bytes = sizeof(FwdShared<L>);
+      if (plan.segments > 1) {
+        e = ensure_dynamic_smem<scan_fwd_kernel<T, L, true>>(bytes);
+        if (e == cudaSuccess) scan_fwd_kernel<T, L, true><<<(unsigned)(plan.ctas * (plan.segments - 1)), 2 * NT, bytes, s>>>(p);
+      }
+      if (e == cudaSuccess) e = ensure_dynamic_smem<scan_fwd_kernel<T, L, false>>(bytes);
+      if (e == cudaSuccess) scan_fwd_kernel<T, L, false><<<(unsigned)(plan.ctas * plan.segments), 2 * NT, bytes, s>>>(p);
     });
   });
+  if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
   return launched("selective scan forward", plan.segments > 1 ? 2 : 1);
 }
 
@@ -901,7 +1087,7 @@ extern "C" int rewy_scan_bwd(const RewyScanArgs* a, rewy_stream_t st) {
       e = ensure_dynamic_smem<scan_bwd_kernel<T, L>>(sizeof(BwdShared<L>));
       if (e != cudaSuccess) return;
       if (plan.segments > 1) scan_bwd_state_kernel<T, L><<<(unsigned)(plan.ctas * (plan.segments - 1)), NT, 0, s>>>(p);
-      scan_bwd_kernel<T, L><<<(unsigned)(plan.ctas * plan.segments), NT, sizeof(BwdShared<L>), s>>>(p);
+      scan_bwd_kernel<T, L><<<(unsigned)(plan.ctas * plan.segments), 2 * NT, sizeof(BwdShared<L>), s>>>(p);
     });
     if (e != cudaSuccess) return;
     const long long rows = (long long)a->B * a->T * a->G;
@@ -923,10 +1109,12 @@ extern "C" int rewy_scan_step(const RewyScanStepArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->u != nullptr && a->dt != nullptr && a->Bm != nullptr && a->C != nullptr && a->A != nullptr && a->state != nullptr && a->y != nullptr,
                 REWY_ERR_NULL, "a required pointer of the scan step is NULL");
   const bool wide = a->N % 4 == 0 && !unaligned16(a->state) && !unaligned16(a->A);
+  bool wide_bc = a->N % 4 == 0 && !unaligned16(a->Bm) && !unaligned16(a->C);
+  for (int i = 0; i < 2; i++) wide_bc = wide_bc && a->B_stride[i] % 4 == 0 && a->C_stride[i] % 4 == 0;
   with_type(a->dtype, [&](auto t) {
     with_lanes(a->N, [&](auto l) {
-      const int CH = NT / l.value, blocks = (a->M + CH - 1) / CH;
-      scan_step_kernel<decltype(t), l.value><<<(unsigned)((long long)blocks * a->B), NT, 0, (cudaStream_t)st>>>(*a, blocks, wide);
+      const int per = NT / l.value * 2, blocks = (a->M + per - 1) / per;
+      scan_step_kernel<decltype(t), l.value><<<(unsigned)((long long)blocks * a->B), NT, 0, (cudaStream_t)st>>>(*a, blocks, wide, wide_bc);
     });
   });
   return launched("selective scan step");
