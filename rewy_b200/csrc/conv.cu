@@ -16,7 +16,9 @@ namespace rewy {
 namespace {
 
 constexpr int WARPS = 8;
-constexpr int FWD_V = 4, BWD_V = 2;  // neighbouring channels per lane
+template <class T>
+constexpr int lane_channels() { return 8 / sizeof(T); }
+constexpr int U = 4, RING = 4;  // tokens per group of copies; groups that a thread's ring holds
 
 struct ConvParams {
   RewyConvArgs a;
@@ -37,18 +39,18 @@ __device__ __forceinline__ Span span_after(const RewyConvArgs& a, const Span& p)
   return {s, p.end, s + 1 < a.num_seqs ? min(max(a.cu_seqlens[s + 1], p.end + 1), a.T) : a.T};
 }
 
-template <class T, int W, int V>
+template <class T, int W, int V, bool WIDE>
 struct Columns {  // a warp's channels
   const RewyConvArgs& a;
   const T* x;
   long long state_row;  // elements of one sequence's state
   int c0, valid;
-  bool wide;
+  static constexpr bool wide = WIDE;
   float weight[W][V], bias[V];
 
   __device__ __forceinline__ Columns(const ConvParams& p, int b, int channel)
       : a(p.a), x(static_cast<const T*>(p.a.x) + b * p.a.x_batch_stride), state_row((long long)(W - 1) * p.a.D), c0(channel),
-        valid(p.a.D - channel), wide(p.wide) {
+        valid(WIDE ? V : p.a.D - channel) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
 #pragma unroll
@@ -68,22 +70,47 @@ struct Columns {  // a warp's channels
       else if (a.initial_state != nullptr)
         load_some<T, V>(v, static_cast<const T*>(a.initial_state) + s.s * state_row + (long long)(W - 1 + pos - s.begin) * a.D + c0, valid, wide);
       else zero_pack(v);
-#pragma unroll
-      for (int i = 0; i < V; i++) win[j][i] = to_f32(v.v[i]);
+      to_floats(win[j], v);
     }
   }
 };
 
-template <class T, int W, int V>
-__global__ void __launch_bounds__(WARPS * 32, 3) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
-  constexpr int U = 4;
+// A thread's inputs on their way through shared memory, N tensors, U tokens at a time: three groups are under way while one is
+// worked on, without registers that hold them.  A thread reads only what it has copied itself.
+template <class T, int V, int N>
+struct Ring {
+  using P = Pack<T, V>;
+  static constexpr int BYTES = RING * U * N * WARPS * 32 * (int)sizeof(P);
+  P* own;      // of this thread; its slots are a CTA's width apart
+  __device__ __forceinline__ explicit Ring(unsigned char* smem) : own(reinterpret_cast<P*>(smem) + threadIdx.x) {}
+  __device__ __forceinline__ P& slot(int group, int u, int i) const { return own[(((group & (RING - 1)) * U + u) * N + i) * WARPS * 32]; }
+  __device__ __forceinline__ void copy(int group, int u, int i, const T* from, int valid, bool wide) const {
+    P& to = slot(group, u, i);
+    if (wide && valid >= V) {
+      const unsigned dst = (unsigned)__cvta_generic_to_shared(&to);
+      static_assert(sizeof(P) == 8, "one copy is eight bytes");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(from) : "memory");
+    } else {
+      load_some<T, V>(to, from, valid, false);
+    }
+  }
+  __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory"); }
+  __device__ __forceinline__ static void wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+};
+
+// WIDE: whole accesses only
+template <class T, int W, int V, bool WIDE>
+__global__ void __launch_bounds__(WARPS * 32, 4) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring<T, V, 1> ring(smem);
   const int channel = (blockIdx.x % p.channel_blocks * 32 + (threadIdx.x & 31)) * V;
   const unsigned rest = blockIdx.x / p.channel_blocks;
   const int b = rest / p.token_blocks;
   const long long first = ((long long)(rest % p.token_blocks) * WARPS + (threadIdx.x >> 5)) * p.token_block;
   if (channel >= p.a.D || first >= p.a.T) return;
   const int t0 = (int)first, t1 = (int)min(first + p.token_block, (long long)p.a.T);
-  const Columns<T, W, V> c(p, b, channel);
+  const Columns<T, W, V, WIDE> c(p, b, channel);
   T* y = static_cast<T*>(p.a.y) + (long long)b * p.a.T * p.a.D + channel;
   Span s = span_at(p.a, b, t0);
   for (int from = t0; from < t1;) {   // the part of one sequence that lies in the block
@@ -91,44 +118,51 @@ __global__ void __launch_bounds__(WARPS * 32, 3) conv_fwd_kernel(const __grid_co
     float win[W - 1][V];
     c.window(win, s, from);
     auto token = [&](int t, const Pack<T, V>& in) {
-      Pack<T, V> out;
+      float now[V], pre[V];
+      to_floats(now, in);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float now = to_f32(in.v[i]);
-        float pre = fmaf(c.weight[W - 1][i], now, c.bias[i]);
+        pre[i] = fmaf(c.weight[W - 1][i], now[i], c.bias[i]);
 #pragma unroll
-        for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
-        out.v[i] = from_f32<T>(p.a.activation ? pre * sigmoid_fast(pre) : pre);
+        for (int w = 0; w < W - 1; w++) pre[i] = fmaf(c.weight[w][i], win[w][i], pre[i]);
 #pragma unroll
         for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
-        win[W - 2][i] = now;
+        win[W - 2][i] = now[i];
       }
+      if (p.a.activation)
+#pragma unroll
+        for (int i = 0; i < V; i++) pre[i] *= sigmoid_fast(pre[i]);
+      Pack<T, V> out;
+      from_floats(out, pre);
       store_some<T, V>(y + (long long)t * p.a.D, out, c.valid, c.wide);
     };
-    Pack<T, V> in[U], next[U];
-    int t = from;
-    if (t + U <= to)
+    auto ask = [&](int group) {
 #pragma unroll
-      for (int u = 0; u < U; u++) c.load_x(in[u], t + u);
-    for (; t + U <= to; t += U) {      // the next rows are under way while these are worked on
-      if (t + 2 * U <= to)
+      for (int u = 0; u < U; u++) {
+        const int t = from + group * U + u;
+        if (t < to) ring.copy(group, u, 0, c.x + t * p.a.x_token_stride + channel, c.valid, c.wide);
+      }
+      ring.commit();
+    };
 #pragma unroll
-        for (int u = 0; u < U; u++) c.load_x(next[u], t + U + u);
+    for (int k = 0; k < RING - 1; k++) ask(k);
+    for (int k = 0; from + k * U < to; k++) {
+      ask(k + RING - 1);
+      ring.wait();
+      if (from + k * U + U <= to) {
 #pragma unroll
-      for (int u = 0; u < U; u++) token(t + u, in[u]);
-#pragma unroll
-      for (int u = 0; u < U; u++) in[u] = next[u];
+        for (int u = 0; u < U; u++) token(from + k * U + u, ring.slot(k, u, 0));
+      } else {
+#pragma unroll 1
+        for (int u = 0; from + k * U + u < to; u++) token(from + k * U + u, ring.slot(k, u, 0));
+      }
     }
-    for (; t < to; t++) {
-      c.load_x(in[0], t);
-      token(t, in[0]);
-    }
+    ring.wait_all();
     if (p.a.final_state != nullptr && to == s.end) {
 #pragma unroll
       for (int j = 0; j < W - 1; j++) {
         Pack<T, V> v;
-#pragma unroll
-        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(win[j][i]);
+        from_floats(v, win[j]);
         store_some<T, V>(static_cast<T*>(p.a.final_state) + s.s * c.state_row + (long long)j * p.a.D + channel, v, c.valid, c.wide);
       }
     }
@@ -137,10 +171,10 @@ __global__ void __launch_bounds__(WARPS * 32, 3) conv_fwd_kernel(const __grid_co
   }
 }
 
-template <class T, int W, int V>
-__global__ void __launch_bounds__(WARPS * 32, 3) conv_bwd_kernel(const __grid_constant__ ConvParams p, float* __restrict__ partial) {
-  constexpr int U = 4;
-  __shared__ float sums[WARPS][W + 1][32 * V];
+template <class T, int W, int V, bool WIDE>
+__global__ void __launch_bounds__(WARPS * 32, 2) conv_bwd_kernel(const __grid_constant__ ConvParams p, float* __restrict__ partial) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring<T, V, 2> ring(smem);
   const RewyConvArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int channel = (blockIdx.x % p.channel_blocks * 32 + lane) * V;
@@ -150,7 +184,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) conv_bwd_kernel(const __grid_co
   float dw[W][V] = {}, db[V] = {};
   if (channel < a.D && first < a.T) {
     const int t0 = (int)first, t1 = (int)min(first + p.token_block, (long long)a.T);
-    const Columns<T, W, V> c(p, b, channel);
+    const Columns<T, W, V, WIDE> c(p, b, channel);
     const long long row = (long long)b * a.T;
     const T* dy = static_cast<const T*>(a.dy) + row * a.D + channel;
     T* dx = static_cast<T*>(a.dx) + row * a.D + channel;
@@ -159,44 +193,54 @@ __global__ void __launch_bounds__(WARPS * 32, 3) conv_bwd_kernel(const __grid_co
       const int to = min(t1, s.end);
       float win[W - 1][V], g[W - 1][V] = {};
       c.window(win, s, from);
-      auto load = [&](Pack<T, V>& x, Pack<T, V>& d, int t) {
-        c.load_x(x, t);
-        load_some<T, V>(d, dy + (long long)t * a.D, c.valid, c.wide);
+      const int stop = to + W - 1, real = min(stop, s.end);   // tokens of the next block too; beyond the sequence there is no g
+      auto ask = [&](int group) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const int t = from + group * U + u;
+          if (t < real) {
+            ring.copy(group, u, 0, c.x + t * a.x_token_stride + channel, c.valid, c.wide);
+            ring.copy(group, u, 1, dy + (long long)t * a.D, c.valid, c.wide);
+          }
+        }
+        ring.commit();
       };
       // Token t of the sequence: its g, and out, the complete gradient W-1 tokens before it.  OWN: it counts for dweight.
       auto step = [&](auto own, const Pack<T, V>& in, const Pack<T, V>& d, float (&out)[V]) {
+        float x[V], gi[V];
+        to_floats(x, in);
+        to_floats(gi, d);
+        if (a.activation)
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          const float x = to_f32(in.v[i]);
-          float gi = to_f32(d.v[i]);
-          if (a.activation) {
-            float pre = fmaf(c.weight[W - 1][i], x, c.bias[i]);
+          for (int i = 0; i < V; i++) {
+            float pre = fmaf(c.weight[W - 1][i], x[i], c.bias[i]);
 #pragma unroll
             for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
             const float sig = sigmoid_fast(pre);
-            gi *= sig * fmaf(pre, 1.f - sig, 1.f);
+            gi[i] *= sig * fmaf(pre, 1.f - sig, 1.f);
           }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
           if (own.value) {
 #pragma unroll
-            for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi, win[w][i], dw[w][i]);
-            dw[W - 1][i] = fmaf(gi, x, dw[W - 1][i]);
-            db[i] += gi;
+            for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi[i], win[w][i], dw[w][i]);
+            dw[W - 1][i] = fmaf(gi[i], x[i], dw[W - 1][i]);
+            db[i] += gi[i];
           }
 #pragma unroll
           for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
-          win[W - 2][i] = x;
-          out[i] = c.weight[0][i] * gi;
+          win[W - 2][i] = x[i];
+          out[i] = c.weight[0][i] * gi[i];
 #pragma unroll
           for (int w = 1; w < W; w++) out[i] = fmaf(c.weight[w][i], g[W - 1 - w][i], out[i]);
 #pragma unroll
           for (int j = 0; j < W - 2; j++) g[j][i] = g[j + 1][i];
-          g[W - 2][i] = gi;
+          g[W - 2][i] = gi[i];
         }
       };
       auto put = [&](int pos, float (&out)[V]) {
         Pack<T, V> v;
-#pragma unroll
-        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
+        from_floats(v, out);
         store_some<T, V>(dx + (long long)pos * a.D, v, c.valid, c.wide);
       };
       // At the edges: rows before the sequence are its initial state's, the last ones get the final state's gradient too.
@@ -215,51 +259,46 @@ __global__ void __launch_bounds__(WARPS * 32, 3) conv_bwd_kernel(const __grid_co
           return;
         }
         Pack<T, V> v;
-#pragma unroll
-        for (int i = 0; i < V; i++) v.v[i] = from_f32<T>(out[i]);
+        from_floats(v, out);
         store_some<T, V>(static_cast<T*>(a.dinitial_state) + s.s * c.state_row + (long long)(W - 1 + pos - s.begin) * a.D + channel, v, c.valid, c.wide);
       };
       float out[V];
-      int t = from;
-      Pack<T, V> in[U], d[U], next[U], nd[U];
+#pragma unroll
+      for (int k = 0; k < RING - 1; k++) ask(k);
+      for (int k = 0; from + k * U < stop; k++) {
+        const int t = from + k * U;
+        ask(k + RING - 1);
+        ring.wait();
+        if (t >= from + W - 1 && t + U <= to) {
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            step(std::true_type(), ring.slot(k, u, 0), ring.slot(k, u, 1), out);
+            put(t + u - (W - 1), out);
+          }
+        } else {       // the first tokens, the last ones and those of the next block
 #pragma unroll 1
-      for (; t < min(from + W - 1, to); t++) {
-        load(in[0], d[0], t);
-        step(std::true_type(), in[0], d[0], out);
-        put_edge(t - (W - 1), out);
-      }
-      if (t + U <= to)
-#pragma unroll
-        for (int u = 0; u < U; u++) load(in[u], d[u], t + u);
-      for (; t + U <= to; t += U) {   // the next rows are under way while these are worked on
-        if (t + 2 * U <= to)
-#pragma unroll
-          for (int u = 0; u < U; u++) load(next[u], nd[u], t + U + u);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          step(std::true_type(), in[u], d[u], out);
-          put(t + u - (W - 1), out);
+          for (int u = 0; u < U && t + u < stop; u++) {
+            Pack<T, V> in, d;
+            zero_pack(in);
+            zero_pack(d);
+            if (t + u < real) {
+              in = ring.slot(k, u, 0);
+              d = ring.slot(k, u, 1);
+            }
+            if (t + u < to) step(std::true_type(), in, d, out);
+            else step(std::false_type(), in, d, out);
+            put_edge(t + u - (W - 1), out);
+          }
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) { in[u] = next[u]; d[u] = nd[u]; }
       }
-#pragma unroll 1
-      for (; t < to; t++) {
-        load(in[0], d[0], t);
-        step(std::true_type(), in[0], d[0], out);
-        put(t - (W - 1), out);
-      }
-#pragma unroll 1
-      for (; t < to + W - 1; t++) {   // tokens of the next block, and beyond the sequence, where there is no g
-        if (t < s.end) load(in[0], d[0], t);
-        else { zero_pack(in[0]); zero_pack(d[0]); }
-        step(std::false_type(), in[0], d[0], out);
-        put_edge(t - (W - 1), out);
-      }
+      ring.wait_all();
       from = to;
       if (from < t1) s = span_after(a, s);
     }
   }
+  __syncthreads();   // the rings have been read: their room takes the sums
+  float(*const sums)[W + 1][32 * V] = reinterpret_cast<float(*)[W + 1][32 * V]>(smem);
+  static_assert(sizeof(float) * WARPS * (W + 1) * 32 * V <= Ring<T, V, 2>::BYTES, "the sums fit the rings");
 #pragma unroll
   for (int i = 0; i < V; i++) {
 #pragma unroll
@@ -347,7 +386,7 @@ int check_conv(const RewyConvArgs* a) {
 // Tokens per warp.  Long blocks load fewer rows twice (W-1 per block) and leave fewer sums; short ones give a small problem
 // enough warps: B=1 T=2000 D=1024 has 4 warps of channels, blocks of 8 make 1000 warps of them.
 int token_block(long long tokens, int warps_per_token) {
-  int block = 32;
+  int block = 64;
   while (block > 8 && tokens / block * warps_per_token < 148 * 24) block /= 2;
   return block;
 }
@@ -357,7 +396,7 @@ ConvParams conv_params(const RewyConvArgs& a, int V, bool rows_wide) {
   p.a = a;
   const int e = element_bytes(a.dtype), access = V * e;
   p.channel_blocks = (a.D + 32 * V - 1) / (32 * V);
-  p.token_block = token_block((long long)a.B * a.T, p.channel_blocks);
+  p.token_block = token_block((long long)a.B * a.T, (a.D + 127) / 128);
   p.token_blocks = (a.T + p.token_block * WARPS - 1) / (p.token_block * WARPS);
   auto row = [&](const void* q) { return (reinterpret_cast<uintptr_t>(q) % access) == 0; };
   p.wide = rows_wide && a.D % V == 0 && a.x_token_stride % V == 0 && a.x_batch_stride % V == 0 && row(a.x) && row(a.y) && row(a.dy) && row(a.dx) &&
@@ -379,13 +418,21 @@ using namespace rewy;
 extern "C" int rewy_conv_fwd(const RewyConvArgs* a, rewy_stream_t st) {
   if (const int rc = check_conv(a)) return rc;
   LAYER_REQUIRE(a->y != nullptr, REWY_ERR_NULL, "y is NULL");
+  cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = FWD_V;
+    constexpr int V = lane_channels<T>(), bytes = Ring<T, V, 1>::BYTES;
     const ConvParams p = conv_params(*a, V, true);
     const unsigned grid = (unsigned)((long long)p.channel_blocks * p.token_blocks * a->B);
-    with_taps(a->W, [&](auto w) { conv_fwd_kernel<T, w.value, V><<<grid, WARPS * 32, 0, (cudaStream_t)st>>>(p); });
+    with_taps(a->W, [&](auto w) {
+      auto go = [&](auto wide) {
+        e = ensure_dynamic_smem<conv_fwd_kernel<T, w.value, V, wide.value>>(bytes);
+        if (e == cudaSuccess) conv_fwd_kernel<T, w.value, V, wide.value><<<grid, WARPS * 32, bytes, (cudaStream_t)st>>>(p);
+      };
+      p.wide ? go(std::true_type()) : go(std::false_type());
+    });
   });
+  if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
   return launched("causal convolution forward");
 }
 
@@ -393,7 +440,7 @@ extern "C" size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D,
   if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4) return 0;
   RewyConvArgs a{};
   a.B = B; a.T = T; a.D = D; a.W = W;
-  const ConvParams p = conv_params(a, BWD_V, true);
+  const ConvParams p = conv_params(a, 4, true);
   return (size_t)p.token_blocks * B * (W + 1) * D * sizeof(float);
 }
 
@@ -402,15 +449,24 @@ extern "C" int rewy_conv_bwd(const RewyConvArgs* a, rewy_stream_t st) {
   LAYER_REQUIRE(a->dy != nullptr && a->dx != nullptr && a->dweight != nullptr, REWY_ERR_NULL, "dy, dx or dweight is NULL");
   LAYER_REQUIRE(a->workspace != nullptr && a->workspace_bytes >= rewy_conv_bwd_workspace_bytes(a->B, a->T, a->D, a->W), REWY_ERR_WORKSPACE,
                 "the workspace of the convolution backward is too small");
-  constexpr int V = BWD_V;
-  const ConvParams p = conv_params(*a, V, true);
-  const int parts = p.token_blocks * a->B;
   float* partial = static_cast<float*>(a->workspace);
+  int parts = 0;
+  cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
+    constexpr int V = lane_channels<T>(), bytes = Ring<T, V, 2>::BYTES;
+    const ConvParams p = conv_params(*a, V, true);
+    parts = p.token_blocks * a->B;
     const unsigned grid = (unsigned)((long long)p.channel_blocks * parts);
-    with_taps(a->W, [&](auto w) { conv_bwd_kernel<T, w.value, V><<<grid, WARPS * 32, 0, (cudaStream_t)st>>>(p, partial); });
+    with_taps(a->W, [&](auto w) {
+      auto go = [&](auto wide) {
+        e = ensure_dynamic_smem<conv_bwd_kernel<T, w.value, V, wide.value>>(bytes);
+        if (e == cudaSuccess) conv_bwd_kernel<T, w.value, V, wide.value><<<grid, WARPS * 32, bytes, (cudaStream_t)st>>>(p, partial);
+      };
+      p.wide ? go(std::true_type()) : go(std::false_type());
+    });
   });
+  if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
   conv_sums_kernel<<<(unsigned)(((long long)(a->W + 1) * a->D + 255) / 256), 256, 0, (cudaStream_t)st>>>(partial, parts, a->D, a->W, a->dweight, a->dbias,
                                                                                                          a->param_dtype);
   return launched("causal convolution backward", 2);

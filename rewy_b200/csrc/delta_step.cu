@@ -33,7 +33,7 @@ __device__ __forceinline__ void store_state(float* p, float4 x, int valid) {
 
 // WIDE: every row of the state starts on 16 bytes and holds whole groups of four
 template <class T, bool V_FIRST, bool WIDE>
-__global__ void __launch_bounds__(NT, 6) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices) {
+__global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices) {
   __shared__ float sk[NT], sq[NT], serase[NT], sdecay[NT], red[4][3], part[4][2][SLICE];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x % slices;

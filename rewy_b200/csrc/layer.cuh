@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdio>
+#include <type_traits>
 #include "common.cuh"
 
 namespace rewy {
@@ -60,6 +61,46 @@ template <class T, int V>
 __device__ __forceinline__ void zero_pack(Pack<T, V>& d) {
 #pragma unroll
   for (int i = 0; i < V; i++) d.v[i] = from_f32<T>(0.f);
+}
+// All elements of a group as FP32 and back, two 16-bit elements per instruction
+template <class T, int V>
+__device__ __forceinline__ void to_floats(float (&f)[V], const Pack<T, V>& p) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i++) f[i] = to_f32(p.v[i]);
+  } else {
+    static_assert(V % 2 == 0, "pairs");
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) {
+      const uint32_t u = reinterpret_cast<const uint32_t*>(&p)[i];
+      if constexpr (std::is_same_v<T, bf16>) {
+        f[2 * i] = __uint_as_float(u << 16);
+        f[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+      } else {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        f[2 * i] = x.x; f[2 * i + 1] = x.y;
+      }
+    }
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void from_floats(Pack<T, V>& p, const float (&f)[V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i++) p.v[i] = from_f32<T>(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) {
+      uint32_t u;
+      if constexpr (std::is_same_v<T, bf16>) {
+        u = pack_bf16(f[2 * i], f[2 * i + 1]);
+      } else {
+        const __half2 x = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        u = *reinterpret_cast<const uint32_t*>(&x);
+      }
+      reinterpret_cast<uint32_t*>(&p)[i] = u;
+    }
+  }
 }
 // V elements of which the first `valid` exist; `wide`: the address is aligned for whole accesses
 template <class T, int V>

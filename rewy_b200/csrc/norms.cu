@@ -23,8 +23,10 @@ struct NormParams {
   float* partial;  // [CTAs][2][D]
 };
 
-__device__ __forceinline__ long long row_start(long long r, long long inner, const int64_t (&stride)[2]) {
-  const long long o = r / inner;
+// (rows at one distance need no division; fewer than 2^32 rows a short one)
+__device__ __forceinline__ long long row_start(long long r, long long inner, long long rows, const int64_t (&stride)[2]) {
+  if (inner >= rows) return r * stride[1];
+  const long long o = rows <= 0xffffffffLL ? (long long)((unsigned)r / (unsigned)inner) : r / inner;
   return o * stride[0] + (r - o * inner) * stride[1];
 }
 
@@ -198,11 +200,23 @@ __device__ __forceinline__ void read8(float (&x)[E], const float* p) {
   const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
   x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
-template <int N>
-__device__ __forceinline__ float act_of(float g, int activation, float& slope) {
+// act(g) and, if asked for, act'(g)
+template <bool SILU, bool SLOPE>
+__device__ __forceinline__ float act_of(float g, float& slope) {
   const float sig = sigmoid_fast(g);
-  if constexpr (N > 0) slope = activation == 0 ? sig * fmaf(g, 1.f - sig, 1.f) : sig * (1.f - sig);
-  return activation == 0 ? g * sig : sig;
+  if constexpr (SLOPE) slope = SILU ? sig * fmaf(g, 1.f - sig, 1.f) : sig * (1.f - sig);
+  return SILU ? g * sig : sig;
+}
+// f(SiLU?, gate first?) with both as types: what is asked once stands outside the loops over elements
+template <class F>
+__device__ __forceinline__ void with_gate(const RewyNormArgs& a, F&& f) {
+  if (a.activation == 0) {
+    if (a.gate_first) f(std::true_type(), std::true_type());
+    else f(std::true_type(), std::false_type());
+  } else {
+    if (a.gate_first) f(std::false_type(), std::true_type());
+    else f(std::false_type(), std::false_type());
+  }
 }
 
 // CTAs on an SM that the registers are cut for
@@ -232,35 +246,42 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
   GatedFwd<T, TPR, NV> in;
   in.smem = smem; in.wide = p.wide;
   auto point = [&](long long r) {
-    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
-    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.other_stride);
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.rows, a.x_stride);
+    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.rows, a.other_stride);
   };
-  for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
-    float t[NV][E], sum[1] = {0.f}, slope;   // what is normalised, times what stands behind the norm
+  with_gate(a, [&](auto silu, auto gate_first) {
+    for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
+      float t[NV][E], sum[1] = {0.f}, slope;   // what is normalised, times what stands behind the norm
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+      for (int v = 0; v < NV; v++) {
+        float g[E];
+        to_floats(t[v], in.pa[0][v]);
+        to_floats(g, in.pa[1][v]);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float x = to_f32(in.pa[0][v].v[e]), act = act_of<0>(to_f32(in.pa[1][v].v[e]), a.activation, slope);
-        t[v][e] = x * act;
-        const float n = a.gate_first ? t[v][e] : x;
-        sum[0] = fmaf(n, n, sum[0]);       // elements that do not exist are zero
+        for (int e = 0; e < E; e++) {            // elements that do not exist are zero
+          const float x = t[v][e];
+          t[v][e] = x * act_of<silu.value, false>(g[e], slope);
+          const float n = gate_first.value ? t[v][e] : x;
+          sum[0] = fmaf(n, n, sum[0]);
+        }
       }
-    row_sums<TPR>(sum, red, parity);
-    const float rs = rsqrtf(sum[0] / a.D + a.eps);
-    if (!real) return;
-    T* y = static_cast<T*>(a.y) + r * a.D;
+      row_sums<TPR>(sum, red, parity);
+      const float rs = rsqrtf(sum[0] / a.D + a.eps);
+      if (!real) return;
+      T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v);
-      if (c >= a.D) continue;
-      float wv[E];
-      read8(wv, w + c);
-      Pack<T, E> out;
+      for (int v = 0; v < NV; v++) {
+        const int c = Y::column(v);
+        if (c >= a.D) continue;
+        float wv[E];
+        read8(wv, w + c);
+        Pack<T, E> out;
 #pragma unroll
-      for (int e = 0; e < E; e++) out.v[e] = from_f32<T>(t[v][e] * rs * wv[e]);
-      store_some<T, E>(y + c, out, a.D - c, p.wide);
-    }
+        for (int e = 0; e < E; e++) wv[e] *= t[v][e] * rs;
+        from_floats(out, wv);
+        store_some<T, E>(y + c, out, a.D - c, p.wide);
+      }
+    });
   });
 }
 
@@ -277,47 +298,55 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
   GatedBwd<T, TPR, NV> in;
   in.smem = smem; in.wide = p.wide;
   auto point = [&](long long r) {
-    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
-    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.other_stride);
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.rows, a.x_stride);
+    in.a[1] = static_cast<const T*>(a.gate) + row_start(r, a.other_inner, a.rows, a.other_stride);
     in.a[2] = static_cast<const T*>(a.dy) + r * a.D;
   };
-  for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
-    float sum[2] = {0.f, 0.f}, slope;
+  with_gate(a, [&](auto silu, auto gate_first) {
+    for_rows<TPR, NV>(in, a.rows, a.D, point, [](int) { return true; }, [&](long long r, bool real, int parity) {
+      float sum[2] = {0.f, 0.f}, slope;
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-      float wv[E];
-      read8(wv, w + Y::column(v));
+      for (int v = 0; v < NV; v++) {
+        float wv[E], x[E], g[E], d[E];
+        read8(wv, w + Y::column(v));
+        to_floats(x, in.pa[0][v]);
+        to_floats(g, in.pa[1][v]);
+        to_floats(d, in.pa[2][v]);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float x = to_f32(in.pa[0][v].v[e]), act = act_of<0>(to_f32(in.pa[1][v].v[e]), a.activation, slope), dn = to_f32(in.pa[2][v].v[e]) * wv[e];
-        const float t = a.gate_first ? x * act : x;
-        sum[0] = fmaf(t, t, sum[0]);
-        sum[1] = fmaf(dn * act, x, sum[1]);    // dn t either way
+        for (int e = 0; e < E; e++) {
+          const float act = act_of<silu.value, false>(g[e], slope), dn = d[e] * wv[e], t = gate_first.value ? x[e] * act : x[e];
+          sum[0] = fmaf(t, t, sum[0]);
+          sum[1] = fmaf(dn * act, x[e], sum[1]);    // dn t either way
+        }
       }
-    }
-    row_sums<TPR>(sum, red, parity);
-    if (!real) return;
-    const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
+      row_sums<TPR>(sum, red, parity);
+      if (!real) return;
+      const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-      const int c = Y::column(v);
-      if (c >= a.D) continue;
-      float wv[E];
-      read8(wv, w + c);
-      Pack<T, E> ox, og;
+      for (int v = 0; v < NV; v++) {
+        const int c = Y::column(v);
+        if (c >= a.D) continue;
+        float wv[E], x[E], g[E], d[E];
+        read8(wv, w + c);
+        to_floats(x, in.pa[0][v]);
+        to_floats(g, in.pa[1][v]);
+        to_floats(d, in.pa[2][v]);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float act = act_of<1>(to_f32(in.pa[1][v].v[e]), a.activation, slope);
-        const float xv = to_f32(in.pa[0][v].v[e]), d = to_f32(in.pa[2][v].v[e]), dn = d * wv[e];
-        // gate first: v = x act, dx = dv act, dgate = dv x act'.  Else dgate = dn n act', dx = r dn act - back x
-        const float dv = a.gate_first ? fmaf(rs, dn, -back * (xv * act)) : rs * dn;
-        ox.v[e] = from_f32<T>(a.gate_first ? dv * act : fmaf(dv, act, -back * xv));
-        og.v[e] = from_f32<T>(dv * xv * slope);
-        dw[v][e] = fmaf(d, xv * act * rs, dw[v][e]);
+        for (int e = 0; e < E; e++) {
+          const float act = act_of<silu.value, true>(g[e], slope), xv = x[e], dn = d[e] * wv[e];
+          // gate first: v = x act, dx = dv act, dgate = dv x act'.  Else dgate = dn n act', dx = r dn act - back x
+          const float dv = gate_first.value ? fmaf(rs, dn, -back * (xv * act)) : rs * dn;
+          x[e] = gate_first.value ? dv * act : fmaf(dv, act, -back * xv);
+          g[e] = dv * xv * slope;
+          dw[v][e] = fmaf(d[e], xv * act * rs, dw[v][e]);
+        }
+        Pack<T, E> ox, og;
+        from_floats(ox, x);
+        from_floats(og, g);
+        store_some<T, E>(static_cast<T*>(a.dx) + r * a.D + c, ox, a.D - c, p.wide);
+        store_some<T, E>(static_cast<T*>(a.dgate) + r * a.D + c, og, a.D - c, p.wide);
       }
-      store_some<T, E>(static_cast<T*>(a.dx) + r * a.D + c, ox, a.D - c, p.wide);
-      store_some<T, E>(static_cast<T*>(a.dgate) + r * a.D + c, og, a.D - c, p.wide);
-    }
+    });
   });
   store_column_sums<TPR, NV>(dw, reinterpret_cast<float*>(smem), p.partial + (long long)blockIdx.x * 2 * a.D, a.D);
 }
@@ -337,18 +366,20 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
   in.smem = smem; in.wide = p.wide;
   const bool has = a.residual != nullptr;
   auto point = [&](long long r) {
-    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
-    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.other_stride) : 0);
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.rows, a.x_stride);
+    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.rows, a.other_stride) : 0);
   };
   for_rows<TPR, NV>(in, a.rows, a.D, point, [&](int i) { return i == 0 || has; }, [&](long long r, bool real, int parity) {
     float t[NV][E], sum[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      float sv[E];
+      float sv[E], x[E], res[E];
       read8(sv, s + Y::column(v));
+      to_floats(x, in.pa[0][v]);
+      to_floats(res, in.pb[0][v]);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        t[v][e] = fmaf(sv[e], to_f32(in.pa[0][v].v[e]), to_f32(in.pb[0][v].v[e]));
+        t[v][e] = fmaf(sv[e], x[e], res[e]);
         sum[0] = fmaf(t[v][e], t[v][e], sum[0]);
       }
     }
@@ -364,10 +395,9 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
       Pack<T, E> oy;
       Pack<TR, E> orr;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        oy.v[e] = from_f32<T>(t[v][e] * rs * wv[e]);
-        orr.v[e] = from_f32<TR>(t[v][e]);
-      }
+      for (int e = 0; e < E; e++) wv[e] *= t[v][e] * rs;
+      from_floats(oy, wv);
+      from_floats(orr, t[v]);
       store_some<T, E>(static_cast<T*>(a.y) + r * a.D + c, oy, a.D - c, p.wide);
       store_some<TR, E>(static_cast<TR*>(a.residual_out) + r * a.D + c, orr, a.D - c, p.wide);
     }
@@ -392,9 +422,9 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
   in.smem = smem; in.wide = p.wide;
   const bool has = a.residual != nullptr, back_too = a.dresidual_out != nullptr;
   auto point = [&](long long r) {
-    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.x_stride);
+    in.a[0] = static_cast<const T*>(a.x) + row_start(r, a.x_inner, a.rows, a.x_stride);
     in.a[1] = static_cast<const T*>(a.dy) + r * a.D;
-    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.other_stride) : 0);
+    in.b[0] = static_cast<const TR*>(a.residual) + (has ? row_start(r, a.other_inner, a.rows, a.other_stride) : 0);
     in.b[1] = static_cast<const TR*>(a.dresidual_out) + (back_too ? r * a.D : 0);
   };
   auto scales = [&](float(&sv)[E], int v) {
@@ -407,14 +437,17 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      float wv[E], sv[E];
+      float wv[E], sv[E], x[E], res[E], d[E];
       read8(wv, w + Y::column(v));
       scales(sv, v);
+      to_floats(x, in.pa[0][v]);
+      to_floats(res, in.pb[0][v]);
+      to_floats(d, in.pa[1][v]);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float t = fmaf(sv[e], to_f32(in.pa[0][v].v[e]), to_f32(in.pb[0][v].v[e]));
+        const float t = fmaf(sv[e], x[e], res[e]);
         sum[0] = fmaf(t, t, sum[0]);
-        sum[1] = fmaf(to_f32(in.pa[1][v].v[e]) * wv[e], t, sum[1]);
+        sum[1] = fmaf(d[e] * wv[e], t, sum[1]);
       }
     }
     row_sums<TPR>(sum, red, parity);
@@ -424,20 +457,26 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
       if (c >= a.D) continue;
-      float wv[E], sv[E];
+      float wv[E], sv[E], x[E], res[E], d[E], dro[E];
       read8(wv, w + c);
       scales(sv, v);
+      to_floats(x, in.pa[0][v]);
+      to_floats(res, in.pb[0][v]);
+      to_floats(d, in.pa[1][v]);
+      to_floats(dro, in.pb[1][v]);
       Pack<T, E> ox;
       Pack<TR, E> orr;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float xv = to_f32(in.pa[0][v].v[e]), t = fmaf(sv[e], xv, to_f32(in.pb[0][v].v[e])), d = to_f32(in.pa[1][v].v[e]);
-        const float dt = to_f32(in.pb[1][v].v[e]) + fmaf(rs, d * wv[e], -back * t);
-        ox.v[e] = from_f32<T>(sv[e] * dt);
-        orr.v[e] = from_f32<TR>(dt);
-        dw[v][e] = fmaf(d, t * rs, dw[v][e]);
+        const float xv = x[e], t = fmaf(sv[e], xv, res[e]);
+        const float dt = dro[e] + fmaf(rs, d[e] * wv[e], -back * t);
+        x[e] = sv[e] * dt;
+        res[e] = dt;
+        dw[v][e] = fmaf(d[e], t * rs, dw[v][e]);
         if constexpr (SCALE) ds[v][e] = fmaf(xv, dt, ds[v][e]);
       }
+      from_floats(ox, x);
+      from_floats(orr, res);
       store_some<T, E>(static_cast<T*>(a.dx) + r * a.D + c, ox, a.D - c, p.wide);
       if (has) store_some<TR, E>(static_cast<TR*>(a.dresidual) + r * a.D + c, orr, a.D - c, p.wide);
     }

@@ -26,11 +26,16 @@
 namespace rewy {
 namespace {
 
-constexpr int TT = 32;    // tokens per tile
-constexpr int NT = 128;   // threads that run the recurrence
-constexpr int S = 4;      // states per thread
+constexpr int TILE = 32;  // segments hold a multiple of so many tokens
 constexpr int CK = 16;    // tokens between checkpoints
 constexpr float LN2 = 0.6931471805599453f;
+
+// N <= L S states of a channel: S to a thread, L neighbouring threads.  NS threads run the recurrence of CH channels in tiles of
+// TT tokens, NH threads do what stands around it.
+template <int L_, int S_, int NS_, int NH_, int TT_>
+struct Shape {
+  static constexpr int L = L_, S = S_, P = S_ / 2, NS = NS_, NH = NH_, TT = TT_, CH = NS_ / L_, NP = L_ * S_, YS = CH + 8, THREADS = NS_ + NH_, WARPS = NS_ / 32;
+};
 
 struct ScanParams {
   RewyScanArgs a;
@@ -41,9 +46,9 @@ struct ScanParams {
 };
 
 // Where a CTA works.
-template <int L>
+template <class C>
 struct Place {
-  static constexpr int CH = NT / L, NP = S * L;
+  static constexpr int CH = C::CH;
   int b, seg, g, cb, m0, valid;        // first channel and how many exist
   int t0, t1;                          // tokens of the segment
   __device__ __forceinline__ Place(const ScanParams& p, int seg_offset, int seg_count) {
@@ -75,24 +80,61 @@ struct Sequence {
   }
 };
 
-__device__ __forceinline__ void load4(float (&x)[S], const float* p, int n0, int N, bool ok, bool wide) {
+template <int S>
+__device__ __forceinline__ void load_states(float (&x)[S], const float* p, int n0, int N, bool ok, bool wide) {
   if (ok && wide && n0 < N) {
-    const float4 v = *reinterpret_cast<const float4*>(p + n0);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    if constexpr (S == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + n0);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(p + n0);
+      x[0] = v.x; x[1] = v.y;
+    }
     return;
   }
 #pragma unroll
   for (int i = 0; i < S; i++) x[i] = ok && n0 + i < N ? p[n0 + i] : 0.f;
 }
-__device__ __forceinline__ void store4(float* p, const float (&x)[S], int n0, int N, bool ok, bool wide) {
+template <int S>
+__device__ __forceinline__ void store_states(float* p, const float (&x)[S], int n0, int N, bool ok, bool wide) {
   if (!ok) return;
   if (wide) {
-    if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(x[0], x[1], x[2], x[3]);
+    if (n0 >= N) return;
+    if constexpr (S == 4) *reinterpret_cast<float4*>(p + n0) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<float2*>(p + n0) = make_float2(x[0], x[1]);
     return;
   }
 #pragma unroll
   for (int i = 0; i < S; i++)
     if (n0 + i < N) p[n0 + i] = x[i];
+}
+// The same as pairs
+template <int P>
+__device__ __forceinline__ void load_pairs(F2 (&x)[P], const float* p, int n0, int N, bool ok, bool wide) {
+  float v[2 * P];
+  load_states(v, p, n0, N, ok, wide);
+#pragma unroll
+  for (int i = 0; i < P; i++) x[i] = pair(v[2 * i], v[2 * i + 1]);
+}
+template <int P>
+__device__ __forceinline__ void store_pairs(float* p, const F2 (&x)[P], int n0, int N, bool ok, bool wide) {
+  float v[2 * P];
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const float2 h = halves(x[i]);
+    v[2 * i] = h.x; v[2 * i + 1] = h.y;
+  }
+  store_states(p, v, n0, N, ok, wide);
+}
+// P pairs from shared memory
+template <int P>
+__device__ __forceinline__ void shared_pairs(F2 (&x)[P], const float* p) {
+  if constexpr (P == 2) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+    x[0].v = v.x; x[1].v = v.y;
+  } else {
+    x[0].v = *reinterpret_cast<const unsigned long long*>(p);
+  }
 }
 
 // Sums over the L lanes of a channel, for G sets of four values.  Afterwards lane l of them holds in x[.][0] (L = 2: x[.][0], x[.][1])
@@ -133,32 +175,31 @@ __device__ __forceinline__ void put_sums(float* at, int stride, const float (&x)
   }
 }
 
-// Sums of v (dB and dC of a thread's four states) over the warp's 32 / L channels, the lanes that differ in the bits from L up.
+// Sums of v (dB and dC of a thread's S states) over the warp's 32 / L channels, the lanes that differ in the bits from L up.
 // Each exchange halves the values that a lane is left with; it puts them at places i of a row of [dB | dC] counted from
 // sum_place, where `put` gets them.
-template <int L>
+template <class C>
 __device__ __forceinline__ int sum_place(int lane, int n0) {
-  constexpr int NP = S * L;
-  int base = 0, n = 8;
+  int base = 0, n = 2 * C::S;
 #pragma unroll
-  for (int m = 16; m >= L && n > 1; m >>= 1) {
+  for (int m = 16; m >= C::L && n > 1; m >>= 1) {
     n >>= 1;
     base += lane & m ? n : 0;
   }
-  return (base >> 2) * NP + n0 + (base & 3);
+  return (base / C::S) * C::NP + n0 + base % C::S;
 }
-template <int L, int G, class F>
-__device__ __forceinline__ void sum_channels(float (&v)[G][8], int lane, F&& put) {  // G tokens step by step together
-  int n = 8;
+template <class C, int G, class F>
+__device__ __forceinline__ void sum_channels(float (&v)[G][2 * C::S], int lane, F&& put) {  // G tokens step by step together
+  int n = 2 * C::S;
 #pragma unroll
-  for (int m = 16; m >= L; m >>= 1) {
+  for (int m = 16; m >= C::L; m >>= 1) {
     const bool up = lane & m;
     if (n > 1) {
       n >>= 1;
 #pragma unroll
       for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < C::S; i++)
           if (i < n) {
             const float keep = up ? v[g][i + n] : v[g][i], give = up ? v[g][i] : v[g][i + n];
             v[g][i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
@@ -171,7 +212,7 @@ __device__ __forceinline__ void sum_channels(float (&v)[G][8], int lane, F&& put
 #pragma unroll
   for (int g = 0; g < G; g++)
 #pragma unroll
-    for (int i = 0; i < 4; i++)   // n <= 4: the values lie in one half of the row
+    for (int i = 0; i < C::S; i++)   // the values lie in one half of the row: the first exchange has chosen it
       if (i < n) put(g, i, v[g][i]);
 }
 
@@ -185,11 +226,11 @@ __device__ __forceinline__ void write8(float* p, const float (&x)[8]) {
 }
 
 // A tile's rows of one [B,T,M] tensor: 8 channels per access.
-template <class T, int L>
+template <class C>
 struct Rows {
-  static constexpr int CH = NT / L, PER_TOKEN = CH / 8, COUNT = TT * PER_TOKEN, EACH = (COUNT + NT - 1) / NT;
+  static constexpr int PER_TOKEN = C::CH / 8, COUNT = C::TT * PER_TOKEN, EACH = (COUNT + C::NH - 1) / C::NH;
   __device__ static __forceinline__ bool mine(int k, int& tok, int& c) {
-    const int i = threadIdx.x % NT + k * NT;
+    const int i = (int)threadIdx.x - C::NS + k * C::NH;
     tok = i / PER_TOKEN;
     c = i % PER_TOKEN * 8;
     return i < COUNT;
@@ -200,23 +241,23 @@ __device__ __forceinline__ void fetch8(Pack<T, 8>& d, const T* base, long long t
   load_some<T, 8>(d, base + t * token_stride + c, t < t1 ? valid - c : 0, wide);
 }
 // B and C of a tile as FP32 [TT][NP]; WHICH: 1 B, 2 C, 3 both
-template <class T, int L, int WHICH>
+template <class T, class C, int WHICH>
 struct Shared {
-  static constexpr int NP = S * L, PER_TOKEN = NP / 8, TENSORS = WHICH == 3 ? 2 : 1, COUNT = TT * PER_TOKEN * TENSORS, EACH = (COUNT + NT - 1) / NT;
+  static constexpr int PER_TOKEN = C::NP / 8, TENSORS = WHICH == 3 ? 2 : 1, COUNT = C::TT * PER_TOKEN * TENSORS, EACH = (COUNT + C::NH - 1) / C::NH;
   Pack<T, 8> v[EACH];
-  __device__ __forceinline__ void fetch(const ScanParams& p, const T* B, const T* C, int t0, int t1) {
+  __device__ __forceinline__ void fetch(const ScanParams& p, const T* Bm, const T* Cm, int t0, int t1) {
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
-      const int i = threadIdx.x % NT + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      const int i = (int)threadIdx.x - C::NS + k * C::NH, which = WHICH == 3 ? i / (C::TT * PER_TOKEN) : WHICH - 1, j = i % (C::TT * PER_TOKEN);
       const int t = t0 + j / PER_TOKEN, n = j % PER_TOKEN * 8;
       if (i < COUNT)
-        load_some<T, 8>(v[k], (which ? C + t * p.a.C_stride[1] : B + t * p.a.B_stride[1]) + n, t < t1 ? p.a.N - n : 0, p.wide_bc);
+        load_some<T, 8>(v[k], (which ? Cm + t * p.a.C_stride[1] : Bm + t * p.a.B_stride[1]) + n, t < t1 ? p.a.N - n : 0, p.wide_bc);
     }
   }
   __device__ __forceinline__ void publish(float* sB, float* sC) const {
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
-      const int i = threadIdx.x % NT + k * NT, which = WHICH == 3 ? i / (TT * PER_TOKEN) : WHICH - 1, j = i % (TT * PER_TOKEN);
+      const int i = (int)threadIdx.x - C::NS + k * C::NH, which = WHICH == 3 ? i / (C::TT * PER_TOKEN) : WHICH - 1, j = i % (C::TT * PER_TOKEN);
       if (i < COUNT) {
         float* to = (which ? sC : sB) + j * 8;
 #pragma unroll
@@ -241,43 +282,44 @@ __device__ __forceinline__ void steps_of(float (&d)[8], float (&slope)[8], bool 
 }
 
 // State at the first token of segment `seg` of a sequence that began before it, from the ends of the segments between.
+template <int S>
 __device__ __forceinline__ void join_forward(float (&h)[S], const ScanParams& p, int b, int seg, int begin, long long m, const float (&A2)[S], int n0, bool ok) {
   const int first = begin / p.seg_len;
   for (int j = first; j < seg; j++) {
     const long long row = ((long long)b * p.segments + j) * p.a.M + m;
     float end[S];
-    load4(end, p.seg_state + row * p.a.N, n0, p.a.N, ok, p.wide_state);
+    load_states(end, p.seg_state + row * p.a.N, n0, p.a.N, ok, p.wide_state);
     const float d = ok ? p.seg_dt[row] : 0.f;
 #pragma unroll
     for (int i = 0; i < S; i++) h[i] = j == first ? end[i] : fmaf(ex2(A2[i] * d), h[i], end[i]);
   }
 }
 
-template <int L>
+template <class C>
 struct FwdShared {
-  static constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
-  float dt[2][TT * CH], du[2][TT * CH], B[2][TT * NP], C[2][TT * NP], y[2][TT * YS];  // du: dt u
+  static constexpr int CH = C::CH, NP = C::NP, YS = C::YS, TT = C::TT;
+  float dt[2][TT * CH], du[2][TT * CH], B[2][TT * NP], Cm[2][TT * NP], y[2][TT * YS];  // du: dt u
 };
 
 // STATE_ONLY: the first pass of a scan in segments (all but the last one).
 // Two groups of four warps: the first runs the recurrence of a tile, the second meanwhile writes what came of the tile before
 // and prepares the tile behind.
-template <class T, int L, bool STATE_ONLY>
-__global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
-  constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
-  using R = Rows<T, L>;
+template <class T, class C, bool STATE_ONLY>
+__global__ void __launch_bounds__(C::THREADS, 2) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = C::CH, NP = C::NP, YS = C::YS, L = C::L, S = C::S, P = C::P, TT = C::TT;
+  using R = Rows<C>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
-  FwdShared<L>& sm = *reinterpret_cast<FwdShared<L>*>(raw_smem);
+  FwdShared<C>& sm = *reinterpret_cast<FwdShared<C>*>(raw_smem);
   const RewyScanArgs& a = p.a;
-  const Place<L> at(p, 0, STATE_ONLY ? p.segments - 1 : p.segments);
+  const Place<C> at(p, 0, STATE_ONLY ? p.segments - 1 : p.segments);
   const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
   const bool gated = !STATE_ONLY && a.z != nullptr;
-  if (threadIdx.x >= NT) {
+  if (threadIdx.x >= C::NS) {
     const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
     const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
     const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
     const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-    const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+    const T* Cm = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
     float bias[R::EACH][8], Dv[R::EACH][8];
 #pragma unroll
     for (int k = 0; k < R::EACH; k++) {
@@ -290,7 +332,7 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
       }
     }
     Pack<T, 8> ru[R::EACH], rd[R::EACH], xu[R::EACH], xz[R::EACH];
-    Shared<T, L, STATE_ONLY ? 1 : 3> bc;
+    Shared<T, C, STATE_ONLY ? 1 : 3> bc;
     auto fetch = [&](int t) {
 #pragma unroll
       for (int k = 0; k < R::EACH; k++) {
@@ -299,27 +341,29 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
         fetch8(ru[k], u, a.u_stride[1], t + tok, at.t1, c, at.valid, p.wide);
         fetch8(rd[k], dt, a.dt_stride[1], t + tok, at.t1, c, at.valid, p.wide);
       }
-      bc.fetch(p, Bm, C, t, at.t1);
+      bc.fetch(p, Bm, Cm, t, at.t1);
     };
     auto publish = [&](int t, int buf) {
 #pragma unroll
       for (int k = 0; k < R::EACH; k++) {
         int tok, c;
         if (!R::mine(k, tok, c)) continue;
-        float d[8], w[8];
+        float d[8], w[8], x[8];
+        to_floats(d, rd[k]);
+        to_floats(x, ru[k]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) d[e] = to_f32(rd[k].v[e]) + bias[k][e];
+        for (int e = 0; e < 8; e++) d[e] += bias[k][e];
         steps_of<false>(d, w, a.softplus);
         const int real = t + tok < at.t1 ? at.valid - c : 0;   // a token that does not exist: no decay, no input
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           d[e] = e < real ? d[e] : 0.f;
-          w[e] = d[e] * to_f32(ru[k].v[e]);
+          w[e] = d[e] * x[e];
         }
         write8(&sm.dt[buf][tok * CH + c], d);
         write8(&sm.du[buf][tok * CH + c], w);
       }
-      bc.publish(sm.B[buf], sm.C[buf]);
+      bc.publish(sm.B[buf], sm.Cm[buf]);
     };
     auto fetch_again = [&](int t0) {   // u and z of the tile whose recurrence has been run
 #pragma unroll
@@ -336,19 +380,18 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
       for (int k = 0; k < R::EACH; k++) {
         int tok, c;
         if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
-        float y[8];
+        float y[8], x[8];
         read8(y, &sm.y[buf][tok * YS + c]);
+        to_floats(x, xu[k]);
         Pack<T, 8> out;
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = fmaf(Dv[k][e], to_f32(xu[k].v[e]), y[e]);
-        if (gated)
+        for (int e = 0; e < 8; e++) y[e] = fmaf(Dv[k][e], x[e], y[e]);
+        if (gated) {
+          to_floats(x, xz[k]);
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float g = to_f32(xz[k].v[e]);
-            y[e] *= g * sigmoid_fast(g);
-          }
-#pragma unroll
-        for (int e = 0; e < 8; e++) out.v[e] = from_f32<T>(y[e]);
+          for (int e = 0; e < 8; e++) y[e] *= x[e] * sigmoid_fast(x[e]);
+        }
+        from_floats(out, y);
         store_some<T, 8>(static_cast<T*>(a.y) + ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c, out, at.valid - c, p.wide);
       }
     };
@@ -376,16 +419,18 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
   const bool ok = ch < at.valid;
   const long long m = at.m0 + ch;
   float A2[S], h[S] = {};
-  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+  load_states(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
-  const F2 A01 = pair(A2[0], A2[1]), A23 = pair(A2[2], A2[3]);
+  F2 A2p[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) A2p[i] = pair(A2[2 * i], A2[2 * i + 1]);
 
   Sequence q;
   q.at(a, at.b, at.t0);
-  auto start = [&](int s) { load4(h, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state); };
+  auto start = [&](int s) { load_states(h, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state); };
   auto finish = [&](int s) {
-    if (!STATE_ONLY && a.final_state != nullptr) store4(a.final_state + ((long long)s * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
+    if (!STATE_ONLY && a.final_state != nullptr) store_states(a.final_state + ((long long)s * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
   };
   if (q.begin == at.t0) start(q.s);
   else if (!STATE_ONLY) join_forward(h, p, at.b, at.seg, q.begin, m, A2, n0, ok);
@@ -395,7 +440,7 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
   for (int i = 0; i < tiles; i++) {
     const int t0 = at.t0 + i * TT, buf = i & 1;
     const float *__restrict__ const sdt = sm.dt[buf] + ch, *__restrict__ const sdu = sm.du[buf] + ch;
-    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.C[buf] + n0;
+    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.Cm[buf] + n0;
     float* __restrict__ const sy = sm.y[buf] + ch;
     // Eight tokens; check: a sequence may begin inside the tile
     auto tokens = [&](auto check, int k) {
@@ -404,20 +449,21 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
       for (int half = 0; half < 2; half++) {
         const int kh = k + 4 * half;
         if (!STATE_ONLY && kh % CK == 0 && a.checkpoints != nullptr && t0 + kh < a.T)
-          store4(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + kh) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
-        F2 e01[4], e23[4], g01[4], g23[4];
-        ulonglong2 Cv[4];
+          store_states(a.checkpoints + (((long long)at.b * ((a.T + CK - 1) / CK) + (t0 + kh) / CK) * a.M + m) * a.N, h, n0, a.N, ok, p.wide_state);
+        F2 dec[4][P], in[4][P], Cv[4][P];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const float dj = sdt[(kh + j) * CH];
           const F2 d = both(dj), w = both(sdu[(kh + j) * CH]);
-          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (kh + j) * NP);
-          if (!STATE_ONLY) Cv[j] = *reinterpret_cast<const ulonglong2*>(sC + (kh + j) * NP);
+          F2 Bv[P];
+          shared_pairs(Bv, sB + (kh + j) * NP);
+          if (!STATE_ONLY) shared_pairs(Cv[j], sC + (kh + j) * NP);
           else total += dj;
-          e01[j] = ex2_2(mul2(d, A01));
-          e23[j] = ex2_2(mul2(d, A23));
-          g01[j] = mul2(w, F2{Bv.x});
-          g23[j] = mul2(w, F2{Bv.y});
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            dec[j][i] = ex2_2(mul2(d, A2p[i]));
+            in[j][i] = mul2(w, Bv[i]);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -426,10 +472,15 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
             q.advance(a);
             start(q.s);
           }
-          const F2 h01 = fma2(e01[j], pair(h[0], h[1]), g01[j]), h23 = fma2(e23[j], pair(h[2], h[3]), g23[j]);
-          const float2 u01 = halves(h01), u23 = halves(h23);
-          h[0] = u01.x; h[1] = u01.y; h[2] = u23.x; h[3] = u23.y;
-          if constexpr (!STATE_ONLY) y[half][j] = sum_halves(fma2(F2{Cv[j].x}, h01, mul2(F2{Cv[j].y}, h23)));
+          F2 sum;
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const F2 x = fma2(dec[j][i], pair(h[2 * i], h[2 * i + 1]), in[j][i]);
+            const float2 hx = halves(x);
+            h[2 * i] = hx.x; h[2 * i + 1] = hx.y;
+            if (!STATE_ONLY) sum = i ? fma2(Cv[j][i], x, sum) : mul2(Cv[j][i], x);
+          }
+          if constexpr (!STATE_ONLY) y[half][j] = sum_halves(sum);
         }
       }
       if constexpr (!STATE_ONLY) {
@@ -449,7 +500,7 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
   }
   if constexpr (STATE_ONLY) {
     const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
-    store4(p.seg_state + row * a.N, h, n0, a.N, ok, p.wide_state);
+    store_states(p.seg_state + row * a.N, h, n0, a.N, ok, p.wide_state);
     if (ok && sl == 0) p.seg_dt[row] = total;
   } else {
     if (at.t1 == a.T || at.t1 == q.next) finish(q.s);
@@ -459,21 +510,21 @@ __global__ void __launch_bounds__(2 * NT) scan_fwd_kernel(const __grid_constant_
 // ---- backward --------------------------------------------------------------------------------------------------------
 
 // Gradient of the state that token t1 - 1 hands on: from the segments behind, or from the final state's gradient.
-template <int L>
-__device__ __forceinline__ void join_backward(float (&carry)[S], const ScanParams& p, const Place<L>& at, long long m, const float (&A2)[S], int n0, bool ok) {
+template <class C, int S>
+__device__ __forceinline__ void join_backward(float (&carry)[S], const ScanParams& p, const Place<C>& at, long long m, const float (&A2)[S], int n0, bool ok) {
   const RewyScanArgs& a = p.a;
   Sequence q;
   q.at(a, at.b, at.t1 - 1);
   const int end = min(q.next, a.T);
   if (end <= at.t1) {   // the sequence ends with this segment
-    load4(carry, a.dfinal_state + ((long long)q.s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state);
+    load_states(carry, a.dfinal_state + ((long long)q.s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state);
     return;
   }
   const int last = (end - 1) / p.seg_len;
   for (int j = last; j > at.seg; j--) {
     const long long row = ((long long)at.b * p.segments + j) * a.M + m;
     float out[S];
-    load4(out, p.seg_state + row * a.N, n0, a.N, ok, p.wide_state);
+    load_states(out, p.seg_state + row * a.N, n0, a.N, ok, p.wide_state);
     const float d = ok ? p.seg_dt[row] : 0.f;
 #pragma unroll
     for (int i = 0; i < S; i++) carry[i] = j == last ? out[i] : fmaf(ex2(A2[i] * d), carry[i], out[i]);
@@ -481,159 +532,192 @@ __device__ __forceinline__ void join_backward(float (&carry)[S], const ScanParam
 }
 
 // First pass over the segments but the first: the gradient that leaves each one's first token for the state before it.
-template <class T, int L>
-__global__ void __launch_bounds__(NT) scan_bwd_state_kernel(const __grid_constant__ ScanParams p) {
-  constexpr int CH = NT / L, NP = S * L;
-  using R = Rows<T, L>;
-  __shared__ __align__(16) float sdt[TT * CH], sdy[TT * CH], sC[TT * NP], sbias[CH];
+template <class T, class C>
+__global__ void __launch_bounds__(C::THREADS) scan_bwd_state_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = C::CH, NP = C::NP, L = C::L, S = C::S, TT = C::TT;
+  using R = Rows<C>;
+  __shared__ __align__(16) float sdt[2][TT * CH], sdy[2][TT * CH], sC[2][TT * NP];
   const RewyScanArgs& a = p.a;
-  const Place<L> at(p, 1, p.segments - 1);
+  const Place<C> at(p, 1, p.segments - 1);
+  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  if (threadIdx.x >= C::NS) {
+    const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
+    const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
+    const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
+    const T* Cm = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+    Pack<T, 8> xd[R::EACH], xy[R::EACH], xz[R::EACH];
+    Shared<T, C, 2> cc;
+    float bias[R::EACH][8];
+#pragma unroll
+    for (int k = 0; k < R::EACH; k++) {
+      int tok, c;
+      R::mine(k, tok, c);
+#pragma unroll
+      for (int e = 0; e < 8; e++) bias[k][e] = a.dt_bias != nullptr && c + e < at.valid ? a.dt_bias[at.m0 + c + e] : 0.f;
+    }
+    auto fetch = [&](int t0) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        fetch8(xd[k], dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+        fetch8(xy[k], dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+        if (a.z != nullptr) fetch8(xz[k], z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+      }
+      cc.fetch(p, nullptr, Cm, t0, at.t1);
+    };
+    auto publish = [&](int t0, int buf) {
+#pragma unroll
+      for (int k = 0; k < R::EACH; k++) {
+        int tok, c;
+        if (!R::mine(k, tok, c)) continue;
+        float d[8], g[8], v[8];
+        to_floats(d, xd[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] += bias[k][e];
+        steps_of<false>(d, g, a.softplus);
+        to_floats(g, xy[k]);
+        if (a.z != nullptr) {
+          to_floats(v, xz[k]);
+#pragma unroll
+          for (int e = 0; e < 8; e++) g[e] *= v[e] * sigmoid_fast(v[e]);
+        }
+        const int real = t0 + tok < at.t1 ? at.valid - c : 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          d[e] = e < real ? d[e] : 0.f;
+          g[e] = e < real ? g[e] : 0.f;
+        }
+        write8(&sdt[buf][tok * CH + c], d);
+        write8(&sdy[buf][tok * CH + c], g);
+      }
+      cc.publish(nullptr, sC[buf]);
+    };
+    fetch(at.t0 + (tiles - 1) * TT);
+    publish(at.t0 + (tiles - 1) * TT, (tiles - 1) & 1);
+    if (tiles > 1) fetch(at.t0 + (tiles - 2) * TT);
+    __syncthreads();
+    for (int tile = tiles - 1; tile >= 0; tile--) {
+      if (tile > 0) publish(at.t0 + (tile - 1) * TT, (tile - 1) & 1);
+      if (tile > 1) fetch(at.t0 + (tile - 2) * TT);
+      __syncthreads();
+    }
+    return;
+  }
   const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
   const bool ok = ch < at.valid;
   const long long m = at.m0 + ch;
-  const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
-  const T* z = static_cast<const T*>(a.z) + (a.z != nullptr ? at.b * a.z_stride[0] + at.m0 : 0);
-  const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
-  const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  for (int c = threadIdx.x; c < CH; c += NT) sbias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
   float A2[S], carry[S] = {}, total = 0.f;
-  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+  load_states(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
   Sequence q;
   q.at(a, at.b, at.t1 - 1);
-  auto last_of = [&](int s) { load4(carry, a.dfinal_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state); };
+  auto last_of = [&](int s) { load_states(carry, a.dfinal_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state); };
   if (min(q.next, a.T) <= at.t1) last_of(q.s);
-  const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
+  __syncthreads();
   for (int tile = tiles - 1; tile >= 0; tile--) {
-    const int t0 = at.t0 + tile * TT;
-    __syncthreads();   // sbias; the tile before has been read
+    const int t0 = at.t0 + tile * TT, buf = tile & 1;
+    auto token = [&](int k) {
+      const float d = sdt[buf][k * CH + ch], g = sdy[buf][k * CH + ch];
+      const float* const c = &sC[buf][k * NP + n0];
 #pragma unroll
-    for (int k = 0; k < R::EACH; k++) {
-      int tok, c;
-      if (!R::mine(k, tok, c)) continue;
-      Pack<T, 8> xd, xy, xz;
-      fetch8(xd, dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      fetch8(xy, dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
-      if (a.z != nullptr) fetch8(xz, z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-      float d[8], g[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) d[e] = to_f32(xd.v[e]) + sbias[c + e];
-      steps_of<false>(d, g, a.softplus);
-#pragma unroll
-      for (int e = 0; e < 8; e++) g[e] = to_f32(xy.v[e]);
-      if (a.z != nullptr)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float v = to_f32(xz.v[e]);
-          g[e] *= v * sigmoid_fast(v);
-        }
-      const int real = t0 + tok < at.t1 ? at.valid - c : 0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        d[e] = e < real ? d[e] : 0.f;
-        g[e] = e < real ? g[e] : 0.f;
-      }
-      write8(sdt + tok * CH + c, d);
-      write8(sdy + tok * CH + c, g);
-    }
-    Shared<T, L, 2> cc;
-    cc.fetch(p, nullptr, C, t0, at.t1);
-    cc.publish(nullptr, sC);
-    __syncthreads();
-#pragma unroll 4
-    for (int k = TT - 1; k >= 0; k--) {
-      const float d = sdt[k * CH + ch], g = sdy[k * CH + ch];
-      const float4 Cv = *reinterpret_cast<const float4*>(sC + k * NP + n0);
-      carry[0] = ex2(d * A2[0]) * fmaf(Cv.x, g, carry[0]);
-      carry[1] = ex2(d * A2[1]) * fmaf(Cv.y, g, carry[1]);
-      carry[2] = ex2(d * A2[2]) * fmaf(Cv.z, g, carry[2]);
-      carry[3] = ex2(d * A2[3]) * fmaf(Cv.w, g, carry[3]);
+      for (int i = 0; i < S; i++) carry[i] = ex2(d * A2[i]) * fmaf(c[i], g, carry[i]);
       total += d;
-      if (a.cu_seqlens != nullptr && t0 + k == q.begin && q.s > 0 && t0 + k > at.t0) {   // what flows on belongs to the sequence before
-        q.at(a, at.b, t0 + k - 1);
-        last_of(q.s);
+    };
+    if (a.cu_seqlens == nullptr || q.begin < t0 || q.s == 0) {     // (the first sequence begins with the first segment)
+#pragma unroll 4
+      for (int k = TT - 1; k >= 0; k--) token(k);
+    } else {
+#pragma unroll 1
+      for (int k = TT - 1; k >= 0; k--) {
+        token(k);
+        if (t0 + k == q.begin && q.s > 0 && t0 + k > at.t0) {   // what flows on belongs to the sequence before
+          q.at(a, at.b, t0 + k - 1);
+          last_of(q.s);
+        }
       }
     }
+    __syncthreads();
   }
   const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
-  store4(p.seg_state + row * a.N, carry, n0, a.N, ok, p.wide_state);
+  store_states(p.seg_state + row * a.N, carry, n0, a.N, ok, p.wide_state);
   if (ok && sl == 0) p.seg_dt[row] = total;
 }
 
-template <int L>
+template <class C>
 struct BwdShared {
-  static constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
-  float4 x[2][TT * CH];                                       // dt, dt u, dy' at place(token, channel)
-  float B[2][TT * NP], C[2][TT * NP];
+  static constexpr int CH = C::CH, NP = C::NP, YS = C::YS, TT = C::TT;
+  float4 x[2][TT * CH];                                       // dt, dt u, dy' and the slope of dt, at place(token, channel)
+  float B[2][TT * NP], Cm[2][TT * NP];
   float drive[2][TT * YS], decay[2][TT * YS], y[2][TT * YS];  // per token and channel: sum gh B, sum q A2, sum C h
-  float bc[2][NT / 32][TT][2 * NP];                           // each warp's sums over its channels
+  float bc[2][C::WARPS][TT][2 * NP];                           // each warp's sums over its channels
   float bias[CH], D[CH];
   // A thread writes the entries of eight neighbouring channels: turned by what keeps the threads of a quarter warp apart
   __device__ static __forceinline__ int place(int tok, int c) { return tok * CH + (c & ~7) + ((c ^ ((c >> 3) + CH / 8 * tok)) & 7); }
 };
 
 // Two groups of four warps, as in the forward: the recurrence of a tile beside what stands around the tiles next to it.
-template <class T, int L>
-__global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
-  constexpr int CH = NT / L, NP = S * L, YS = CH + 8;
-  using R = Rows<T, L>;
+template <class T, class C>
+__global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int CH = C::CH, NP = C::NP, YS = C::YS, L = C::L, S = C::S, P = C::P, TT = C::TT;
+  using R = Rows<C>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
-  BwdShared<L>& sm = *reinterpret_cast<BwdShared<L>*>(raw_smem);
+  BwdShared<C>& sm = *reinterpret_cast<BwdShared<C>*>(raw_smem);
   const RewyScanArgs& a = p.a;
-  const Place<L> at(p, 0, p.segments);
+  const Place<C> at(p, 0, p.segments);
   const bool gated = a.z != nullptr;
   const int tiles = (at.t1 - at.t0 + TT - 1) / TT;
   float* const part = p.part_m + ((long long)at.b * p.segments + at.seg) * ((long long)a.M * (a.N + 2));
-  if (threadIdx.x >= NT) {
+  if (threadIdx.x >= C::NS) {
     const T* u = static_cast<const T*>(a.u) + at.b * a.u_stride[0] + at.m0;
     const T* dt = static_cast<const T*>(a.dt) + at.b * a.dt_stride[0] + at.m0;
     const T* z = static_cast<const T*>(a.z) + (gated ? at.b * a.z_stride[0] + at.m0 : 0);
     const T* dy = static_cast<const T*>(a.dy) + (long long)at.b * a.T * a.M + at.m0;
     const T* Bm = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-    const T* C = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-    const int me = threadIdx.x - NT;
+    const T* Cm = static_cast<const T*>(a.C) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
+    const int me = threadIdx.x - C::NS;
     struct Inputs {
       Pack<T, 8> u[R::EACH], dt[R::EACH], dy[R::EACH], z[R::EACH];
     };
-    auto fetch = [&](Inputs& x, int t0) {
+    auto fetch = [&](Inputs& x, int t0, bool all) {
 #pragma unroll
       for (int k = 0; k < R::EACH; k++) {
         int tok, c;
         if (!R::mine(k, tok, c)) continue;
         fetch8(x.u[k], u, a.u_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-        fetch8(x.dt[k], dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
-        fetch8(x.dy[k], dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
+        if (all) fetch8(x.dt[k], dt, a.dt_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
+        if (all || gated) fetch8(x.dy[k], dy, (long long)a.M, t0 + tok, at.t1, c, at.valid, p.wide);
         if (gated) fetch8(x.z[k], z, a.z_stride[1], t0 + tok, at.t1, c, at.valid, p.wide);
       }
     };
     Inputs ahead, behind;      // of the tile that is prepared next, of the one that is finished next
-    Shared<T, L, 3> bc;
+    Shared<T, C, 3> bc;
     auto prepare = [&](int t0, int buf) {
 #pragma unroll
       for (int k = 0; k < R::EACH; k++) {
         int tok, c;
         if (!R::mine(k, tok, c)) continue;
-        float d[8], g[8];
+        float d[8], g[8], slope[8], x[8];
         read8(d, sm.bias + c);
+        to_floats(x, ahead.dt[k]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) d[e] += to_f32(ahead.dt[k].v[e]);
-        steps_of<false>(d, g, a.softplus);
+        for (int e = 0; e < 8; e++) d[e] += x[e];
+        steps_of<true>(d, slope, a.softplus);
+        to_floats(g, ahead.dy[k]);
+        if (gated) {
+          to_floats(x, ahead.z[k]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) g[e] = to_f32(ahead.dy[k].v[e]);
-        if (gated)
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float v = to_f32(ahead.z[k].v[e]);
-            g[e] *= v * sigmoid_fast(v);
-          }
+          for (int e = 0; e < 8; e++) g[e] *= x[e] * sigmoid_fast(x[e]);
+        }
+        to_floats(x, ahead.u[k]);
         const int real = t0 + tok < at.t1 ? at.valid - c : 0;
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          sm.x[buf][BwdShared<L>::place(tok, c + e)] =
-              e < real ? make_float4(d[e], d[e] * to_f32(ahead.u[k].v[e]), g[e], 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+          sm.x[buf][BwdShared<C>::place(tok, c + e)] =
+              e < real ? make_float4(d[e], d[e] * x[e], g[e], slope[e]) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      bc.publish(sm.B[buf], sm.C[buf]);
+      bc.publish(sm.B[buf], sm.Cm[buf]);
     };
     float sD[R::EACH][8] = {}, sbias[R::EACH][8] = {};   // sums over the tokens that this thread sees
     auto finish_tile = [&](int t0, int buf) {
@@ -642,54 +726,57 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
         int tok, c;
         if (!R::mine(k, tok, c) || t0 + tok >= at.t1 || c >= at.valid) continue;
         Pack<T, 8> ou, od, oz;
-        float drive[8], x[8], g[8], d[8], slope[8];
+        float drive[8], decay[8], uv[8], z8[8];
         const float* const Dv = sm.D + c;
-#pragma unroll
-        for (int e = 0; e < 8; e++) g[e] = to_f32(behind.dy[k].v[e]);
+        to_floats(uv, behind.u[k]);
         if (gated) {
-          read8(x, &sm.y[buf][tok * YS + c]);
+          float y[8], dy8[8];
+          read8(y, &sm.y[buf][tok * YS + c]);
+          to_floats(z8, behind.z[k]);
+          to_floats(dy8, behind.dy[k]);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            const float v = to_f32(behind.z[k].v[e]), s = sigmoid_fast(v);
-            oz.v[e] = from_f32<T>(g[e] * fmaf(Dv[e], to_f32(behind.u[k].v[e]), x[e]) * s * fmaf(v, 1.f - s, 1.f));
-            g[e] *= v * s;
+            const float s = sigmoid_fast(z8[e]);
+            z8[e] = dy8[e] * fmaf(Dv[e], uv[e], y[e]) * s * fmaf(z8[e], 1.f - s, 1.f);
           }
+          from_floats(oz, z8);
         }
-        read8(d, sm.bias + c);
-#pragma unroll
-        for (int e = 0; e < 8; e++) d[e] += to_f32(behind.dt[k].v[e]);
-        steps_of<true>(d, slope, a.softplus);
         read8(drive, &sm.drive[buf][tok * YS + c]);
-        read8(x, &sm.decay[buf][tok * YS + c]);
+        read8(decay, &sm.decay[buf][tok * YS + c]);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float uv = to_f32(behind.u[k].v[e]), dd = fmaf(uv, drive[e], LN2 * x[e]) * slope[e];
-          ou.v[e] = from_f32<T>(fmaf(Dv[e], g[e], drive[e] * d[e]));
-          od.v[e] = from_f32<T>(dd);
-          sD[k][e] = fmaf(g[e], uv, sD[k][e]);     // (channels that do not exist are not read)
+          const float4 x = sm.x[buf][BwdShared<C>::place(tok, c + e)];   // as this thread left it
+          const float dd = fmaf(uv[e], drive[e], LN2 * decay[e]) * x.w;
+          drive[e] = fmaf(Dv[e], x.z, drive[e] * x.x);
+          decay[e] = dd;
+          sD[k][e] = fmaf(x.z, uv[e], sD[k][e]);     // (channels that do not exist are not read)
           sbias[k][e] += dd;
         }
+        from_floats(ou, drive);
+        from_floats(od, decay);
         const long long to = ((long long)at.b * a.T + t0 + tok) * a.M + at.m0 + c;
         store_some<T, 8>(static_cast<T*>(a.du) + to, ou, at.valid - c, p.wide);
         store_some<T, 8>(static_cast<T*>(a.ddt) + to, od, at.valid - c, p.wide);
         if (gated) store_some<T, 8>(static_cast<T*>(a.dz) + to, oz, at.valid - c, p.wide);
       }
-      // the warps' sums over their channels: a thread adds one place of the row for every NT / (2 NP)-th token
-      constexpr int EVERY = NT / (2 * NP) > 0 ? NT / (2 * NP) : 1;
-      const int v = me % (2 * NP), n = v % NP;
-      if (n < a.N) {
+      // the warps' sums over their channels, a place of the row after the other
+      constexpr int SPAN = C::NH < 2 * NP ? C::NH : 2 * NP, EVERY = C::NH / SPAN;   // a group of SPAN threads takes every EVERY-th token
+#pragma unroll
+      for (int v = me % SPAN; v < 2 * NP; v += SPAN) {
+        const int n = v % NP;
+        if (n >= a.N) continue;
         float* to = p.part_bc + ((((long long)at.cb * a.B + at.b) * a.T + t0) * a.G + at.g) * 2 * a.N + v / NP * a.N + n;
         const int row = a.G * 2 * a.N;
 #pragma unroll 4
-        for (int tok = me / (2 * NP); tok < TT; tok += EVERY) {
+        for (int tok = me / SPAN; tok < TT; tok += EVERY) {
           float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < NT / 32; w++) sum += sm.bc[buf][w][tok][v];
+          for (int w = 0; w < C::WARPS; w++) sum += sm.bc[buf][w][tok][v];
           if (t0 + tok < at.t1) to[(long long)tok * row] = sum;
         }
       }
     };
-    for (int c = me; c < CH; c += NT) {
+    for (int c = me; c < CH; c += C::NH) {
       sm.bias[c] = a.dt_bias != nullptr && c < at.valid ? a.dt_bias[at.m0 + c] : 0.f;
       sm.D[c] = a.D != nullptr && c < at.valid ? a.D[at.m0 + c] : 0.f;
     }
@@ -697,32 +784,32 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
     // What a step reads has been asked for a step before.
     {
       const int t0 = at.t0 + (tiles - 1) * TT;
-      fetch(ahead, t0);
-      bc.fetch(p, Bm, C, t0, at.t1);
+      fetch(ahead, t0, true);
+      bc.fetch(p, Bm, Cm, t0, at.t1);
       prepare(t0, (tiles - 1) & 1);
       behind = ahead;
       if (tiles > 1) {
-        fetch(ahead, t0 - TT);
-        bc.fetch(p, Bm, C, t0 - TT, at.t1);
+        fetch(ahead, t0 - TT, true);
+        bc.fetch(p, Bm, Cm, t0 - TT, at.t1);
       }
     }
     __syncthreads();
     for (int tile = tiles - 1; tile >= 0; tile--) {
       const int t0 = at.t0 + tile * TT;
+      if (tile + 1 < tiles) {      // before the operands of the next tile take the place of its own: a thread reads what it wrote
+        finish_tile(t0 + TT, (tile + 1) & 1);
+        fetch(behind, t0, false);
+      }
       if (tile > 0) prepare(t0 - TT, (tile - 1) & 1);
       if (tile > 1) {
-        fetch(ahead, t0 - 2 * TT);
-        bc.fetch(p, Bm, C, t0 - 2 * TT, at.t1);
-      }
-      if (tile + 1 < tiles) {
-        finish_tile(t0 + TT, (tile + 1) & 1);
-        fetch(behind, t0);
+        fetch(ahead, t0 - 2 * TT, true);
+        bc.fetch(p, Bm, Cm, t0 - 2 * TT, at.t1);
       }
       __syncthreads();
     }
     finish_tile(at.t0, 0);
-    // over the tokens of a tile, in the room of the operands, which nothing reads any more
-    float *const all_D = reinterpret_cast<float*>(sm.x[0]), *const all_bias = all_D + TT * CH;
+    // over the tokens of a tile, in the room of the operands of the tile behind, which nothing reads any more
+    float *const all_D = reinterpret_cast<float*>(sm.x[1]), *const all_bias = all_D + TT * CH;
 #pragma unroll
     for (int k = 0; k < R::EACH; k++) {
       int tok, c;
@@ -730,8 +817,8 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
       write8(all_D + tok * CH + c, sD[k]);
       write8(all_bias + tok * CH + c, sbias[k]);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");   // this group only
-    for (int c = me; c < at.valid; c += NT) {
+    asm volatile("bar.sync 1, %0;" ::"n"(C::NH) : "memory");   // this group only
+    for (int c = me; c < at.valid; c += C::NH) {
       float x = 0.f, y = 0.f;
 #pragma unroll 4
       for (int k = 0; k < TT; k++) { x += all_D[k * CH + c]; y += all_bias[k * CH + c]; }
@@ -745,48 +832,45 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
   const bool ok = ch < at.valid;
   const long long m = at.m0 + ch;
   float A2[S], carry4[S] = {};
-  load4(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
+  load_states(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
-  join_backward<L>(carry4, p, at, m, A2, n0, ok);
-  const F2 A2p[2] = {pair(A2[0], A2[1]), pair(A2[2], A2[3])};
-  F2 carry[2] = {pair(carry4[0], carry4[1]), pair(carry4[2], carry4[3])}, dA[2] = {both(0.f), both(0.f)}, dA_lost[2] = {both(0.f), both(0.f)};
-  const int place = sum_place<L>(lane, n0);
-  auto initial = [&](F2(&x)[2], int s) {
-    float v[S];
-    load4(v, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
-    x[0] = pair(v[0], v[1]);
-    x[1] = pair(v[2], v[3]);
+  join_backward(carry4, p, at, m, A2, n0, ok);
+  F2 A2p[P], carry[P], dA[P], dA_lost[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    A2p[i] = pair(A2[2 * i], A2[2 * i + 1]);
+    carry[i] = pair(carry4[2 * i], carry4[2 * i + 1]);
+    dA[i] = dA_lost[i] = both(0.f);
+  }
+  const int place = sum_place<C>(lane, n0);
+  auto initial = [&](F2(&x)[P], int s) {
+    load_pairs(x, a.initial_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.initial_state != nullptr, p.wide_state);
   };
   // The gradient that leaves a sequence's first token is its initial state's; the token before belongs to another one.
   auto leave = [&](int s) {
-    const float2 c01 = halves(carry[0]), c23 = halves(carry[1]);
-    const float out[S] = {c01.x, c01.y, c23.x, c23.y};
-    if (a.dinitial_state != nullptr) store4(a.dinitial_state + ((long long)s * a.M + m) * a.N, out, n0, a.N, ok, p.wide_state);
+    if (a.dinitial_state != nullptr) store_pairs(a.dinitial_state + ((long long)s * a.M + m) * a.N, carry, n0, a.N, ok, p.wide_state);
     const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s > 0;
-    float v[S];
-    load4(v, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
-    carry[0] = pair(v[0], v[1]);
-    carry[1] = pair(v[2], v[3]);
+    load_pairs(carry, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
   };
   const float* const kept = a.checkpoints + ((long long)at.b * ((a.T + CK - 1) / CK) * a.M + m) * a.N;
-  float next[S];   // the state before the 16 tokens that come next
-  load4(next, kept + (long long)((at.t1 - 1) / CK) * a.M * a.N, n0, a.N, ok, p.wide_state);
+  F2 next[P];   // the state before the 16 tokens that come next
+  load_pairs(next, kept + (long long)((at.t1 - 1) / CK) * a.M * a.N, n0, a.N, ok, p.wide_state);
   __syncthreads();
   __syncthreads();
   for (int tile = tiles - 1; tile >= 0; tile--) {
     const int t0 = at.t0 + tile * TT, buf = tile & 1;
     const float4* __restrict__ const sx = sm.x[buf];
-    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.C[buf] + n0;
+    const float *__restrict__ const sB = sm.B[buf] + n0, *__restrict__ const sC = sm.Cm[buf] + n0;
     float *__restrict__ const to_drive = sm.drive[buf] + ch, *__restrict__ const to_decay = sm.decay[buf] + ch, *__restrict__ const to_y = sm.y[buf] + ch;
     float* __restrict__ const to_bc = &sm.bc[buf][warp][0][place];
 #pragma unroll 1
     for (int sub = TT / CK - 1; sub >= 0; sub--) {
       const int k0 = sub * CK, ts = t0 + k0;
       if (ts >= at.t1) continue;
-      // bit j: a sequence starts at token ts + j; `s_last`: the sequence of the last one that does
+      // bit j: a sequence starts at token ts + j; s_low: the sequence of token ts
       unsigned starts = ts == 0 ? 1u : 0u;
-      int s_last = at.b, s_low = at.b;
+      int s_low = at.b;
       if (a.cu_seqlens != nullptr) {
         Sequence q;
         q.at(a, at.b, ts);
@@ -796,58 +880,62 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
           q.advance(a);
           starts |= 1u << (q.begin - ts);
         }
-        s_last = q.s;
       }
-      F2 before[2] = {pair(next[0], next[1]), pair(next[2], next[3])}, local[2] = {both(0.f), both(0.f)};
-      if (ts > at.t0) load4(next, kept + (long long)(ts / CK - 1) * a.M * a.N, n0, a.N, ok, p.wide_state);
+      F2 before[P], local[P];
+#pragma unroll
+      for (int i = 0; i < P; i++) {
+        before[i] = next[i];
+        local[i] = both(0.f);
+      }
+      if (ts > at.t0) load_pairs(next, kept + (long long)(ts / CK - 1) * a.M * a.N, n0, a.N, ok, p.wide_state);
       if (starts & 1u) initial(before, s_low);
       // inside: sequences begin behind the first of the 16 tokens
       auto walk = [&](auto inside) {
-        F2 h[CK][2], x[2] = {before[0], before[1]};
+        F2 h[CK][P], x[P];
+#pragma unroll
+        for (int i = 0; i < P; i++) x[i] = before[i];
         int s = s_low;
 #pragma unroll
         for (int j = 0; j < CK; j++) {
           if (inside.value && j > 0 && (starts >> j & 1u)) initial(x, ++s);
-          const float2 v = *reinterpret_cast<const float2*>(sx + k0 * CH + BwdShared<L>::place(j, ch));
+          const float2 v = *reinterpret_cast<const float2*>(sx + k0 * CH + BwdShared<C>::place(j, ch));
           const F2 d = both(v.x), w = both(v.y);
-          const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k0 + j) * NP);
-          const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}};
+          F2 Bv[P];
+          shared_pairs(Bv, sB + (k0 + j) * NP);
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            x[i] = fma2(ex2_2(mul2(d, A2p[i])), x[i], mul2(w, b2[i]));
-            h[j][i] = x[i];
-          }
+          for (int i = 0; i < P; i++) h[j][i] = x[i] = fma2(ex2_2(mul2(d, A2p[i])), x[i], mul2(w, Bv[i]));
         }
-        s = s_last;
 #pragma unroll
         for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
-          float sums[3][4], v[2][8];   // drive, decay, y of four tokens; dB and dC of this channel of two
+          float sums[3][4], v[2][2 * S];   // drive, decay, y of four tokens; dB and dC of this channel of two
 #pragma unroll
           for (int jj = 3; jj >= 0; jj--) {
             const int j = j4 + jj;
-            const float4 xv = sx[k0 * CH + BwdShared<L>::place(j, ch)];
+            const float4 xv = sx[k0 * CH + BwdShared<C>::place(j, ch)];
             const F2 d = both(xv.x), w = both(xv.y), g = both(xv.z);
-            const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(sB + (k0 + j) * NP), Cv = *reinterpret_cast<const ulonglong2*>(sC + (k0 + j) * NP);
-            const F2 b2[2] = {F2{Bv.x}, F2{Bv.y}}, c2[2] = {F2{Cv.x}, F2{Cv.y}};
-            F2 old[2] = {j == 0 ? before[0] : h[j > 0 ? j - 1 : 0][0], j == 0 ? before[1] : h[j > 0 ? j - 1 : 0][1]};
+            F2 Bv[P], Cv[P], old[P];
+            shared_pairs(Bv, sB + (k0 + j) * NP);
+            shared_pairs(Cv, sC + (k0 + j) * NP);
+#pragma unroll
+            for (int i = 0; i < P; i++) old[i] = j == 0 ? before[i] : h[j > 0 ? j - 1 : 0][i];
             const bool first = inside.value && j > 0 && (starts >> j & 1u);
             if (first) initial(old, s);
             F2 dr, de, yy;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const F2 gh = fma2(c2[i], g, carry[i]);
+            for (int i = 0; i < P; i++) {
+              const F2 gh = fma2(Cv[i], g, carry[i]);
               carry[i] = mul2(ex2_2(mul2(d, A2p[i])), gh);
               const F2 qv = mul2(carry[i], old[i]);
-              dr = i ? fma2(gh, b2[i], dr) : mul2(gh, b2[i]);
+              dr = i ? fma2(gh, Bv[i], dr) : mul2(gh, Bv[i]);
               de = i ? fma2(qv, A2p[i], de) : mul2(qv, A2p[i]);
-              yy = i ? fma2(c2[i], h[j][i], yy) : mul2(c2[i], h[j][i]);
+              yy = i ? fma2(Cv[i], h[j][i], yy) : mul2(Cv[i], h[j][i]);
               local[i] = fma2(qv, d, local[i]);
               const float2 vb = halves(mul2(gh, w)), vc = halves(mul2(g, h[j][i]));
-              v[jj & 1][2 * i] = vb.x; v[jj & 1][2 * i + 1] = vb.y; v[jj & 1][4 + 2 * i] = vc.x; v[jj & 1][5 + 2 * i] = vc.y;
+              v[jj & 1][2 * i] = vb.x; v[jj & 1][2 * i + 1] = vb.y; v[jj & 1][S + 2 * i] = vc.x; v[jj & 1][S + 2 * i + 1] = vc.y;
             }
             sums[0][jj] = sum_halves(dr); sums[1][jj] = sum_halves(de); sums[2][jj] = sum_halves(yy);
             if (first) leave(s--);
-            if (jj % 2 == 0) sum_channels<L>(v, lane, [&](int odd, int i, float e) { to_bc[(k0 + j + odd) * 2 * NP + i] = e; });
+            if (jj % 2 == 0) sum_channels<C>(v, lane, [&](int odd, int i, float e) { to_bc[(k0 + j + odd) * 2 * NP + i] = e; });
           }
           sum_states<L>(sums, sl);
           put_sums<L>(to_drive + (k0 + j4) * YS, YS, sums[0], sl);
@@ -860,7 +948,7 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
       if (starts & 1u) leave(s_low);
       // dA over thousands of tokens: sums of 16, joined with what each addition rounds off
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
+      for (int i = 0; i < P; i++) {
         const F2 add = add2(local[i], dA_lost[i]), sum = add2(dA[i], add);
         dA_lost[i] = add2(add, neg2(add2(sum, neg2(dA[i]))));
         dA[i] = sum;
@@ -868,9 +956,7 @@ __global__ void __launch_bounds__(2 * NT, 2) scan_bwd_kernel(const __grid_consta
     }
     __syncthreads();
   }
-  const float2 d01 = halves(dA[0]), d23 = halves(dA[1]);
-  const float out[S] = {d01.x, d01.y, d23.x, d23.y};
-  store4(part + m * a.N, out, n0, a.N, ok, false);
+  store_pairs(part + m * a.N, dA, n0, a.N, ok, false);
 }
 
 // dB, dC [B*T][G][N] from the CTAs' sums [blocks][B*T][G][2][N]
@@ -899,8 +985,8 @@ __global__ void __launch_bounds__(256) scan_sum_m_kernel(const float* __restrict
 // One token per row: a channel's states over L lanes as above, two channels per thread.  Everything that does not depend on the
 // slot is asked for before the slot is looked at.
 template <class T, int L>
-__global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide, bool wide_bc) {
-  constexpr int CH = NT / L, U = 2;
+__global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide, bool wide_bc) {
+  constexpr int S = 4, CH = 128 / L, U = 2;
   const int b = blockIdx.x / blocks, sl = threadIdx.x % L, n0 = sl * S;
   const long long first = (long long)(blockIdx.x % blocks) * CH * U + threadIdx.x / L;
   float A2[U][S], u[U], d[U], z[U], D[U];
@@ -910,7 +996,7 @@ __global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ R
     const long long m = first + i * CH;
     const bool ok = m < a.M;
     const int g = ok ? (int)(m / (a.M / a.G)) : 0;
-    load4(A2[i], a.A + m * a.N, n0, a.N, ok, wide);
+    load_states(A2[i], a.A + m * a.N, n0, a.N, ok, wide);
     load_some<T, S>(Bv[i], static_cast<const T*>(a.Bm) + b * a.B_stride[0] + g * a.B_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
     load_some<T, S>(Cv[i], static_cast<const T*>(a.C) + b * a.C_stride[0] + g * a.C_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
     u[i] = ok ? to_f32(static_cast<const T*>(a.u)[b * a.u_stride + m]) : 0.f;
@@ -928,7 +1014,7 @@ __global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ R
   }
   float h[U][S], out[U];
 #pragma unroll
-  for (int i = 0; i < U; i++) load4(h[i], a.state + (slot * a.M + first + i * CH) * a.N, n0, a.N, first + i * CH < a.M, wide);
+  for (int i = 0; i < U; i++) load_states(h[i], a.state + (slot * a.M + first + i * CH) * a.N, n0, a.N, first + i * CH < a.M, wide);
 #pragma unroll
   for (int i = 0; i < U; i++) {
     float sig;
@@ -939,7 +1025,7 @@ __global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ R
       h[i][k] = fmaf(ex2(d[i] * (A2[i][k] * LOG2E)), h[i][k], d[i] * u[i] * to_f32(Bv[i].v[k]));
       out[i] = fmaf(to_f32(Cv[i].v[k]), h[i][k], out[i]);
     }
-    store4(a.state + (slot * a.M + first + i * CH) * a.N, h[i], n0, a.N, first + i * CH < a.M, wide);
+    store_states(a.state + (slot * a.M + first + i * CH) * a.N, h[i], n0, a.N, first + i * CH < a.M, wide);
   }
 #pragma unroll
   for (int k = L / 2; k > 0; k >>= 1)
@@ -955,15 +1041,21 @@ __global__ void __launch_bounds__(NT) scan_step_kernel(const __grid_constant__ R
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
-int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+// f(Shape()) for N states
 template <class F>
-void with_lanes(int N, F&& f) {
-  switch (lanes_of(N)) {
-    case 2: f(std::integral_constant<int, 2>()); break;
-    case 4: f(std::integral_constant<int, 4>()); break;
-    case 8: f(std::integral_constant<int, 8>()); break;
-    default: f(std::integral_constant<int, 16>()); break;
-  }
+void with_shape(int N, F&& f) {
+  if (N <= 8) f(Shape<4, 2, 128, 128, 32>());
+  else if (N <= 16) f(Shape<4, 4, 128, 128, 32>());
+  else if (N <= 32) f(Shape<8, 4, 128, 128, 32>());
+  else f(Shape<16, 4, 128, 128, 32>());
+}
+int channels_of(int N) { return N <= 16 ? 32 : N <= 32 ? 16 : 8; }   // per CTA, as above
+template <class F>
+void with_step_lanes(int N, F&& f) {
+  if (N <= 8) f(std::integral_constant<int, 2>());
+  else if (N <= 16) f(std::integral_constant<int, 4>());
+  else if (N <= 32) f(std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 16>());
 }
 
 struct Plan {
@@ -973,15 +1065,21 @@ struct Plan {
 };
 Plan make_plan(int B, int T, int M, int N, int G, bool backward) {
   Plan p{};
-  const int CH = NT / lanes_of(N), Mg = M / G;
+  const int CH = channels_of(N), Mg = M / G;
   p.blocks = (Mg + CH - 1) / CH;
   p.ctas = (long long)p.blocks * G * B;
-  const int tiles = (T + TT - 1) / TT;
-  long long want = p.ctas >= 74 ? 1 : 148 * 3 / p.ctas;
+  const int tiles = (T + TILE - 1) / TILE;
+  // Two CTAs fit an SM.  Segments cost a first pass (0.6 of the forward, 0.25 of the backward), and a CTA alone on its SM is 1.5
+  // times as fast as one beside another: fewer than three segments do not pay.  As many as fill the GPU once, or twice where
+  // that leaves fewer tokens to each place (64 CTAs: 9 segments instead of 4 measure 442 us against 487 for 16001 tokens of
+  // 2048 channels; 32 CTAs: 9 instead of 13, which take two rounds, 84 us against 94 for 2000 tokens of 1024 channels).
+  const long long once = 2 * 148 / p.ctas, twice = 4 * 148 / p.ctas;
+  long long want = 2 * once < 0.95 * twice ? twice : once;
+  if (once < 3) want = 1;
   if (want > tiles / 4) want = tiles / 4;
-  if (want < 3) want = 1;                             // two segments cost what they save
+  if (want < 3) want = 1;
   const int tiles_per = (int)((tiles + want - 1) / want);
-  p.seg_len = tiles_per * TT;
+  p.seg_len = tiles_per * TILE;
   p.segments = (T + p.seg_len - 1) / p.seg_len;
   const size_t rows = (size_t)B * p.segments * M;
   p.seg_state = p.segments > 1 ? rows * N : 0;
@@ -1056,15 +1154,16 @@ extern "C" int rewy_scan_fwd(const RewyScanArgs* a, rewy_stream_t st) {
   const cudaStream_t s = (cudaStream_t)st;
   cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
-    with_lanes(a->N, [&](auto l) {
+    with_shape(a->N, [&](auto c) {
       using T = decltype(t);
-      constexpr int L = l.value, bytes = sizeof(FwdShared<L>);
+      using C = decltype(c);
+      constexpr int bytes = sizeof(FwdShared<C>);
       if (plan.segments > 1) {
-        e = ensure_dynamic_smem<scan_fwd_kernel<T, L, true>>(bytes);
-        if (e == cudaSuccess) scan_fwd_kernel<T, L, true><<<(unsigned)(plan.ctas * (plan.segments - 1)), 2 * NT, bytes, s>>>(p);
+        e = ensure_dynamic_smem<scan_fwd_kernel<T, C, true>>(bytes);
+        if (e == cudaSuccess) scan_fwd_kernel<T, C, true><<<(unsigned)(plan.ctas * (plan.segments - 1)), C::THREADS, bytes, s>>>(p);
       }
-      if (e == cudaSuccess) e = ensure_dynamic_smem<scan_fwd_kernel<T, L, false>>(bytes);
-      if (e == cudaSuccess) scan_fwd_kernel<T, L, false><<<(unsigned)(plan.ctas * plan.segments), 2 * NT, bytes, s>>>(p);
+      if (e == cudaSuccess) e = ensure_dynamic_smem<scan_fwd_kernel<T, C, false>>(bytes);
+      if (e == cudaSuccess) scan_fwd_kernel<T, C, false><<<(unsigned)(plan.ctas * plan.segments), C::THREADS, bytes, s>>>(p);
     });
   });
   if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
@@ -1082,12 +1181,12 @@ extern "C" int rewy_scan_bwd(const RewyScanArgs* a, rewy_stream_t st) {
   cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    with_lanes(a->N, [&](auto l) {
-      constexpr int L = l.value;
-      e = ensure_dynamic_smem<scan_bwd_kernel<T, L>>(sizeof(BwdShared<L>));
+    with_shape(a->N, [&](auto c) {
+      using C = decltype(c);
+      e = ensure_dynamic_smem<scan_bwd_kernel<T, C>>(sizeof(BwdShared<C>));
       if (e != cudaSuccess) return;
-      if (plan.segments > 1) scan_bwd_state_kernel<T, L><<<(unsigned)(plan.ctas * (plan.segments - 1)), NT, 0, s>>>(p);
-      scan_bwd_kernel<T, L><<<(unsigned)(plan.ctas * plan.segments), 2 * NT, sizeof(BwdShared<L>), s>>>(p);
+      if (plan.segments > 1) scan_bwd_state_kernel<T, C><<<(unsigned)(plan.ctas * (plan.segments - 1)), C::THREADS, 0, s>>>(p);
+      scan_bwd_kernel<T, C><<<(unsigned)(plan.ctas * plan.segments), C::THREADS, sizeof(BwdShared<C>), s>>>(p);
     });
     if (e != cudaSuccess) return;
     const long long rows = (long long)a->B * a->T * a->G;
@@ -1112,9 +1211,9 @@ extern "C" int rewy_scan_step(const RewyScanStepArgs* a, rewy_stream_t st) {
   bool wide_bc = a->N % 4 == 0 && !unaligned16(a->Bm) && !unaligned16(a->C);
   for (int i = 0; i < 2; i++) wide_bc = wide_bc && a->B_stride[i] % 4 == 0 && a->C_stride[i] % 4 == 0;
   with_type(a->dtype, [&](auto t) {
-    with_lanes(a->N, [&](auto l) {
-      const int per = NT / l.value * 2, blocks = (a->M + per - 1) / per;
-      scan_step_kernel<decltype(t), l.value><<<(unsigned)((long long)blocks * a->B), NT, 0, (cudaStream_t)st>>>(*a, blocks, wide, wide_bc);
+    with_step_lanes(a->N, [&](auto l) {
+      const int per = 128 / l.value * 2, blocks = (a->M + per - 1) / per;
+      scan_step_kernel<decltype(t), l.value><<<(unsigned)((long long)blocks * a->B), 128, 0, (cudaStream_t)st>>>(*a, blocks, wide, wide_bc);
     });
   });
   return launched("selective scan step");
