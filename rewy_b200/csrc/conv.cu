@@ -39,6 +39,18 @@ __device__ __forceinline__ Span span_after(const RewyConvArgs& a, const Span& p)
   return {s, p.end, s + 1 < a.num_seqs ? min(max(a.cu_seqlens[s + 1], p.end + 1), a.T) : a.T};
 }
 
+// The W taps of a channel
+template <int W>
+__device__ __forceinline__ void load_taps(float (&w)[W], const void* weight, int dtype, long long channel) {
+  if (W == 4 && dtype == REWY_F32 && (reinterpret_cast<uintptr_t>(weight) & 15) == 0) {
+    const float4 v = __ldg(static_cast<const float4*>(weight) + channel);
+    w[0] = v.x; w[1] = v.y; w[W > 2 ? 2 : 0] = v.z; w[W - 1] = v.w;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < W; j++) w[j] = param_at(weight, dtype, channel * W + j);
+}
+
 template <class T, int W, int V, bool WIDE>
 struct Columns {  // a warp's channels
   const RewyConvArgs& a;
@@ -46,22 +58,30 @@ struct Columns {  // a warp's channels
   long long state_row;  // elements of one sequence's state
   int c0, valid;
   static constexpr bool wide = WIDE;
-  float weight[W][V], bias[V];
+  static constexpr int P = V / 2;   // arithmetic on two channels at a time
+  F2 weight[W][P], bias[P];
 
   __device__ __forceinline__ Columns(const ConvParams& p, int b, int channel)
       : a(p.a), x(static_cast<const T*>(p.a.x) + b * p.a.x_batch_stride), state_row((long long)(W - 1) * p.a.D), c0(channel),
         valid(WIDE ? V : p.a.D - channel) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
+    for (int i = 0; i < P; i++) {
+      float taps[2][W] = {}, both_bias[2] = {};
 #pragma unroll
-      for (int w = 0; w < W; w++) weight[w][i] = i < valid ? param_at(a.weight, a.param_dtype, (long long)(c0 + i) * W + w) : 0.f;
-      bias[i] = a.bias != nullptr && i < valid ? param_at(a.bias, a.param_dtype, c0 + i) : 0.f;
+      for (int k = 0; k < 2; k++)
+        if (2 * i + k < valid) {
+          load_taps(taps[k], a.weight, a.param_dtype, c0 + 2 * i + k);
+          if (a.bias != nullptr) both_bias[k] = param_at(a.bias, a.param_dtype, c0 + 2 * i + k);
+        }
+#pragma unroll
+      for (int w = 0; w < W; w++) weight[w][i] = pair(taps[0][w], taps[1][w]);
+      bias[i] = pair(both_bias[0], both_bias[1]);
     }
   }
   __device__ __forceinline__ void load_x(Pack<T, V>& d, int t) const { load_some<T, V>(d, x + t * a.x_token_stride + c0, valid, wide); }
   __device__ __forceinline__ long long at(int row, long long rows_before) const { return (rows_before + row) * a.D + c0; }
   // the W-1 inputs before token t of sequence s
-  __device__ __forceinline__ void window(float (&win)[W - 1][V], const Span& s, int t) const {
+  __device__ __forceinline__ void window(F2 (&win)[W - 1][P], const Span& s, int t) const {
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
       const int pos = t - (W - 1) + j;
@@ -70,7 +90,7 @@ struct Columns {  // a warp's channels
       else if (a.initial_state != nullptr)
         load_some<T, V>(v, static_cast<const T*>(a.initial_state) + s.s * state_row + (long long)(W - 1 + pos - s.begin) * a.D + c0, valid, wide);
       else zero_pack(v);
-      to_floats(win[j], v);
+      to_pairs(win[j], v);
     }
   }
 };
@@ -104,6 +124,7 @@ template <class T, int W, int V, bool WIDE>
 __global__ void __launch_bounds__(WARPS * 32, 4) conv_fwd_kernel(const __grid_constant__ ConvParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   const Ring<T, V, 1> ring(smem);
+  constexpr int P = V / 2;
   const int channel = (blockIdx.x % p.channel_blocks * 32 + (threadIdx.x & 31)) * V;
   const unsigned rest = blockIdx.x / p.channel_blocks;
   const int b = rest / p.token_blocks;
@@ -115,16 +136,19 @@ __global__ void __launch_bounds__(WARPS * 32, 4) conv_fwd_kernel(const __grid_co
   Span s = span_at(p.a, b, t0);
   for (int from = t0; from < t1;) {   // the part of one sequence that lies in the block
     const int to = min(t1, s.end);
-    float win[W - 1][V];
+    F2 win[W - 1][P];
     c.window(win, s, from);
     auto token = [&](int t, const Pack<T, V>& in) {
-      float now[V], pre[V];
-      to_floats(now, in);
+      F2 now[P];
+      float pre[V];
+      to_pairs(now, in);
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        pre[i] = fmaf(c.weight[W - 1][i], now[i], c.bias[i]);
+      for (int i = 0; i < P; i++) {
+        F2 sum = fma2(c.weight[W - 1][i], now[i], c.bias[i]);
 #pragma unroll
-        for (int w = 0; w < W - 1; w++) pre[i] = fmaf(c.weight[w][i], win[w][i], pre[i]);
+        for (int w = 0; w < W - 1; w++) sum = fma2(c.weight[w][i], win[w][i], sum);
+        const float2 h = halves(sum);
+        pre[2 * i] = h.x; pre[2 * i + 1] = h.y;
 #pragma unroll
         for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
         win[W - 2][i] = now[i];
@@ -162,7 +186,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) conv_fwd_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < W - 1; j++) {
         Pack<T, V> v;
-        from_floats(v, win[j]);
+        from_pairs(v, win[j]);
         store_some<T, V>(static_cast<T*>(p.a.final_state) + s.s * c.state_row + (long long)j * p.a.D + channel, v, c.valid, c.wide);
       }
     }
@@ -181,7 +205,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) conv_bwd_kernel(const __grid_co
   const unsigned rest = blockIdx.x / p.channel_blocks;
   const int b = rest / p.token_blocks;
   const long long first = ((long long)(rest % p.token_blocks) * WARPS + warp) * p.token_block;
-  float dw[W][V] = {}, db[V] = {};
+  constexpr int P = V / 2;
+  F2 dw[W][P], db[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    db[i] = both(0.f);
+#pragma unroll
+    for (int w = 0; w < W; w++) dw[w][i] = both(0.f);
+  }
   if (channel < a.D && first < a.T) {
     const int t0 = (int)first, t1 = (int)min(first + p.token_block, (long long)a.T);
     const Columns<T, W, V, WIDE> c(p, b, channel);
@@ -191,8 +222,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) conv_bwd_kernel(const __grid_co
     Span s = span_at(a, b, t0);
     for (int from = t0; from < t1;) {        // the part of one sequence that lies in the block
       const int to = min(t1, s.end);
-      float win[W - 1][V], g[W - 1][V] = {};
+      F2 win[W - 1][P], g[W - 1][P];
       c.window(win, s, from);
+#pragma unroll
+      for (int j = 0; j < W - 1; j++)
+#pragma unroll
+        for (int i = 0; i < P; i++) g[j][i] = both(0.f);
       const int stop = to + W - 1, real = min(stop, s.end);   // tokens of the next block too; beyond the sequence there is no g
       auto ask = [&](int group) {
 #pragma unroll
@@ -207,32 +242,35 @@ __global__ void __launch_bounds__(WARPS * 32, 2) conv_bwd_kernel(const __grid_co
       };
       // Token t of the sequence: its g, and out, the complete gradient W-1 tokens before it.  OWN: it counts for dweight.
       auto step = [&](auto own, const Pack<T, V>& in, const Pack<T, V>& d, float (&out)[V]) {
-        float x[V], gi[V];
-        to_floats(x, in);
-        to_floats(gi, d);
+        F2 x[P], gi[P];
+        to_pairs(x, in);
+        to_pairs(gi, d);
         if (a.activation)
 #pragma unroll
-          for (int i = 0; i < V; i++) {
-            float pre = fmaf(c.weight[W - 1][i], x[i], c.bias[i]);
+          for (int i = 0; i < P; i++) {
+            F2 pre = fma2(c.weight[W - 1][i], x[i], c.bias[i]);
 #pragma unroll
-            for (int w = 0; w < W - 1; w++) pre = fmaf(c.weight[w][i], win[w][i], pre);
-            const float sig = sigmoid_fast(pre);
-            gi[i] *= sig * fmaf(pre, 1.f - sig, 1.f);
+            for (int w = 0; w < W - 1; w++) pre = fma2(c.weight[w][i], win[w][i], pre);
+            const float2 h = halves(pre);
+            const F2 sig = pair(sigmoid_fast(h.x), sigmoid_fast(h.y));
+            gi[i] = mul2(mul2(gi[i], sig), fma2(pre, fma2(sig, both(-1.f), both(1.f)), both(1.f)));
           }
 #pragma unroll
-        for (int i = 0; i < V; i++) {
+        for (int i = 0; i < P; i++) {
           if (own.value) {
 #pragma unroll
-            for (int w = 0; w < W - 1; w++) dw[w][i] = fmaf(gi[i], win[w][i], dw[w][i]);
-            dw[W - 1][i] = fmaf(gi[i], x[i], dw[W - 1][i]);
-            db[i] += gi[i];
+            for (int w = 0; w < W - 1; w++) dw[w][i] = fma2(gi[i], win[w][i], dw[w][i]);
+            dw[W - 1][i] = fma2(gi[i], x[i], dw[W - 1][i]);
+            db[i] = add2(db[i], gi[i]);
           }
 #pragma unroll
           for (int j = 0; j < W - 2; j++) win[j][i] = win[j + 1][i];
           win[W - 2][i] = x[i];
-          out[i] = c.weight[0][i] * gi[i];
+          F2 sum = mul2(c.weight[0][i], gi[i]);
 #pragma unroll
-          for (int w = 1; w < W; w++) out[i] = fmaf(c.weight[w][i], g[W - 1 - w][i], out[i]);
+          for (int w = 1; w < W; w++) sum = fma2(c.weight[w][i], g[W - 1 - w][i], sum);
+          const float2 h = halves(sum);
+          out[2 * i] = h.x; out[2 * i + 1] = h.y;
 #pragma unroll
           for (int j = 0; j < W - 2; j++) g[j][i] = g[j + 1][i];
           g[W - 2][i] = gi[i];
@@ -300,10 +338,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) conv_bwd_kernel(const __grid_co
   float(*const sums)[W + 1][32 * V] = reinterpret_cast<float(*)[W + 1][32 * V]>(smem);
   static_assert(sizeof(float) * WARPS * (W + 1) * 32 * V <= Ring<T, V, 2>::BYTES, "the sums fit the rings");
 #pragma unroll
-  for (int i = 0; i < V; i++) {
+  for (int i = 0; i < P; i++) {
 #pragma unroll
-    for (int w = 0; w < W; w++) sums[warp][w][lane * V + i] = dw[w][i];
-    sums[warp][W][lane * V + i] = db[i];
+    for (int w = 0; w <= W; w++) *reinterpret_cast<unsigned long long*>(&sums[warp][w][lane * V + 2 * i]) = (w < W ? dw[w < W ? w : 0][i] : db[i]).v;
   }
   __syncthreads();
   const int c0 = blockIdx.x % p.channel_blocks * 32 * V;
@@ -335,36 +372,52 @@ template <class T, int V>
 __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ RewyConvStepArgs a, int channel_blocks, bool wide) {
   const int b = blockIdx.x / channel_blocks, c0 = (blockIdx.x % channel_blocks * 128 + threadIdx.x) * V;
   const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
-  if (c0 >= a.D) return;
   const int valid = a.D - c0, W = a.W;
-  T* y = static_cast<T*>(a.y) + (long long)b * a.D + c0;
-  Pack<T, V> now;
-  if (slot < 0) {
-    zero_pack(now);
-    store_some<T, V>(y, now, valid, wide);
-    return;
-  }
-  T* state = static_cast<T*>(a.state) + slot * (W - 1) * a.D + c0;
-  load_some<T, V>(now, static_cast<const T*>(a.x) + b * a.x_stride + c0, valid, wide);
-  Pack<T, V> old[3];
+  T* state = static_cast<T*>(a.state) + (slot < 0 ? 0 : slot) * (W - 1) * a.D + c0;
+  Pack<T, V> now, old[3];
 #pragma unroll
   for (int j = 0; j < 3; j++)
-    if (j < W - 1) {   // (written in this kernel: not through the read-only path)
+    if (j < W - 1 && slot >= 0 && valid > 0) {   // (written in this kernel: not through the read-only path)
       if (wide && valid >= V) old[j] = *reinterpret_cast<const Pack<T, V>*>(state + (long long)j * a.D);
       else
         for (int i = 0; i < V; i++) old[j].v[i] = i < valid ? state[(long long)j * a.D + i] : from_f32<T>(0.f);
+    } else {
+      zero_pack(old[j]);
     }
-  Pack<T, V> out;
+  load_some<T, V>(now, static_cast<const T*>(a.x) + b * a.x_stride + c0, valid, wide);
+  float weight[V][4], pre[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    if (i >= valid) continue;
-    const long long row = (long long)(c0 + i) * W;
-    float pre = fmaf(param_at(a.weight, a.param_dtype, row + W - 1), to_f32(now.v[i]), a.bias != nullptr ? param_at(a.bias, a.param_dtype, c0 + i) : 0.f);
+    pre[i] = a.bias != nullptr && i < valid ? param_at(a.bias, a.param_dtype, c0 + i) : 0.f;
+    if (W == 4 && i < valid) {
+      load_taps<4>(weight[i], a.weight, a.param_dtype, c0 + i);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 3; j++)
-      if (j < W - 1) pre = fmaf(param_at(a.weight, a.param_dtype, row + j), to_f32(old[j].v[i]), pre);
-    out.v[i] = from_f32<T>(a.activation ? pre * sigmoid_fast(pre) : pre);
+      for (int j = 0; j < 4; j++) weight[i][j] = j < W && i < valid ? param_at(a.weight, a.param_dtype, (long long)(c0 + i) * W + j) : 0.f;
+    }
   }
+  const bool skip = row_repeats(a.slots, a.slots_i64, b, slot) || slot < 0;
+  if (valid <= 0) return;
+  T* y = static_cast<T*>(a.y) + (long long)b * a.D + c0;
+  Pack<T, V> out;
+  if (skip) {
+    zero_pack(out);
+    store_some<T, V>(y, out, valid, wide);
+    return;
+  }
+  float x[V];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (j >= W) continue;
+    if (j == W - 1) to_floats(x, now);
+    else to_floats(x, old[j < 3 ? j : 2]);
+#pragma unroll
+    for (int i = 0; i < V; i++) pre[i] = fmaf(weight[i][j], x[i], pre[i]);
+  }
+  if (a.activation)
+#pragma unroll
+    for (int i = 0; i < V; i++) pre[i] *= sigmoid_fast(pre[i]);
+  from_floats(out, pre);
   store_some<T, V>(y, out, valid, wide);
 #pragma unroll
   for (int j = 0; j < 3; j++)

@@ -41,11 +41,7 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
   const int hv = rest % a.HV, b = rest / a.HV, v0 = slice * SLICE;
   const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool), head = (long long)b * a.HV + hv;
   T* o = static_cast<T*>(a.o) + head * a.V;
-  if (slot < 0) {
-    if (tid < SLICE && v0 + tid < a.V) o[v0 + tid] = from_f32<T>(0.f);
-    return;
-  }
-  float* state = a.state + (slot * a.HV + hv) * ((long long)a.K * a.V);
+  float* state = a.state + ((slot < 0 ? 0 : slot) * a.HV + hv) * ((long long)a.K * a.V);
   // this thread's state vectors: [K,V] four value channels of key rows kr + 16 i; [V,K] four key channels of value rows vr + 4 i
   const int c4 = V_FIRST ? lane * 4 : (tid & 7) * 4, r0 = V_FIRST ? warp : tid >> 3;
   float4 S[ROWS];
@@ -53,25 +49,36 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
   for (int i = 0; i < ROWS; i++) {
     const int r = V_FIRST ? v0 + r0 + 4 * i : r0 + 16 * i, c = V_FIRST ? c4 : v0 + c4;
     const int rows = V_FIRST ? a.V : a.K, cols = V_FIRST ? a.K : a.V;
-    S[i] = load_state<WIDE>(state + (long long)r * cols + c, r < rows ? cols - c : 0);
+    S[i] = load_state<WIDE>(state + (long long)r * cols + c, r < rows && slot >= 0 ? cols - c : 0);
+  }
+  // Everything is asked for before anything is used: what the state should give for k (before the part that is erased is taken
+  // off), the gates of this thread's key channel, the write strength.
+  constexpr int TARGETS = V_FIRST ? ROWS : 4;
+  T value[TARGETS], write[TARGETS];
+#pragma unroll
+  for (int i = 0; i < TARGETS; i++) {
+    const int v = v0 + (V_FIRST ? r0 + 4 * i : c4 + i);
+    value[i] = v < a.V ? static_cast<const T*>(a.v)[head * a.V + v] : from_f32<T>(0.f);
+    write[i] = a.family == REWY_GDN2 && v < a.V ? static_cast<const T*>(a.w_gate)[head * a.V + v] : from_f32<T>(1.f);
   }
   const long long qk = ((long long)b * a.H + hv / (a.HV / a.H)) * a.K;
-  float q = 0.f, k = 0.f, erase = 1.f, decay = 1.f;
-  if (tid < a.K) {
-    q = to_f32(static_cast<const T*>(a.q)[qk + tid]);
-    k = to_f32(static_cast<const T*>(a.k)[qk + tid]);
-    if (a.family == REWY_GDN2) erase = to_f32(static_cast<const T*>(a.b_gate)[head * a.K + tid]);
-    if (a.family == REWY_GDN) {
-      decay = ex2(LOG2E * param_at(a.g, a.gate_dtype, head));
-    } else if (a.family != REWY_DELTA) {
-      float g = param_at(a.g, a.gate_dtype, head * a.K + tid);
-      if (a.A_log != nullptr) {
-        float sig;
-        g = -ex2(LOG2E * a.A_log[hv]) * softplus_fast(g + (a.dt_bias != nullptr ? a.dt_bias[(long long)hv * a.K + tid] : 0.f), sig);
-      }
-      decay = ex2(LOG2E * g);
-    }
+  const bool key = tid < a.K, fused = a.A_log != nullptr;
+  const T raw_q = key ? static_cast<const T*>(a.q)[qk + tid] : from_f32<T>(0.f), raw_k = key ? static_cast<const T*>(a.k)[qk + tid] : from_f32<T>(0.f);
+  const T raw_erase = key && a.family == REWY_GDN2 ? static_cast<const T*>(a.b_gate)[head * a.K + tid] : from_f32<T>(1.f);
+  float beta = a.family != REWY_GDN2 ? param_at(a.beta, a.beta_dtype, head) : 1.f;
+  float g = a.family == REWY_DELTA || !key ? 0.f : param_at(a.g, a.gate_dtype, a.family == REWY_GDN ? head : head * a.K + tid);
+  const float rate = fused ? a.A_log[hv] : 0.f, shift = fused && key && a.dt_bias != nullptr ? a.dt_bias[(long long)hv * a.K + tid] : 0.f;
+  if (row_repeats(a.slots, a.slots_i64, b, slot) || slot < 0) {
+    if (tid < SLICE && v0 + tid < a.V) o[v0 + tid] = from_f32<T>(0.f);
+    return;
   }
+  const float q = to_f32(raw_q), k = to_f32(raw_k), erase = to_f32(raw_erase);
+  if (fused && key) {
+    float sig;
+    g = -ex2(LOG2E * rate) * softplus_fast(g + shift, sig);
+  }
+  const float decay = ex2(LOG2E * g);
+  if (a.beta_scale != 0.f) beta = a.beta_scale * sigmoid_fast(beta);
   float qq = q * q, kk = k * k, dot = q * k;
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) {
@@ -91,16 +98,6 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
   serase[tid] = k * kn * erase;
   sdecay[tid] = decay;
   __syncthreads();
-  float beta = 1.f;
-  if (a.family != REWY_GDN2) {
-    beta = param_at(a.beta, a.beta_dtype, head);
-    if (a.beta_scale != 0.f) beta = a.beta_scale * sigmoid_fast(beta);
-  }
-  auto target = [&](int v) {   // what the state should give for k, before the erase part is taken off
-    const float x = v < a.V ? to_f32(static_cast<const T*>(a.v)[head * a.V + v]) : 0.f;
-    return a.family == REWY_GDN2 && v < a.V ? x * to_f32(static_cast<const T*>(a.w_gate)[head * a.V + v]) : x;
-  };
-
   if constexpr (!V_FIRST) {
     float e[4] = {}, p[4] = {};
 #pragma unroll
@@ -127,7 +124,7 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
       const int c = c4 + i;
       const float erased = (part[0][0][c] + part[1][0][c]) + (part[2][0][c] + part[3][0][c]);
       const float seen = (part[0][1][c] + part[1][1][c]) + (part[2][1][c] + part[3][1][c]);
-      r4[i] = beta * (target(v0 + c) - erased);
+      r4[i] = beta * (to_f32(value[i]) * to_f32(write[i]) - erased);
       if (tid < 8 && v0 + c < a.V) o[v0 + c] = from_f32<T>(a.scale * fmaf(dot, r4[i], seen));
     }
 #pragma unroll
@@ -151,7 +148,7 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
         e += __shfl_xor_sync(0xffffffffu, e, m);
         p += __shfl_xor_sync(0xffffffffu, p, m);
       }
-      const float r = beta * (target(v) - e);
+      const float r = beta * (to_f32(value[i]) * to_f32(write[i]) - e);
       if (lane == 0 && v < a.V) o[v] = from_f32<T>(a.scale * fmaf(dot, r, p));
       S[i].x = fmaf(kx.x, r, S[i].x); S[i].y = fmaf(kx.y, r, S[i].y); S[i].z = fmaf(kx.z, r, S[i].z); S[i].w = fmaf(kx.w, r, S[i].w);
       store_state<WIDE>(state + (long long)v * a.K + c4, S[i], v < a.V ? a.K - c4 : 0);

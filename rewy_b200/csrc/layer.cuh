@@ -183,6 +183,23 @@ __device__ __forceinline__ float sum_halves(F2 a) {
   const float2 h = halves(a);
   return h.x + h.y;
 }
+template <class T, int V>
+__device__ __forceinline__ void to_pairs(F2 (&x)[V / 2], const Pack<T, V>& p) {
+  float f[V];
+  to_floats(f, p);
+#pragma unroll
+  for (int i = 0; i < V / 2; i++) x[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+template <class T, int V>
+__device__ __forceinline__ void from_pairs(Pack<T, V>& p, const F2 (&x)[V / 2]) {
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V / 2; i++) {
+    const float2 h = halves(x[i]);
+    f[2 * i] = h.x; f[2 * i + 1] = h.y;
+  }
+  from_floats(p, f);
+}
 __device__ __forceinline__ F2 ex2_2(F2 a) {
   const float2 h = halves(a);
   return pair(ex2(h.x), ex2(h.y));
@@ -215,16 +232,21 @@ __device__ __forceinline__ int packed_sequence(const int* cu, int num_seqs, int 
   return lo;
 }
 
-// The row of a state pool that row b of a batch of single tokens works on: -1 (nothing is done) if the index is outside the pool
-// or an earlier row has the same one.  Called by all threads of a block.
+// The state of a pool that row b of a batch of single tokens works on, -1 if its index lies outside the pool; and whether an earlier
+// row has the same index, which is asked by all threads of a block together, after they have asked for their part of the state:
+// then the row is skipped like one without a state.
+__device__ __forceinline__ long long slot_at(const void* slots, int slots_are_i64, int i) {
+  return slots_are_i64 ? static_cast<const long long*>(slots)[i] : (long long)static_cast<const int*>(slots)[i];
+}
 __device__ __forceinline__ long long pool_row(const void* slots, int slots_are_i64, int b, long long pool) {
-  if (slots == nullptr) return b;
-  auto at = [&](int i) { return slots_are_i64 ? static_cast<const long long*>(slots)[i] : (long long)static_cast<const int*>(slots)[i]; };
-  const long long mine = at(b);
+  const long long mine = slots == nullptr ? b : slot_at(slots, slots_are_i64, b);
+  return mine < 0 || mine >= pool ? -1 : mine;
+}
+__device__ __forceinline__ bool row_repeats(const void* slots, int slots_are_i64, int b, long long mine) {
+  if (slots == nullptr || mine < 0) return false;   // the same for all threads
   bool again = false;
-  for (int i = threadIdx.x; i < b; i += blockDim.x) again |= at(i) == mine;
-  const int any = __syncthreads_or(again);
-  return any || mine < 0 || mine >= pool ? -1 : mine;
+  for (int i = threadIdx.x; i < b; i += blockDim.x) again |= slot_at(slots, slots_are_i64, i) == mine;
+  return __syncthreads_or(again);
 }
 
 inline bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

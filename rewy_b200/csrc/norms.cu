@@ -21,6 +21,7 @@ struct NormParams {
   RewyNormArgs a;
   bool wide;
   float* partial;  // [CTAs][2][D]
+  float inv_D;
 };
 
 // (rows at one distance need no division; fewer than 2^32 rows a short one)
@@ -47,11 +48,11 @@ __device__ __forceinline__ void row_sums(float (&x)[N], float* red, int parity) 
       for (int i = 0; i < N; i++) to[warp * N + i] = x[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      x[i] = 0.f;
+    for (int i = 0; i < N; i++) x[i] = to[(first + (threadIdx.x & (WARPS - 1))) * N + i];
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) x[i] += to[(first + w) * N + i];
-    }
+    for (int m = WARPS / 2; m > 0; m >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], m);
   }
 }
 
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
         }
       }
       row_sums<TPR>(sum, red, parity);
-      const float rs = rsqrtf(sum[0] / a.D + a.eps);
+      const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps));
       if (!real) return;
       T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
       }
       row_sums<TPR>(sum, red, parity);
       if (!real) return;
-      const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
+      const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), back = rs * rs * rs * (sum[1] * p.inv_D);
 #pragma unroll
       for (int v = 0; v < NV; v++) {
         const int c = Y::column(v);
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
     }
     row_sums<TPR>(sum, red, parity);
     if (!real) return;
-    const float rs = rsqrtf(sum[0] / a.D + a.eps);
+    const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps));
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
     }
     row_sums<TPR>(sum, red, parity);
     if (!real) return;
-    const float rs = rsqrtf(sum[0] / a.D + a.eps), back = rs * rs * rs * (sum[1] / a.D);
+    const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), back = rs * rs * rs * (sum[1] * p.inv_D);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
@@ -547,7 +548,7 @@ int check_norm(const RewyNormArgs* a) {
   return REWY_OK;
 }
 NormParams norm_params(const RewyNormArgs& a) {
-  NormParams p{a, false, static_cast<float*>(a.workspace)};
+  NormParams p{a, false, static_cast<float*>(a.workspace), 1.f / (float)a.D};
   bool w = a.D % E == 0;
   for (const void* q : {a.x, a.gate, a.residual, (const void*)a.y, (const void*)a.residual_out, a.dy, a.dresidual_out, (const void*)a.dx, (const void*)a.dgate,
                         (const void*)a.dresidual})

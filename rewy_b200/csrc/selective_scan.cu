@@ -982,20 +982,20 @@ __global__ void __launch_bounds__(256) scan_sum_m_kernel(const float* __restrict
   if (to != nullptr) *to = sum;
 }
 
-// One token per row: a channel's states over L lanes as above, two channels per thread.  Everything that does not depend on the
-// slot is asked for before the slot is looked at.
+// One token per row: a channel's states over L lanes as above, two channels per thread.
 template <class T, int L>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ RewyScanStepArgs a, int blocks, bool wide, bool wide_bc) {
   constexpr int S = 4, CH = 128 / L, U = 2;
   const int b = blockIdx.x / blocks, sl = threadIdx.x % L, n0 = sl * S;
   const long long first = (long long)(blockIdx.x % blocks) * CH * U + threadIdx.x / L;
-  float A2[U][S], u[U], d[U], z[U], D[U];
+  const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
+  float A2[U][S], u[U], d[U], z[U], D[U], h[U][S], out[U];
   Pack<T, S> Bv[U], Cv[U];
 #pragma unroll
   for (int i = 0; i < U; i++) {
     const long long m = first + i * CH;
     const bool ok = m < a.M;
-    const int g = ok ? (int)(m / (a.M / a.G)) : 0;
+    const int g = ok && a.G > 1 ? (int)m / (a.M / a.G) : 0;
     load_states(A2[i], a.A + m * a.N, n0, a.N, ok, wide);
     load_some<T, S>(Bv[i], static_cast<const T*>(a.Bm) + b * a.B_stride[0] + g * a.B_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
     load_some<T, S>(Cv[i], static_cast<const T*>(a.C) + b * a.C_stride[0] + g * a.C_stride[1] + n0, ok ? a.N - n0 : 0, wide_bc);
@@ -1004,17 +1004,15 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ 
     z[i] = ok && a.z != nullptr ? to_f32(static_cast<const T*>(a.z)[b * a.z_stride + m]) : 0.f;
     D[i] = ok && a.D != nullptr ? a.D[m] : 0.f;
   }
-  const long long slot = pool_row(a.slots, a.slots_i64, b, a.pool);
+#pragma unroll
+  for (int i = 0; i < U; i++) load_states(h[i], a.state + (slot * a.M + first + i * CH) * a.N, n0, a.N, slot >= 0 && first + i * CH < a.M, wide);
   T* y = static_cast<T*>(a.y) + (long long)b * a.M;
-  if (slot < 0) {
+  if (row_repeats(a.slots, a.slots_i64, b, slot) || slot < 0) {
 #pragma unroll
     for (int i = 0; i < U; i++)
       if (first + i * CH < a.M && sl == 0) y[first + i * CH] = from_f32<T>(0.f);
     return;
   }
-  float h[U][S], out[U];
-#pragma unroll
-  for (int i = 0; i < U; i++) load_states(h[i], a.state + (slot * a.M + first + i * CH) * a.N, n0, a.N, first + i * CH < a.M, wide);
 #pragma unroll
   for (int i = 0; i < U; i++) {
     float sig;
