@@ -22,7 +22,7 @@ __device__ __forceinline__ float4 load_state(const float* p, int valid) {
 template <bool WIDE>
 __device__ __forceinline__ void store_state(float* p, float4 x, int valid) {
   if constexpr (WIDE) {
-    if (valid > 0) *reinterpret_cast<float4*>(p) = x;
+    if (valid > 0) __stcs(reinterpret_cast<float4*>(p), x);   // not read again before the next token: 62 -> 56 us
     return;
   }
   if (valid > 0) p[0] = x.x;
@@ -34,7 +34,8 @@ __device__ __forceinline__ void store_state(float* p, float4 x, int valid) {
 // WIDE: every row of the state starts on 16 bytes and holds whole groups of four
 template <class T, bool V_FIRST, bool WIDE>
 __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant__ RewyDeltaStepArgs a, int slices) {
-  __shared__ float sk[NT], sq[NT], serase[NT], sdecay[NT], red[4][3], part[4][2][SLICE];
+  __shared__ __align__(16) float sk[NT], sq[NT], serase[NT], sdecay[NT], red[3][4];
+  __shared__ __align__(16) float part[4][2][SLICE];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x % slices;
   const unsigned rest = blockIdx.x / slices;
@@ -86,11 +87,13 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
     kk += __shfl_xor_sync(0xffffffffu, kk, m);
     dot += __shfl_xor_sync(0xffffffffu, dot, m);
   }
-  if (lane == 0) { red[warp][0] = qq; red[warp][1] = kk; red[warp][2] = dot; }
+  if (lane == 0) { red[0][warp] = qq; red[1][warp] = kk; red[2][warp] = dot; }
   __syncthreads();
-  qq = red[0][0] + red[1][0] + red[2][0] + red[3][0];
-  kk = red[0][1] + red[1][1] + red[2][1] + red[3][1];
-  dot = red[0][2] + red[1][2] + red[2][2] + red[3][2];
+  auto total = [&](int i) {
+    const float4 x = *reinterpret_cast<const float4*>(red[i]);
+    return (x.x + x.y) + (x.z + x.w);
+  };
+  qq = total(0); kk = total(1); dot = total(2);
   const float qn = a.qk_norm ? rsqrtf(qq + 1e-6f) : 1.f, kn = a.qk_norm ? rsqrtf(kk + 1e-6f) : 1.f;
   dot *= qn * kn;
   sq[tid] = q * qn;
@@ -99,40 +102,53 @@ __global__ void __launch_bounds__(NT, 8) delta_step_kernel(const __grid_constant
   sdecay[tid] = decay;
   __syncthreads();
   if constexpr (!V_FIRST) {
-    float e[4] = {}, p[4] = {};
+    F2 x[ROWS][2], e[2] = {both(0.f), both(0.f)}, p[2] = {both(0.f), both(0.f)};
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
       const int r = r0 + 16 * i;
-      const float d = sdecay[r], x = serase[r], y = sq[r];
-      S[i].x *= d; S[i].y *= d; S[i].z *= d; S[i].w *= d;
-      e[0] = fmaf(x, S[i].x, e[0]); e[1] = fmaf(x, S[i].y, e[1]); e[2] = fmaf(x, S[i].z, e[2]); e[3] = fmaf(x, S[i].w, e[3]);
-      p[0] = fmaf(y, S[i].x, p[0]); p[1] = fmaf(y, S[i].y, p[1]); p[2] = fmaf(y, S[i].z, p[2]); p[3] = fmaf(y, S[i].w, p[3]);
+      const F2 d = both(sdecay[r]), er = both(serase[r]), qr = both(sq[r]);
+      x[i][0] = mul2(pair(S[i].x, S[i].y), d);
+      x[i][1] = mul2(pair(S[i].z, S[i].w), d);
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        e[k] = fma2(er, x[i][k], e[k]);
+        p[k] = fma2(qr, x[i][k], p[k]);
+      }
+    }
+    float sums[8];   // e, then p
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const float2 a2 = halves(e[k]), b2 = halves(p[k]);
+      sums[2 * k] = a2.x; sums[2 * k + 1] = a2.y; sums[4 + 2 * k] = b2.x; sums[5 + 2 * k] = b2.y;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int m = 16; m >= 8; m >>= 1)
 #pragma unroll
-      for (int m = 16; m >= 8; m >>= 1) {
-        e[i] += __shfl_xor_sync(0xffffffffu, e[i], m);
-        p[i] += __shfl_xor_sync(0xffffffffu, p[i], m);
-      }
-      if (lane < 8) { part[warp][0][c4 + i] = e[i]; part[warp][1][c4 + i] = p[i]; }
+      for (int i = 0; i < 8; i++) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], m);
+    if (lane < 8) {
+      *reinterpret_cast<float4*>(&part[warp][0][c4]) = make_float4(sums[0], sums[1], sums[2], sums[3]);
+      *reinterpret_cast<float4*>(&part[warp][1][c4]) = make_float4(sums[4], sums[5], sums[6], sums[7]);
     }
     __syncthreads();
-    float r4[4];
+    float erased[4] = {}, seen[4] = {}, r4[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float4 a4 = *reinterpret_cast<const float4*>(&part[w][0][c4]), b4 = *reinterpret_cast<const float4*>(&part[w][1][c4]);
+      erased[0] += a4.x; erased[1] += a4.y; erased[2] += a4.z; erased[3] += a4.w;
+      seen[0] += b4.x; seen[1] += b4.y; seen[2] += b4.z; seen[3] += b4.w;
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int c = c4 + i;
-      const float erased = (part[0][0][c] + part[1][0][c]) + (part[2][0][c] + part[3][0][c]);
-      const float seen = (part[0][1][c] + part[1][1][c]) + (part[2][1][c] + part[3][1][c]);
-      r4[i] = beta * (to_f32(value[i]) * to_f32(write[i]) - erased);
-      if (tid < 8 && v0 + c < a.V) o[v0 + c] = from_f32<T>(a.scale * fmaf(dot, r4[i], seen));
+      r4[i] = beta * (to_f32(value[i]) * to_f32(write[i]) - erased[i]);
+      if (tid < 8 && v0 + c4 + i < a.V) o[v0 + c4 + i] = from_f32<T>(a.scale * fmaf(dot, r4[i], seen[i]));
     }
+    const F2 r2[2] = {pair(r4[0], r4[1]), pair(r4[2], r4[3])};
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
       const int r = r0 + 16 * i;
-      const float x = sk[r];
-      S[i].x = fmaf(x, r4[0], S[i].x); S[i].y = fmaf(x, r4[1], S[i].y); S[i].z = fmaf(x, r4[2], S[i].z); S[i].w = fmaf(x, r4[3], S[i].w);
-      store_state<WIDE>(state + (long long)r * a.V + v0 + c4, S[i], r < a.K ? a.V - v0 - c4 : 0);
+      const F2 kr = both(sk[r]);
+      const float2 a2 = halves(fma2(kr, r2[0], x[i][0])), b2 = halves(fma2(kr, r2[1], x[i][1]));
+      store_state<WIDE>(state + (long long)r * a.V + v0 + c4, make_float4(a2.x, a2.y, b2.x, b2.y), r < a.K ? a.V - v0 - c4 : 0);
     }
   } else {
     const float4 d = *reinterpret_cast<const float4*>(sdecay + c4), x = *reinterpret_cast<const float4*>(serase + c4),
