@@ -30,6 +30,13 @@ constexpr int TILE = 32;  // segments hold a multiple of so many tokens
 constexpr int CK = 16;    // tokens between checkpoints
 constexpr float LN2 = 0.6931471805599453f;
 
+// exp(dt A) from dt and A log2 e.  The exponential instruction gives results that are 2 to 3 parts in 10^8 too small on average for
+// arguments between -1 and -0.005, and a state that lives for hundreds of tokens would gather that up: 2.0e-6 of dA for 4096
+// tokens.  2.8e-8 on the argument, in the multiply-add that forms it, leaves 1e-8 either way (a step of zero still gives 1).
+constexpr float EX2_LOW = 2.8e-8f;
+__device__ __forceinline__ float decay_of(float d, float A2) { return ex2(fmaf(d, A2, EX2_LOW)); }
+__device__ __forceinline__ F2 decay_of(F2 d, F2 A2) { return ex2_2(fma2(d, A2, both(EX2_LOW))); }
+
 // N <= L S states of a channel: S to a thread, L neighbouring threads.  NS threads run the recurrence of CH channels in tiles of
 // TT tokens, NH threads do what stands around it.
 template <int L_, int S_, int NS_, int NH_, int TT_>
@@ -83,9 +90,12 @@ struct Sequence {
 template <int S>
 __device__ __forceinline__ void load_states(float (&x)[S], const float* p, int n0, int N, bool ok, bool wide) {
   if (ok && wide && n0 < N) {
-    if constexpr (S == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + n0);
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    if constexpr (S >= 4) {
+#pragma unroll
+      for (int i = 0; i < S; i += 4) {
+        const float4 v = n0 + i < N ? *reinterpret_cast<const float4*>(p + n0 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+      }
     } else {
       const float2 v = *reinterpret_cast<const float2*>(p + n0);
       x[0] = v.x; x[1] = v.y;
@@ -100,8 +110,11 @@ __device__ __forceinline__ void store_states(float* p, const float (&x)[S], int 
   if (!ok) return;
   if (wide) {
     if (n0 >= N) return;
-    if constexpr (S == 4) *reinterpret_cast<float4*>(p + n0) = make_float4(x[0], x[1], x[2], x[3]);
-    else *reinterpret_cast<float2*>(p + n0) = make_float2(x[0], x[1]);
+    if constexpr (S >= 4) {
+#pragma unroll
+      for (int i = 0; i < S; i += 4)
+        if (n0 + i < N) *reinterpret_cast<float4*>(p + n0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    } else *reinterpret_cast<float2*>(p + n0) = make_float2(x[0], x[1]);
     return;
   }
 #pragma unroll
@@ -129,9 +142,12 @@ __device__ __forceinline__ void store_pairs(float* p, const F2 (&x)[P], int n0, 
 // P pairs from shared memory
 template <int P>
 __device__ __forceinline__ void shared_pairs(F2 (&x)[P], const float* p) {
-  if constexpr (P == 2) {
-    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
-    x[0].v = v.x; x[1].v = v.y;
+  if constexpr (P >= 2) {
+#pragma unroll
+    for (int i = 0; i < P; i += 2) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p + 2 * i);
+      x[i].v = v.x; x[i + 1].v = v.y;
+    }
   } else {
     x[0].v = *reinterpret_cast<const unsigned long long*>(p);
   }
@@ -461,7 +477,7 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_fwd_kernel(const __grid_co
           else total += dj;
 #pragma unroll
           for (int i = 0; i < P; i++) {
-            dec[j][i] = ex2_2(mul2(d, A2p[i]));
+            dec[j][i] = decay_of(d, A2p[i]);
             in[j][i] = mul2(w, Bv[i]);
           }
         }
@@ -607,13 +623,20 @@ __global__ void __launch_bounds__(C::THREADS) scan_bwd_state_kernel(const __grid
   const int ch = threadIdx.x / L, sl = threadIdx.x % L, n0 = sl * S;
   const bool ok = ch < at.valid;
   const long long m = at.m0 + ch;
-  float A2[S], carry[S] = {}, total = 0.f;
+  float A2[S], gh[S] = {}, step[S], total = 0.f;   // as in the main pass
   load_states(A2, a.A + m * a.N, n0, a.N, ok, p.wide_state);
 #pragma unroll
-  for (int i = 0; i < S; i++) A2[i] *= LOG2E;
+  for (int i = 0; i < S; i++) {
+    A2[i] *= LOG2E;
+    step[i] = 1.f;
+  }
   Sequence q;
   q.at(a, at.b, at.t1 - 1);
-  auto last_of = [&](int s) { load_states(carry, a.dfinal_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state); };
+  auto last_of = [&](int s) {
+    load_states(gh, a.dfinal_state + ((long long)s * a.M + m) * a.N, n0, a.N, ok && a.dfinal_state != nullptr, p.wide_state);
+#pragma unroll
+    for (int i = 0; i < S; i++) step[i] = 1.f;
+  };
   if (min(q.next, a.T) <= at.t1) last_of(q.s);
   __syncthreads();
   for (int tile = tiles - 1; tile >= 0; tile--) {
@@ -622,7 +645,10 @@ __global__ void __launch_bounds__(C::THREADS) scan_bwd_state_kernel(const __grid
       const float d = sdt[buf][k * CH + ch], g = sdy[buf][k * CH + ch];
       const float* const c = &sC[buf][k * NP + n0];
 #pragma unroll
-      for (int i = 0; i < S; i++) carry[i] = ex2(d * A2[i]) * fmaf(c[i], g, carry[i]);
+      for (int i = 0; i < S; i++) {
+        gh[i] = fmaf(step[i], gh[i], c[i] * g);
+        step[i] = decay_of(d, A2[i]);
+      }
       total += d;
     };
     if (a.cu_seqlens == nullptr || q.begin < t0 || q.s == 0) {     // (the first sequence begins with the first segment)
@@ -640,8 +666,10 @@ __global__ void __launch_bounds__(C::THREADS) scan_bwd_state_kernel(const __grid
     }
     __syncthreads();
   }
+#pragma unroll
+  for (int i = 0; i < S; i++) gh[i] *= step[i];
   const long long row = ((long long)at.b * p.segments + at.seg) * a.M + m;
-  store_states(p.seg_state + row * a.N, carry, n0, a.N, ok, p.wide_state);
+  store_states(p.seg_state + row * a.N, gh, n0, a.N, ok, p.wide_state);
   if (ok && sl == 0) p.seg_dt[row] = total;
 }
 
@@ -836,11 +864,14 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_co
 #pragma unroll
   for (int i = 0; i < S; i++) A2[i] *= LOG2E;
   join_backward(carry4, p, at, m, A2, n0, ok);
-  F2 A2p[P], carry[P], dA[P], dA_lost[P];
+  // gh of the token behind and its decay, whose product flows to this one: kept apart, so that the chain over the tokens rounds
+  // once per token, in one multiply-add
+  F2 A2p[P], gh[P], step[P], dA[P], dA_lost[P];
 #pragma unroll
   for (int i = 0; i < P; i++) {
     A2p[i] = pair(A2[2 * i], A2[2 * i + 1]);
-    carry[i] = pair(carry4[2 * i], carry4[2 * i + 1]);
+    gh[i] = pair(carry4[2 * i], carry4[2 * i + 1]);
+    step[i] = both(1.f);
     dA[i] = dA_lost[i] = both(0.f);
   }
   const int place = sum_place<C>(lane, n0);
@@ -849,9 +880,16 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_co
   };
   // The gradient that leaves a sequence's first token is its initial state's; the token before belongs to another one.
   auto leave = [&](int s) {
-    if (a.dinitial_state != nullptr) store_pairs(a.dinitial_state + ((long long)s * a.M + m) * a.N, carry, n0, a.N, ok, p.wide_state);
+    if (a.dinitial_state != nullptr) {
+      F2 out[P];
+#pragma unroll
+      for (int i = 0; i < P; i++) out[i] = mul2(step[i], gh[i]);
+      store_pairs(a.dinitial_state + ((long long)s * a.M + m) * a.N, out, n0, a.N, ok, p.wide_state);
+    }
     const bool has = a.dfinal_state != nullptr && a.cu_seqlens != nullptr && s > 0;
-    load_pairs(carry, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
+    load_pairs(gh, a.dfinal_state + (has ? ((long long)(s - 1) * a.M + m) * a.N : 0), n0, a.N, ok && has, p.wide_state);
+#pragma unroll
+    for (int i = 0; i < P; i++) step[i] = both(1.f);
   };
   const float* const kept = a.checkpoints + ((long long)at.b * ((a.T + CK - 1) / CK) * a.M + m) * a.N;
   F2 next[P];   // the state before the 16 tokens that come next
@@ -903,7 +941,7 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_co
           F2 Bv[P];
           shared_pairs(Bv, sB + (k0 + j) * NP);
 #pragma unroll
-          for (int i = 0; i < P; i++) h[j][i] = x[i] = fma2(ex2_2(mul2(d, A2p[i])), x[i], mul2(w, Bv[i]));
+          for (int i = 0; i < P; i++) h[j][i] = x[i] = fma2(decay_of(d, A2p[i]), x[i], mul2(w, Bv[i]));
         }
 #pragma unroll
         for (int j4 = CK - 4; j4 >= 0; j4 -= 4) {
@@ -923,14 +961,14 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_co
             F2 dr, de, yy;
 #pragma unroll
             for (int i = 0; i < P; i++) {
-              const F2 gh = fma2(Cv[i], g, carry[i]);
-              carry[i] = mul2(ex2_2(mul2(d, A2p[i])), gh);
-              const F2 qv = mul2(carry[i], old[i]);
-              dr = i ? fma2(gh, Bv[i], dr) : mul2(gh, Bv[i]);
+              gh[i] = fma2(step[i], gh[i], mul2(Cv[i], g));
+              step[i] = decay_of(d, A2p[i]);
+              const F2 qv = mul2(mul2(step[i], gh[i]), old[i]);
+              dr = i ? fma2(gh[i], Bv[i], dr) : mul2(gh[i], Bv[i]);
               de = i ? fma2(qv, A2p[i], de) : mul2(qv, A2p[i]);
               yy = i ? fma2(Cv[i], h[j][i], yy) : mul2(Cv[i], h[j][i]);
               local[i] = fma2(qv, d, local[i]);
-              const float2 vb = halves(mul2(gh, w)), vc = halves(mul2(g, h[j][i]));
+              const float2 vb = halves(mul2(gh[i], w)), vc = halves(mul2(g, h[j][i]));
               v[jj & 1][2 * i] = vb.x; v[jj & 1][2 * i + 1] = vb.y; v[jj & 1][S + 2 * i] = vc.x; v[jj & 1][S + 2 * i + 1] = vc.y;
             }
             sums[0][jj] = sum_halves(dr); sums[1][jj] = sum_halves(de); sums[2][jj] = sum_halves(yy);
@@ -959,17 +997,24 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_co
   store_pairs(part + m * a.N, dA, n0, a.N, ok, false);
 }
 
-// dB, dC [B*T][G][N] from the CTAs' sums [blocks][B*T][G][2][N]
-template <class T>
+// dB, dC [B*T][G][N] from the CTAs' sums [blocks][B*T][G][2][N], E neighbouring states per thread
+template <class T, int E>
 __global__ void __launch_bounds__(256) scan_sum_bc_kernel(const float* __restrict__ part, int blocks, long long rows, int N, T* __restrict__ dB, T* __restrict__ dC) {
-  const long long n = rows * 2 * N, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long n = rows * 2 * N, i = ((long long)blockIdx.x * 256 + threadIdx.x) * E;
   if (i >= n) return;
-  float sum = 0.f;
+  float sum[E] = {};
 #pragma unroll 8
-  for (int k = 0; k < blocks; k++) sum += part[k * n + i];
+  for (int k = 0; k < blocks; k++) {
+    Pack<float, E> x;
+    load_pack<float, E>(x, part + k * n + i);
+#pragma unroll
+    for (int e = 0; e < E; e++) sum[e] += x.v[e];
+  }
   const long long row = i / (2 * N);
-  const int v = (int)(i % (2 * N));
-  (v < N ? dB + row * N + v : dC + row * N + v - N)[0] = from_f32<T>(sum);
+  const int v = (int)(i - row * 2 * N);
+  T* to = v < N ? dB + row * N + v : dC + row * N + v - N;
+#pragma unroll
+  for (int e = 0; e < E; e++) to[e] = from_f32<T>(sum[e]);
 }
 // dA [M,N], dD and ddt_bias [M] from the sums [parts][M N + 2 M]
 __global__ void __launch_bounds__(256) scan_sum_m_kernel(const float* __restrict__ part, int parts, long long MN, int M, float* dA, float* dD, float* dbias) {
@@ -1020,7 +1065,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ 
     out[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < S; k++) {
-      h[i][k] = fmaf(ex2(d[i] * (A2[i][k] * LOG2E)), h[i][k], d[i] * u[i] * to_f32(Bv[i].v[k]));
+      h[i][k] = fmaf(decay_of(d[i], A2[i][k] * LOG2E), h[i][k], d[i] * u[i] * to_f32(Bv[i].v[k]));
       out[i] = fmaf(to_f32(Cv[i].v[k]), h[i][k], out[i]);
     }
     store_states(a.state + (slot * a.M + first + i * CH) * a.N, h[i], n0, a.N, first + i * CH < a.M, wide);
@@ -1046,6 +1091,12 @@ void with_shape(int N, F&& f) {
   else if (N <= 16) f(Shape<4, 4, 128, 128, 32>());
   else if (N <= 32) f(Shape<8, 4, 128, 128, 32>());
   else f(Shape<16, 4, 128, 128, 32>());
+}
+// The forward keeps no 16 tokens of states in registers: more of them to a thread
+template <class F>
+void with_forward_shape(int N, F&& f) {
+  if (N > 8 && N <= 16) f(Shape<2, 8, 64, 128, 32>());
+  else with_shape(N, f);
 }
 int channels_of(int N) { return N <= 16 ? 32 : N <= 32 ? 16 : 8; }   // per CTA, as above
 template <class F>
@@ -1152,7 +1203,7 @@ extern "C" int rewy_scan_fwd(const RewyScanArgs* a, rewy_stream_t st) {
   const cudaStream_t s = (cudaStream_t)st;
   cudaError_t e = cudaSuccess;
   with_type(a->dtype, [&](auto t) {
-    with_shape(a->N, [&](auto c) {
+    with_forward_shape(a->N, [&](auto c) {
       using T = decltype(t);
       using C = decltype(c);
       constexpr int bytes = sizeof(FwdShared<C>);
@@ -1188,7 +1239,11 @@ extern "C" int rewy_scan_bwd(const RewyScanArgs* a, rewy_stream_t st) {
     });
     if (e != cudaSuccess) return;
     const long long rows = (long long)a->B * a->T * a->G;
-    scan_sum_bc_kernel<T><<<(unsigned)((rows * 2 * a->N + 255) / 256), 256, 0, s>>>(p.part_bc, plan.blocks, rows, a->N, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
+    const long long n = rows * 2 * a->N;
+    if (a->N % 4 == 0 && !unaligned16(p.part_bc))
+      scan_sum_bc_kernel<T, 4><<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(p.part_bc, plan.blocks, rows, a->N, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
+    else
+      scan_sum_bc_kernel<T, 1><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p.part_bc, plan.blocks, rows, a->N, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
   });
   if (e != cudaSuccess) return report_error(REWY_ERR_LAUNCH, cudaGetErrorString(e));
   const long long MN = (long long)a->M * a->N;

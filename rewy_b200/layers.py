@@ -24,21 +24,29 @@ from . import _capi
 from .runtime import record
 
 
-def _op(name):
-    _capi.load_torch()
-    return getattr(torch.ops.rewy_b200, name).default
+def _operator(op, kind=None):
+    """The torch operator ``op``, loaded with its first call; calls count as ``kind``."""
+    fn, kind = None, kind or op
+
+    def call(*args):
+        nonlocal fn
+        if fn is None:
+            _capi.load_torch()
+            fn = getattr(torch.ops.rewy_b200, op).default
+        out = fn(*args)
+        record(kind, "optimized_forward")
+        return out
+
+    return call
 
 
-_ops = {}
-
-
-def _call(op, kind, *args):
-    fn = _ops.get(op)
-    if fn is None:
-        fn = _ops[op] = _op(op)
-    out = fn(*args)
-    record(kind, "optimized_forward")
-    return out
+_causal_conv = _operator("causal_conv")
+_causal_conv_step = _operator("causal_conv_step")
+_selective_scan = _operator("selective_scan")
+_selective_scan_step = _operator("selective_scan_step")
+_gated_rms_norm = _operator("gated_rms_norm")
+_residual_rms_norm = _operator("residual_rms_norm")
+_delta_step = {name: _operator("delta_step", name) for name in ("step_kda", "step_gated_delta_rule", "step_gdn2", "step_delta_rule")}
 
 
 def _silu(op, activation):
@@ -53,14 +61,14 @@ def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, ou
     """Causal convolution per channel: y_t = act(bias + sum_w weight[:, w] x_(t-W+1+w)).  x [B,T,D]; weight [D,W] (or
     [D,1,W]) with 2 <= W <= 4; bias [D]; activation None or "silu".  ``initial_state`` [B,W-1,D] (packed: [sequences,W-1,D]) in the
     type of x holds the inputs before each sequence, the oldest first (default zeros).  Returns (y, final_state or None)."""
-    return _call("causal_conv", "causal_conv", x, weight, bias, _silu("causal_conv", activation), initial_state, output_final_state,
+    return _causal_conv(x, weight, bias, _silu("causal_conv", activation), initial_state, output_final_state,
                  cu_seqlens, cu_seqlens_cpu)
 
 
 @torch.compiler.disable
 def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None):
     """One token of ``causal_conv`` per row: x [B,D], state [pool,W-1,D] updated in place.  Returns y [B,D]."""
-    return _call("causal_conv_step", "causal_conv_step", x, state, weight, bias, _silu("causal_conv_step", activation), slots)
+    return _causal_conv_step(x, state, weight, bias, _silu("causal_conv_step", activation), slots)
 
 
 @torch.compiler.disable
@@ -72,7 +80,7 @@ def selective_scan(u, dt, A, B, C, D=None, *, z=None, dt_bias=None, dt_softplus=
 
     u, dt, z [B,T,M]; A [M,N]; B, C [B,T,G,N] or [B,T,N] (channel m reads group m // (M // G)); D, dt_bias [M]; N up to 64;
     ``initial_state`` [B,M,N] (packed: [sequences,M,N]).  Returns (y, final_state or None)."""
-    return _call("selective_scan", "selective_scan", u, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state,
+    return _selective_scan(u, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state,
                  cu_seqlens, cu_seqlens_cpu)
 
 
@@ -80,7 +88,7 @@ def selective_scan(u, dt, A, B, C, D=None, *, z=None, dt_bias=None, dt_softplus=
 def selective_scan_step(u, dt, A, B, C, state, D=None, *, z=None, dt_bias=None, dt_softplus=False, slots=None):
     """One token of ``selective_scan`` per row: u, dt, z [B,M], B, C [B,G,N] or [B,N], state [pool,M,N] updated in place.
     Returns y [B,M]."""
-    return _call("selective_scan_step", "selective_scan_step", u, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots)
+    return _selective_scan_step(u, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots)
 
 
 @torch.compiler.disable
@@ -89,7 +97,7 @@ def gated_rms_norm(x, gate, weight, *, eps=1e-6, activation="silu", gate_first=F
     n(v) = v / sqrt(mean(v^2) + eps).  x, gate [..., D]; weight [D]; activation "silu" or "sigmoid"."""
     if activation not in ("silu", "swish", "sigmoid"):
         raise ValueError(f"rewy_b200 gated_rms_norm: activation must be 'silu' or 'sigmoid', got {activation!r}")
-    return _call("gated_rms_norm", "gated_rms_norm", x, gate, weight, eps, int(activation == "sigmoid"), gate_first)
+    return _gated_rms_norm(x, gate, weight, eps, int(activation == "sigmoid"), gate_first)
 
 
 @torch.compiler.disable
@@ -99,12 +107,12 @@ def residual_rms_norm(x, residual, weight, *, scale=None, eps=1e-6):
     is that of the sum before it is rounded to the residual's type.  Returns (y, residual_out)."""
     vector = scale if isinstance(scale, torch.Tensor) else None
     number = 1.0 if scale is None or vector is not None else float(scale)
-    return _call("residual_rms_norm", "residual_rms_norm", x, residual, weight, vector, number, eps)
+    return _residual_rms_norm(x, residual, weight, vector, number, eps)
 
 
 def _step(name, family, q, k, v, state, *, g=None, beta=None, b=None, w=None, scale=None, slots=None, qk_norm=False, beta_scale=0.0,
           A_log=None, dt_bias=None, state_v_first=False):
-    return _call("delta_step", name, _capi.FAMILY_ID[family], q, k, v, g, beta, b, w, state, scale, slots, qk_norm, beta_scale,
+    return _delta_step[name](_capi.FAMILY_ID[family], q, k, v, g, beta, b, w, state, scale, slots, qk_norm, beta_scale,
                  A_log, dt_bias, state_v_first)
 
 
