@@ -606,3 +606,52 @@ def test_steps_refuse_gradients_and_count_as_writes():
     with torch.no_grad():
         rewy_b200.causal_conv_step(x, state, weight)
     assert state._version > version
+
+
+# ---- long tensors and the kernels behind the calls -------------------------------------------------------------------
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in a tensor: its last rows give what they give alone."""
+    gen = torch.Generator(device=DEV).manual_seed(26)
+    rn = lambda *s, t=BF16: torch.empty(*s, device=DEV, dtype=t).normal_(generator=gen)  # noqa: E731
+    D, tail = 4096, 9
+    rows = (1 << 31) // D + 100
+    x, weight = rn(1, rows, D), rn(D, 4, t=FP32) / 2
+    y, fin = rewy_b200.causal_conv(x, weight, activation="silu", output_final_state=True)
+    alone, _ = rewy_b200.causal_conv(x[:, -tail:], weight, activation="silu", initial_state=x[:, -tail - 3:-tail].contiguous())
+    assert torch.equal(y[:, -tail:], alone) and torch.equal(fin, x[:, -3:])
+    del y
+    norm = rn(D, t=FP32)
+    whole = rewy_b200.gated_rms_norm(x, x, norm)
+    assert torch.equal(whole[:, -tail:], rewy_b200.gated_rms_norm(x[:, -tail:], x[:, -tail:], norm))
+    del whole
+    y, r = rewy_b200.residual_rms_norm(x, x, norm, scale=0.5)
+    for a, b in zip((y, r), rewy_b200.residual_rms_norm(x[:, -tail:], x[:, -tail:], norm, scale=0.5)):
+        assert torch.equal(a[:, -tail:], b)
+    del y, r
+    M = 256                                                    # the scan: as many tokens as make 2^31 elements of u
+    u = x.view(1, -1, M)
+    A, Bm = -torch.rand(M, 16, device=DEV) - 0.5, rn(1, u.shape[1], 16)
+    y, _ = rewy_b200.selective_scan(u, u, A, Bm, Bm, dt_softplus=True)
+    short, _ = rewy_b200.selective_scan(u[:, -2000:], u[:, -2000:], A, Bm[:, -2000:], Bm[:, -2000:], dt_softplus=True)
+    _close(y[:, -1000:], short[:, -1000:].float(), "scan")     # 1000 tokens of steps around 0.7 forget where they began
+    del x, u, y
+    pool, one = (1 << 31) // (M * 16) + 3, torch.tensor([-1], device=DEV, dtype=torch.int32)
+    state = torch.zeros(pool, M, 16, device=DEV)
+    state[-1] = 1.0
+    v, b = rn(1, M), rn(1, 16)
+    first, last = (rewy_b200.selective_scan_step(v, v.abs(), A, b, b, s, slots=one + i) for s, i in ((state, pool), (state[-1:].clone(), 1)))
+    assert torch.equal(first, last) and not torch.equal(state[-1], torch.ones_like(state[-1])) and not state[0].any()
+
+
+def test_kernels_are_launched_and_calls_counted():
+    from rewy_b200 import _capi
+    rn = _gen(27)
+    rewy_b200.stats(reset=True)
+    before = _capi.launch_count()
+    x, w = rn(4, 64), rn(64)
+    rewy_b200.gated_rms_norm(x, x, w)
+    rewy_b200.residual_rms_norm(x, None, w)
+    rewy_b200.causal_conv(x[None], rn(64, 4))
+    assert _capi.launch_count() == before + 3
+    assert rewy_b200.stats(reset=True) == {f"{n}.optimized_forward": 1 for n in ("causal_conv", "gated_rms_norm", "residual_rms_norm")}
