@@ -7,6 +7,8 @@
 // waited for), so that even one sequence with few heads fills the SMs.  The state stays in registers between load and store.
 // Both products over the key channels come from one exchange: q^T (S + k r^T) = q^T S + (q k) r.  q, k and the gates are
 // read, normalised and activated by every CTA for itself.  All arithmetic is FP32.
+// Measured, KDA, 64 sequences of 32 heads of 128 x 128, everything fused: 53 us (5.2 TB/s; the same loads and stores alone take 45);
+// one sequence of 16 value heads 4 us.  Before: gates and targets asked for when they were used, single FP32 values, 73 us.
 #include "layer.cuh"
 
 namespace rewy {

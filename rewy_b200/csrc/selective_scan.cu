@@ -6,20 +6,28 @@
 //
 // Everything is FP32 between the element types at both ends; nothing is kept in fewer bits in between.
 //
-// A thread holds four states of one channel, L neighbouring lanes the states of a channel (N <= 4 L), a CTA of 128 threads
-// 128 / L channels, which it takes through a segment of the tokens in tiles of 32: the tile's dt and dt u per channel and its B
-// and C are put into shared memory as FP32 once, with the softplus, by a pass that reads 8 elements per thread.  What bounds
-// the forward is one exponential per (token, channel, state) at 16 per clock and SM; the rest is 27 issue slots per token
-// and warp beside the 32 cycles that its four exponentials take.
+// Recurrence.  A thread holds S states of one channel, L neighbouring lanes the states of a channel (N <= L S), a group of warps 8
+// to 32 channels, which it takes through a segment of the tokens in tiles of 32.  A second group of four warps works beside it:
+// it puts the next tile's dt and dt u per channel, its B and its C into shared memory as FP32 (softplus and gate once per
+// element, eight elements per thread, loads asked for a tile ahead), and writes what came of the tile before.  One barrier per tile.
+// Arithmetic on two states at a time (FP32 pairs).
 // The backward needs h_(t-1) in reverse: the forward leaves the state before every 16th token (4 N / 16 bytes per token and
-// channel), from which 16 tokens are run forward into registers (h and a, one exponential each) and walked back.
-// Sums over the states of a channel are exchanged for four tokens at a time (three shuffles for four lanes and four sums);
-// those over channels (dB, dC) leave each warp scattered over its lanes (seven shuffles for eight values and eight lanes), are
-// added over the CTA's warps in shared memory and over the CTAs by a second kernel, in one order: results repeat bit for bit.
+// channel), from which 16 tokens are run forward into registers and walked back.
+// Sums over the states of a channel are exchanged for several sets of four values step by step together, those over channels
+// (dB, dC) for two tokens; the latter end scattered over the lanes, are added over the CTA's warps in shared memory and over the
+// CTAs by a second kernel, all in one order: results repeat bit for bit.
 //
 // Few channels: the token axis is cut into segments.  A first pass finds each segment's end state from a zero start (backward:
 // the gradient that leaves its first token), and the main pass starts every segment from those before it, joined by
 // h <- exp(A sum dt) h + end.  That doubles the exponentials and pays only where most SMs would idle.
+//
+// Measured, B=2 T=4096 M=4096 N=16 in BF16 with softplus, skip and gate: forward 295 us (the exponentials alone, 16 per clock and
+// SM, take 117, memory 41), backward 1020 us and 47 for the sums of dB and dC (memory 62 and 41).  Both are bound by latency and
+// issue together: 256 CTAs give an SM's schedulers two warps of recurrence each, issue is 50 % active, and what a warp waits for
+// are its own shuffles, exponentials and multiply-adds.  Before: every warp doing everything in turn, 456 and 1875 us; conditions
+// inside the element loops, 340 and 1052.  Tried and not kept (backward): two states per thread and twice the warps 1758 us; eight
+// tokens in registers, half the code, 1031; registers moved from the second group to the first by setmaxnreg 1010; 64 channels
+// per CTA 994 with its sums, but half the CTAs for narrow layers.
 #include <climits>
 #include "layer.cuh"
 
@@ -460,7 +468,7 @@ __global__ void __launch_bounds__(C::THREADS, 2) scan_fwd_kernel(const __grid_co
     float* __restrict__ const sy = sm.y[buf] + ch;
     // Eight tokens; check: a sequence may begin inside the tile
     auto tokens = [&](auto check, int k) {
-      float y[2][4];
+      [[maybe_unused]] float y[2][4];
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int kh = k + 4 * half;

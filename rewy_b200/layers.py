@@ -132,12 +132,13 @@ def _need(name, **tensors):
 def step_kda(q, k, v, g, beta, state, *, scale=None, slots=None, use_qk_l2norm_in_kernel=False, use_gate_in_kernel=False,
              use_beta_sigmoid_in_kernel=False, allow_neg_eigval=False, A_log=None, dt_bias=None, state_v_first=False):
     """One token of ``chunk_kda`` per row.  q, k [B,H,K]; v [B,HV,V]; g [B,HV,K] natural-log decay, or the raw gate input with
-    ``use_gate_in_kernel`` (then ``A_log`` [HV] and optionally ``dt_bias`` [HV*K]); beta [B,HV]; state [pool,HV,K,V] FP32 ([pool,HV,V,K]
+    ``use_gate_in_kernel`` (then ``A_log`` with HV values and optionally ``dt_bias`` with HV*K); beta [B,HV]; state [pool,HV,K,V] FP32 ([pool,HV,V,K]
     with ``state_v_first``) updated in place; HV a multiple of H, K and V up to 128.  Returns o [B,HV,V]."""
     _need("step_kda", g=g, beta=beta)
     if use_gate_in_kernel and A_log is None:
         raise ValueError("A_log must be provided when use_gate_in_kernel=True.")
-    gate = dict(A_log=A_log, dt_bias=dt_bias) if use_gate_in_kernel else {}
+    flat = lambda t: None if t is None else t.float().reshape(-1)  # noqa: E731  (as the chunked operator takes them)
+    gate = dict(A_log=flat(A_log), dt_bias=flat(dt_bias)) if use_gate_in_kernel else {}
     return _step("step_kda", "kda", q, k, v, state, g=g, beta=beta, scale=scale, slots=slots, qk_norm=use_qk_l2norm_in_kernel,
                  beta_scale=_beta_scale(use_beta_sigmoid_in_kernel, allow_neg_eigval), state_v_first=state_v_first, **gate)
 

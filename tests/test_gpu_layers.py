@@ -345,7 +345,7 @@ def test_delta_steps(dtype, family, v_first, B, H, groups, K, V, options):
     if family == "gdn":
         xs["g"] = -rn(B, HV).abs()
     elif family == "kda" and options:
-        xs.update(g=rn(B, HV, K).to(dtype), A_log=rn(HV), dt_bias=rn(HV * K))
+        xs.update(g=rn(B, HV, K).to(dtype), A_log=rn(HV), dt_bias=rn(HV, K))
         kw["use_gate_in_kernel"] = True
     elif family != "delta":
         xs["g"] = -0.2 * rn(B, HV, K).abs()
