@@ -27,7 +27,8 @@
 // are its own shuffles, exponentials and multiply-adds.  Before: every warp doing everything in turn, 456 and 1875 us; conditions
 // inside the element loops, 340 and 1052.  Tried and not kept (backward): two states per thread and twice the warps 1758 us; eight
 // tokens in registers, half the code, 1031; registers moved from the second group to the first by setmaxnreg 1010; 64 channels
-// per CTA 994 with its sums, but half the CTAs for narrow layers.
+// per CTA 994 with its sums, but half the CTAs for narrow layers; two warps in the second group 1131.  (Forward): tiles ahead by
+// asynchronous copies through shared memory 303; two warps in the second group 562.
 #include <climits>
 #include "layer.cuh"
 
