@@ -1,7 +1,8 @@
 // Torch operators of the kernels around a recurrence: arguments checked, outputs allocated, the C ABI called, and the autograd
 // nodes of those that train.  Each operator is one function for every backend key: it refuses what it does not take, tensors on
 // the CPU last, so that its checks run anywhere.  Launches go to torch's current stream of the tensors' device, on which
-// outputs and workspaces are allocated.  Gradients are first order: differentiating them again raises.
+// outputs and workspaces are allocated.  Gradients are first order and reverse mode: differentiating them again raises, and so does an
+// operand or incoming gradient with a forward-mode derivative.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -56,8 +57,14 @@ void want_shape(const char* op, const char* name, const OptTensor& t, at::IntArr
 void want_type(const char* op, const char* name, const OptTensor& t, at::ScalarType type) {
   WANT(!has(t) || t->scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t->scalar_type());
 }
+// no derivative that travels with the values: the kernels would drop it
+template <class Tensors>
+void want_no_tangent(const char* op, const Tensors& tensors) {
+  for (const OptTensor& t : tensors) WANT(!has(t) || !t->_fw_grad(0).defined(), op, ": has no forward-mode derivative, and an input carries one");
+}
 // one CUDA device for all of them
 void want_cuda(const char* op, std::initializer_list<OptTensor> tensors) {
+  want_no_tangent(op, tensors);
   c10::Device device(c10::kCPU);
   for (const auto& t : tensors) {
     if (!has(t)) continue;
@@ -175,6 +182,7 @@ struct Conv : torch::autograd::Function<Conv> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    want_no_tangent("causal_conv backward", grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor x = rows_of(saved[0]), w = saved[1].contiguous(), b = dense(saved[2]), initial = dense(saved[3]), &cu = saved[4];
     const c10::cuda::CUDAGuard guard(x.device());
@@ -299,6 +307,7 @@ struct Scan : torch::autograd::Function<Scan> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    want_no_tangent("selective_scan backward", grads);
     const auto v = ctx->get_saved_variables();
     const ScanInputs s = scan_inputs(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], ctx->saved_data["softplus"].toBool());
     const c10::cuda::CUDAGuard guard(s.u.device());
@@ -471,6 +480,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     return gated_forward(xr, gr, w, eps, act, gate_first);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    want_no_tangent("gated_rms_norm backward", grads);
     const auto v = ctx->get_saved_variables();
     const Tensor x = norm_rows(v[0]), gate = norm_rows(v[1]), w = v[2].contiguous(), dy = grad_or_zeros(grads[0], x.sizes(), x.options());
     const c10::cuda::CUDAGuard guard(x.device());
@@ -523,6 +533,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     return {y, out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    want_no_tangent("residual_rms_norm backward", grads);
     const auto v = ctx->get_saved_variables();
     const Tensor x = norm_rows(v[0]), residual = norm_rows(v[1]), w = v[2].contiguous(), s = dense(v[3]);
     const c10::cuda::CUDAGuard guard(x.device());
