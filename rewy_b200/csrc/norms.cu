@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
       }
       row_sums<TPR>(sum, red, parity);
       if (!real) return;
-      const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), back = rs * rs * rs * (sum[1] * p.inv_D);
+      const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), mean = rs * (sum[1] * p.inv_D);   // of dn n: as large as dn however small the row
 #pragma unroll
       for (int v = 0; v < NV; v++) {
         const int c = Y::column(v);
@@ -339,11 +339,17 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<T, TPR, NV,
 #pragma unroll
         for (int e = 0; e < E; e++) {
           const float act = act_of<silu.value, true>(g[e], slope), xv = x[e], dn = d[e] * wv[e];
-          // gate first: v = x act, dx = dv act, dgate = dv x act'.  Else dgate = dn n act', dx = r dn act - back x
-          const float dv = gate_first.value ? fmaf(rs, dn, -back * (xv * act)) : rs * dn;
-          x[e] = gate_first.value ? dv * act : fmaf(dv, act, -back * xv);
-          g[e] = dv * xv * slope;
-          dw[v][e] = fmaf(d[e], xv * act * rs, dw[v][e]);
+          // gate first: v = x act, dx = dv act, dgate = dv x act'.  Else dgate = dn n act', dx = r (dn act - n mean)
+          const float n = (gate_first.value ? xv * act : xv) * rs;
+          if constexpr (gate_first.value) {
+            const float dv = rs * fmaf(-mean, n, dn);
+            x[e] = dv * act;
+            g[e] = dv * xv * slope;
+          } else {
+            x[e] = rs * fmaf(-mean, n, dn * act);
+            g[e] = dn * n * slope;
+          }
+          dw[v][e] = fmaf(d[e], gate_first.value ? n : n * act, dw[v][e]);
         }
         Pack<T, E> ox, og;
         from_floats(ox, x);
@@ -457,7 +463,7 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
     }
     row_sums<TPR>(sum, red, parity);
     if (!real) return;
-    const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), back = rs * rs * rs * (sum[1] * p.inv_D);
+    const float rs = rsqrtf(fmaf(sum[0], p.inv_D, a.eps)), mean = rs * (sum[1] * p.inv_D);   // of dn n: as large as dn however small the row
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = Y::column(v);
@@ -473,11 +479,11 @@ __global__ void __launch_bounds__(Layout<TPR, NV>::THREADS, resident<TR, TPR, NV
       Pack<TR, E> orr;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float xv = x[e], t = fmaf(sv[e], xv, res[e]);
-        const float dt = dro[e] + fmaf(rs, d[e] * wv[e], -back * t);
+        const float xv = x[e], n = fmaf(sv[e], xv, res[e]) * rs;
+        const float dt = fmaf(rs, fmaf(-mean, n, d[e] * wv[e]), dro[e]);
         x[e] = sv[e] * dt;
         res[e] = dt;
-        dw[v][e] = fmaf(d[e], t * rs, dw[v][e]);
+        dw[v][e] = fmaf(d[e], n, dw[v][e]);
         if constexpr (SCALE) ds[v][e] = fmaf(xv, dt, ds[v][e]);
       }
       from_floats(ox, x);

@@ -94,7 +94,8 @@ def selective_scan_step(u, dt, A, B, C, state, D=None, *, z=None, dt_bias=None, 
 @torch.compiler.disable
 def gated_rms_norm(x, gate, weight, *, eps=1e-6, activation="silu", gate_first=False):
     """n(x) * weight * act(gate) over the last dimension (up to 16384), or with ``gate_first`` n(x * act(gate)) * weight;
-    n(v) = v / sqrt(mean(v^2) + eps).  x, gate [..., D]; weight [D]; activation "silu" or "sigmoid"."""
+    n(v) = v / sqrt(mean(v^2) + eps), squares in FP32: with eps = 0 rows down to an rms of 1e-18.  x, gate [..., D]; weight [D];
+    activation "silu" or "sigmoid"."""
     if activation not in ("silu", "swish", "sigmoid"):
         raise ValueError(f"rewy_b200 gated_rms_norm: activation must be 'silu' or 'sigmoid', got {activation!r}")
     return _gated_rms_norm(x, gate, weight, eps, int(activation == "sigmoid"), gate_first)

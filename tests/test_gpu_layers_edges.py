@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 import rewy_b200
-from test_gpu_layers import NAMES, _calls, _gen, _leaves
+from test_gpu_layers import BF16, FP32, NAMES, _calls, _compare, _gen, _leaves, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,20 @@ def test_a_forward_mode_derivative_is_refused(name):
             seed = forward_ad.make_dual(torch.ones_like(o), torch.ones_like(o))
             with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
                 torch.autograd.grad(o, list(mine.values()), seed, retain_graph=True, allow_unused=True)
+
+
+@pytest.mark.parametrize("dtype", (BF16, FP32))
+@pytest.mark.parametrize("D", (64, 1000, 9001))
+@pytest.mark.parametrize("size", (1e-12, 1e-14, 1e-18))
+def test_norms_of_very_small_rows_without_eps(dtype, D, size):
+    """eps = 0: r is 1 / size, beyond 10^12, and its cube leaves FP32, but every gradient is finite.  Squares down to 10^-36 are
+    ordinary FP32 numbers, so the tolerance is that of other rows."""
+    rn = _gen(31)
+    x, gate, weight = (size * rn(6, D)).to(dtype), rn(6, D).to(dtype), 1 + 0.2 * rn(D)
+    for gate_first in (False, True):
+        kw = dict(eps=0.0, gate_first=gate_first)
+        _compare(lambda **x: (rewy_b200.gated_rms_norm(**x, **kw),), lambda **x: (oracle.gated_rms_norm(**x, **kw),),
+                 dict(x=x, gate=gate, weight=weight), (dtype,))
+    for scale in (0.5, 0.5 + rn(D)):
+        _compare(lambda **x: rewy_b200.residual_rms_norm(**x, eps=0.0), lambda **x: oracle.residual_rms_norm(**x, eps=0.0),
+                 dict(x=x, residual=(size * rn(6, D)).to(dtype), weight=weight, scale=scale), (dtype, dtype))
