@@ -427,12 +427,15 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ 
     if (j < W - 1) store_some<T, V>(state + (long long)j * a.D, j + 1 < W - 1 ? old[j + 1 < 3 ? j + 1 : 2] : now, valid, wide);
 }
 
+// What 32-bit counts of tokens and channels hold
+bool conv_fits(int B, int T, int D) { return (long long)B * T <= (1LL << 30) && D <= (1 << 24); }
+
 int check_conv(const RewyConvArgs* a) {
   LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
   LAYER_REQUIRE(known_dtype(a->dtype) && known_dtype(a->param_dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
   LAYER_REQUIRE(a->W >= 2 && a->W <= 4, REWY_ERR_UNSUPPORTED, "the convolution takes 2 to 4 taps");
   LAYER_REQUIRE(a->B > 0 && a->T > 0 && a->D > 0, REWY_ERR_SHAPE, "B, T and D must be positive");
-  LAYER_REQUIRE((long long)a->B * a->T <= (1LL << 30) && a->D <= (1 << 24), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or D 2^24 channels");
+  LAYER_REQUIRE(conv_fits(a->B, a->T, a->D), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or D 2^24 channels");
   LAYER_REQUIRE(((long long)a->B * a->T / 64 + a->B) * (a->D / 64 + 1) < (1LL << 31), REWY_ERR_SHAPE, "more tokens and channels than one grid holds");
   LAYER_REQUIRE(a->x != nullptr && a->weight != nullptr, REWY_ERR_NULL, "x or weight is NULL");
   LAYER_REQUIRE(a->cu_seqlens == nullptr || (a->B == 1 && a->num_seqs > 0), REWY_ERR_SHAPE, "packed sequences need B = 1 and num_seqs > 0");
@@ -494,7 +497,7 @@ extern "C" int rewy_conv_fwd(const RewyConvArgs* a, rewy_stream_t st) {
 }
 
 extern "C" size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D, int32_t W) {
-  if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4) return 0;
+  if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4 || !conv_fits(B, T, D)) return 0;
   RewyConvArgs a{};
   a.B = B; a.T = T; a.D = D; a.W = W;
   const ConvParams p = conv_params(a, 4, true);

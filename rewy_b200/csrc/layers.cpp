@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -57,6 +58,16 @@ void want_shape(const char* op, const char* name, const OptTensor& t, at::IntArr
 void want_type(const char* op, const char* name, const OptTensor& t, at::ScalarType type) {
   WANT(!has(t) || t->scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t->scalar_type());
 }
+// What the kernels' 32-bit counts hold (the C entries' limits), asked before a size is narrowed to one
+constexpr int64_t MOST_TOKENS = int64_t(1) << 30, MOST_CHANNELS = int64_t(1) << 24, MOST_ROWS = (int64_t(1) << 31) - 1;
+void want_most(const char* op, const char* what, int64_t n, int64_t most) { WANT(n <= most, op, ": takes up to ", most, " ", what, ", got ", n); }
+void want_tokens(const char* op, const Tensor& x) {   // [B, T, channels]
+  want_most(op, "sequences", x.size(0), MOST_TOKENS);
+  want_most(op, "tokens per sequence", x.size(1), MOST_TOKENS);
+  want_most(op, "tokens", x.size(0) * x.size(1), MOST_TOKENS);
+  want_most(op, "channels", x.size(2), MOST_CHANNELS);
+}
+
 // no derivative that travels with the values: the kernels would drop it
 template <class Tensors>
 void want_no_tangent(const char* op, const Tensors& tensors) {
@@ -214,6 +225,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor& x, const Tensor& weight, co
   WANT(x.dim() == 3, op, ": x must have the shape [B, T, D], got ", shape(x));
   dtype_of(x, op, "x");
   WANT(x.size(0) > 0 && x.size(1) > 0 && x.size(2) > 0, op, ": x must not be empty, got ", shape(x));
+  want_tokens(op, x);
   const Tensor w = conv_weight(op, weight, x.size(2));
   dtype_of(w, op, "weight");
   want_shape(op, "bias", bias, {x.size(2)});
@@ -233,6 +245,8 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor& x, const Tensor& weight, co
 Tensor causal_conv_step(const Tensor& x, Tensor state, const Tensor& weight, const OptTensor& bias, bool silu, const OptTensor& slots) {
   const char* op = "causal_conv_step";
   WANT(x.dim() == 2 && x.numel() > 0, op, ": x must have the shape [B, D], got ", shape(x));
+  want_most(op, "rows", x.size(0), MOST_ROWS);
+  want_most(op, "channels", x.size(1), MOST_CHANNELS);
   const Tensor w = conv_weight(op, weight, x.size(1)).contiguous(), xr = rows_of(x);
   WANT(state.dim() == 3 && state.size(0) > 0 && state.size(1) == w.size(1) - 1 && state.size(2) == x.size(1), op, ": state must have the shape [pool, ",
        w.size(1) - 1, ", ", x.size(1), "], got ", shape(state));
@@ -337,6 +351,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& dt, con
   WANT(u.dim() == 3, op, ": u must have the shape [B, T, M], got ", shape(u));
   dtype_of(u, op, "u");
   WANT(u.numel() > 0, op, ": u must not be empty, got ", shape(u));
+  want_tokens(op, u);
   want_shape(op, "dt", dt, u.sizes());
   want_shape(op, "z", z, u.sizes());
   const int64_t M = u.size(2);
@@ -374,6 +389,8 @@ Tensor selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, c
   const char* op = "selective_scan_step";
   WANT(u.dim() == 2 && u.numel() > 0, op, ": u must have the shape [B, M], got ", shape(u));
   const int64_t R = u.size(0), M = u.size(1);
+  want_most(op, "rows", R, MOST_ROWS);
+  want_most(op, "channels", M, MOST_CHANNELS);
   want_shape(op, "dt", dt, {R, M});
   want_shape(op, "z", z, {R, M});
   WANT(A.dim() == 2 && A.size(0) == M, op, ": A must have the shape [", M, ", N], got ", shape(A));
@@ -579,6 +596,8 @@ Tensor delta_step(int64_t family, const Tensor& q, const Tensor& k, const Tensor
   const char* op = STEP_NAMES[family];
   WANT(q.dim() == 3 && v.dim() == 3 && q.numel() > 0 && v.numel() > 0, op, ": q, k must have the shape [B, H, K] and v [B, HV, V], got ", shape(q), " and ", shape(v));
   const int64_t B = q.size(0), H = q.size(1), K = q.size(2), HV = v.size(1), V = v.size(2);
+  want_most(op, "rows", B, MOST_ROWS);
+  want_most(op, "heads", std::max(H, HV), MOST_ROWS);
   want_shape(op, "k", k, {B, H, K});
   WANT(v.size(0) == B && HV % H == 0, op, ": the value heads (", HV, ") must be a multiple of the query/key heads (", H, ") of the same batch");
   WANT(K <= 128 && V <= 128, op, ": head dimensions above 128 are not supported");

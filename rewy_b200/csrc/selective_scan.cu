@@ -1151,13 +1151,16 @@ Plan make_plan(int B, int T, int M, int N, int G, bool backward) {
   return p;
 }
 
+// What 32-bit counts of tokens and channels hold
+bool scan_fits(int B, int T, int M) { return (long long)B * T <= (1LL << 30) && M <= (1 << 24); }
+
 int check_scan(const RewyScanArgs* a, bool backward, Plan& plan) {
   LAYER_REQUIRE(a != nullptr, REWY_ERR_NULL, "args is NULL");
   LAYER_REQUIRE(known_dtype(a->dtype), REWY_ERR_UNSUPPORTED, "unknown element type");
   LAYER_REQUIRE(a->B > 0 && a->T > 0 && a->M > 0 && a->G > 0, REWY_ERR_SHAPE, "B, T, M and G must be positive");
   LAYER_REQUIRE(a->N >= 1 && a->N <= 64, REWY_ERR_UNSUPPORTED, "the scan takes 1 to 64 states per channel");
   LAYER_REQUIRE(a->M % a->G == 0, REWY_ERR_SHAPE, "the channels must divide into the groups of B and C");
-  LAYER_REQUIRE((long long)a->B * a->T <= (1LL << 30) && a->M <= (1 << 24), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or M 2^24 channels");
+  LAYER_REQUIRE(scan_fits(a->B, a->T, a->M), REWY_ERR_SHAPE, "B*T exceeds 2^30 tokens or M 2^24 channels");
   LAYER_REQUIRE(a->u != nullptr && a->dt != nullptr && a->Bm != nullptr && a->C != nullptr && a->A != nullptr, REWY_ERR_NULL, "u, dt, B, C or A is NULL");
   LAYER_REQUIRE(a->cu_seqlens == nullptr || (a->B == 1 && a->num_seqs > 0), REWY_ERR_SHAPE, "packed sequences need B = 1 and num_seqs > 0");
   plan = make_plan(a->B, a->T, a->M, a->N, a->G, backward);
@@ -1194,12 +1197,12 @@ ScanParams scan_params(const RewyScanArgs& a, const Plan& plan) {
 using namespace rewy;
 
 extern "C" size_t rewy_scan_checkpoint_bytes(int32_t B, int32_t T, int32_t M, int32_t N) {
-  if (B <= 0 || T <= 0 || M <= 0 || N <= 0) return 0;
+  if (B <= 0 || T <= 0 || M <= 0 || N <= 0 || N > 64 || !scan_fits(B, T, M)) return 0;
   return (size_t)B * ((T + CK - 1) / CK) * M * N * sizeof(float);
 }
 
 extern "C" size_t rewy_scan_workspace_bytes(int32_t B, int32_t T, int32_t M, int32_t N, int32_t G, int32_t backward) {
-  if (B <= 0 || T <= 0 || M <= 0 || N <= 0 || N > 64 || G <= 0 || M % G) return 0;
+  if (B <= 0 || T <= 0 || M <= 0 || N <= 0 || N > 64 || G <= 0 || M % G || !scan_fits(B, T, M)) return 0;
   const Plan p = make_plan(B, T, M, N, G, backward != 0);
   return (p.seg_state + p.seg_dt + p.bc + p.m) * sizeof(float);
 }

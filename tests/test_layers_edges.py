@@ -59,3 +59,51 @@ def test_an_operand_with_a_forward_mode_derivative_is_refused(call, kw, name):
 def test_jvp_is_refused(call, kw, name):
     with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
         torch.func.jvp(lambda t: call(**{**kw, name: t}), (kw[name],), (torch.ones_like(kw[name]),))
+
+
+def _wide(*s):
+    """A tensor of these sizes over one element: no memory."""
+    return z(1).expand(*s)
+
+
+BIG, N32 = 1 << 32, torch.int32
+LARGE = [
+    (_conv, dict(x=_wide(1, BIG + 64, 4), weight=z(4, 4)), "up to 1073741824 tokens per sequence, got 4294967360"),
+    (_conv, dict(x=_wide(BIG + 2, 64, 4), weight=z(4, 4)), "up to 1073741824 sequences, got 4294967298"),
+    (_conv, dict(x=_wide(1 << 20, 1 << 11, 4), weight=z(4, 4)), "up to 1073741824 tokens, got 2147483648"),
+    (_conv, dict(x=_wide(1, 9, BIG + 8), weight=_wide(BIG + 8, 4)), "up to 16777216 channels, got 4294967304"),
+    (_scan, dict(u=_wide(1, BIG + 9, 12), dt=_wide(1, BIG + 9, 12), B=_wide(1, BIG + 9, 16), C=_wide(1, BIG + 9, 16)),
+     "up to 1073741824 tokens per sequence, got 4294967305"),
+    (_scan, dict(u=_wide(BIG + 1, 9, 12), dt=_wide(BIG + 1, 9, 12), B=_wide(BIG + 1, 9, 16), C=_wide(BIG + 1, 9, 16)), "up to 1073741824 sequences"),
+    (_scan, dict(u=_wide(1, 9, BIG + 8), dt=_wide(1, 9, BIG + 8), A=_wide(BIG + 8, 16)), "up to 16777216 channels"),
+    (_conv_step, dict(x=_wide(BIG + 1, 1), state=z(5, 3, 1), weight=z(1, 4), slots=z(1, dtype=N32).expand(BIG + 1)), "up to 2147483647 rows, got 4294967297"),
+    (_conv_step, dict(x=_wide(2, BIG + 1), state=_wide(5, 3, BIG + 1), weight=_wide(BIG + 1, 4)), "up to 16777216 channels"),
+    (_scan_step, dict(u=_wide(BIG + 1, 12), dt=_wide(BIG + 1, 12), B=_wide(BIG + 1, 16), C=_wide(BIG + 1, 16), slots=z(1, dtype=N32).expand(BIG + 1)),
+     "up to 2147483647 rows"),
+    (_scan_step, dict(u=_wide(2, BIG + 4), dt=_wide(2, BIG + 4), A=_wide(BIG + 4, 16), state=_wide(5, BIG + 4, 16)), "up to 16777216 channels"),
+    (_kda, dict(q=_wide(BIG + 2, 2, 8), k=_wide(BIG + 2, 2, 8), v=_wide(BIG + 2, 4, 6), g=_wide(BIG + 2, 4, 8), beta=_wide(BIG + 2, 4),
+                slots=z(1, dtype=N32).expand(BIG + 2)), "up to 2147483647 rows"),
+    (_kda, dict(v=_wide(2, BIG + 4, 6), g=_wide(2, BIG + 4, 8), beta=_wide(2, BIG + 4), state=_wide(5, BIG + 4, 8, 6)), "up to 2147483647 heads"),
+    (_kda, dict(q=_wide(2, BIG + 2, 8), k=_wide(2, BIG + 2, 8), v=_wide(2, BIG + 2, 6)), "up to 2147483647 heads"),
+]
+
+
+@pytest.mark.parametrize("call,kw,words", LARGE, ids=[f"{c.__name__[1:]}-{i}" for i, (c, _, _) in enumerate(LARGE)])
+def test_sizes_that_32_bits_do_not_hold_are_refused(call, kw, words):
+    """Narrowed before they were asked, 2^32 + 64 tokens would be 64: the rest of the output would never be written."""
+    with pytest.raises(RuntimeError, match=words):
+        call(**kw)
+
+
+def test_workspaces_of_refused_sizes_are_none():
+    import ctypes
+    from rewy_b200 import _capi
+    lib, most = _capi.load(), (1 << 31) - 1
+    for name in ("rewy_conv_bwd_workspace_bytes", "rewy_scan_checkpoint_bytes", "rewy_scan_workspace_bytes"):
+        getattr(lib, name).restype = ctypes.c_size_t
+    for B, T, D in ((1, most, 64), (most, most, 64), (1, 64, most), (1 << 16, (1 << 14) + 1, 64)):
+        assert lib.rewy_conv_bwd_workspace_bytes(B, T, D, 4) == 0
+        assert lib.rewy_scan_checkpoint_bytes(B, T, D, 16) == 0
+        assert lib.rewy_scan_workspace_bytes(B, T, D, 16, 1, 0) == lib.rewy_scan_workspace_bytes(B, T, D, 16, 1, 1) == 0
+    assert lib.rewy_scan_checkpoint_bytes(1, 64, 64, 65) == 0
+    assert lib.rewy_conv_bwd_workspace_bytes(1 << 16, 1 << 14, 64, 4) > 0 and lib.rewy_scan_workspace_bytes(1 << 16, 1 << 14, 64, 16, 1, 1) > 0
