@@ -593,6 +593,7 @@ const char* const STEP_NAMES[] = {"step_delta_rule", "step_gated_delta_rule", "s
 Tensor delta_step(int64_t family, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g, const OptTensor& beta, const OptTensor& b,
                   const OptTensor& w, Tensor state, std::optional<double> scale, const OptTensor& slots, bool qk_norm, double beta_scale, const OptTensor& A_log,
                   const OptTensor& dt_bias, bool state_v_first) {
+  WANT(family >= REWY_DELTA && family <= REWY_GDN2, "delta_step: family must be 0 to 3, got ", family);
   const char* op = STEP_NAMES[family];
   WANT(q.dim() == 3 && v.dim() == 3 && q.numel() > 0 && v.numel() > 0, op, ": q, k must have the shape [B, H, K] and v [B, HV, V], got ", shape(q), " and ", shape(v));
   const int64_t B = q.size(0), H = q.size(1), K = q.size(2), HV = v.size(1), V = v.size(2);

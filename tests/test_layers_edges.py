@@ -107,3 +107,15 @@ def test_workspaces_of_refused_sizes_are_none():
         assert lib.rewy_scan_workspace_bytes(B, T, D, 16, 1, 0) == lib.rewy_scan_workspace_bytes(B, T, D, 16, 1, 1) == 0
     assert lib.rewy_scan_checkpoint_bytes(1, 64, 64, 65) == 0
     assert lib.rewy_conv_bwd_workspace_bytes(1 << 16, 1 << 14, 64, 4) > 0 and lib.rewy_scan_workspace_bytes(1 << 16, 1 << 14, 64, 16, 1, 1) > 0
+
+
+@pytest.mark.parametrize("family", (-1, 4, 7, 1 << 40))
+def test_the_step_operator_itself_refuses_an_unknown_family(family):
+    from rewy_b200 import _capi
+    _capi.load_torch()
+    step = torch.ops.rewy_b200.delta_step
+    operands = (z(2, 2, 8), z(2, 2, 8), z(2, 4, 6), z(2, 4, 8), z(2, 4), None, None, z(5, 4, 8, 6), None, None, False, 0.0, None, None, False)
+    with pytest.raises(RuntimeError, match=f"family must be 0 to 3, got {family}"):
+        step(family, *operands)
+    with pytest.raises(RuntimeError, match="step_kda: needs CUDA tensors"):
+        step(_capi.KDA, *operands)
