@@ -73,6 +73,11 @@ template <class Tensors>
 void want_no_tangent(const char* op, const Tensors& tensors) {
   for (const OptTensor& t : tensors) WANT(!has(t) || !t->_fw_grad(0).defined(), op, ": has no forward-mode derivative, and an input carries one");
 }
+// Tensors that only stand for others have no address: an optional one would be taken for one that is not there.
+bool in_memory(const Tensor& t) {
+  const auto* impl = t.unsafeGetTensorImpl();
+  return impl->has_storage() && (t.numel() == 0 || impl->storage().data() != nullptr);
+}
 // one CUDA device for all of them
 void want_cuda(const char* op, std::initializer_list<OptTensor> tensors) {
   want_no_tangent(op, tensors);
@@ -81,6 +86,7 @@ void want_cuda(const char* op, std::initializer_list<OptTensor> tensors) {
     if (!has(t)) continue;
     WANT(t->is_cuda(), op, ": needs CUDA tensors (there is no CPU fallback)");
     WANT(t->layout() == at::kStrided, op, ": needs dense tensors");
+    WANT(in_memory(*t), op, ": needs tensors with memory of their own, not fake ones, wrappers or a transform's");
     if (!device.is_cuda()) device = t->device();
     WANT(t->device() == device, op, ": tensors are on ", device, " and ", t->device());
   }

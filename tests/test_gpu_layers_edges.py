@@ -41,3 +41,24 @@ def test_norms_of_very_small_rows_without_eps(dtype, D, size):
     for scale in (0.5, 0.5 + rn(D)):
         _compare(lambda **x: rewy_b200.residual_rms_norm(**x, eps=0.0), lambda **x: oracle.residual_rms_norm(**x, eps=0.0),
                  dict(x=x, residual=(size * rn(6, D)).to(dtype), weight=weight, scale=scale), (dtype, dtype))
+
+
+def test_an_optional_operand_without_memory_is_refused():
+    """A bias that is a wrapper beside an input that is none: refused, not left out."""
+    from test_layers_edges import Wrapper
+    rn = _gen(32)
+    x, weight = rn(2, 9, 16), rn(16, 4)
+    with pytest.raises(RuntimeError, match="needs tensors with memory of their own"):
+        rewy_b200.causal_conv(x, weight, Wrapper(rn(16)))
+    with pytest.raises(RuntimeError, match="needs tensors with memory of their own"):
+        rewy_b200.causal_conv_step(x[:, 0], rn(5, 3, 16), weight, slots=Wrapper(torch.zeros(2, dtype=torch.int32)))
+
+
+def test_transforms_give_slices_or_raise():
+    """vmap runs an operator slice by slice; grad of torch.func, which wraps its tensors, raises."""
+    rn = _gen(33)
+    x, gate, weight = rn(3, 4, 64), rn(4, 64), rn(64)
+    got = torch.func.vmap(lambda v: rewy_b200.gated_rms_norm(v, gate, weight))(x)
+    assert torch.equal(got, torch.stack([rewy_b200.gated_rms_norm(v, gate, weight) for v in x]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: rewy_b200.gated_rms_norm(v, gate, weight).sum())(x[0])

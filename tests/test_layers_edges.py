@@ -119,3 +119,31 @@ def test_the_step_operator_itself_refuses_an_unknown_family(family):
         step(family, *operands)
     with pytest.raises(RuntimeError, match="step_kda: needs CUDA tensors"):
         step(_capi.KDA, *operands)
+
+
+class Wrapper(torch.Tensor):
+    """A tensor of the GPU by its device, without memory: what distributed and quantised subclasses are."""
+    @staticmethod
+    def __new__(cls, like):
+        return torch.Tensor._make_wrapper_subclass(cls, like.shape, dtype=like.dtype, device="cuda")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} is not asked for")
+
+
+def test_tensors_without_memory_are_refused():
+    """Their address reads as NULL, which an entry takes for an operand that is not there."""
+    x, gate, weight = Wrapper(z(3, 8)), Wrapper(z(3, 8)), Wrapper(z(8))
+    assert x.is_cuda and x.data_ptr() == 0
+    with pytest.raises(RuntimeError, match="needs tensors with memory of their own"):
+        rewy_b200.gated_rms_norm(x, gate, weight)
+    with pytest.raises(RuntimeError, match="needs tensors with memory of their own"):
+        rewy_b200.causal_conv(Wrapper(z(2, 9, 16)), Wrapper(z(16, 4)), Wrapper(z(16)))
+    with pytest.raises(RuntimeError, match="needs tensors with memory of their own"):
+        rewy_b200.step_delta_rule(*(Wrapper(z(2, 4, 8)) for _ in range(3)), Wrapper(z(2, 4)), Wrapper(z(5, 4, 8, 8)))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        fake = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
+        with pytest.raises(RuntimeError, match="needs tensors with memory of their own|Cannot access data pointer"):
+            rewy_b200.residual_rms_norm(fake(3, 8), fake(3, 8), fake(8))
