@@ -11,9 +11,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <algorithm>
+#include <atomic>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 #include "../../include/rewy_b200.h"
 
 namespace {
@@ -146,6 +148,15 @@ bool any_grad(std::initializer_list<OptTensor> tensors) {
   return false;
 }
 
+// Backwards that have been launched, for the dispatch report: autograd runs them without passing through Python.
+enum { CAUSAL_CONV, SELECTIVE_SCAN, GATED_RMS_NORM, RESIDUAL_RMS_NORM, NODES };
+std::atomic<int64_t> backwards[NODES];
+std::vector<int64_t> layer_backwards() {   // since the last call, in the order above
+  std::vector<int64_t> n;
+  for (auto& count : backwards) n.push_back(count.exchange(0));
+  return n;
+}
+
 // The gradients a node gives, tied to its inputs by one that raises: only a backward that is itself recorded needs it.
 variable_list first_order(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -213,6 +224,7 @@ struct Conv : torch::autograd::Function<Conv> {
     a.dx = dx.data_ptr(); a.dweight = dw.data_ptr(); a.dbias = at_ptr<void>(db); a.dinitial_state = at_ptr<void>(di);
     a.workspace = ws.data_ptr(); a.workspace_bytes = ws.nbytes();
     check(rewy_conv_bwd(&a, stream()), "causal_conv backward");
+    backwards[CAUSAL_CONV]++;
     auto g = first_order({dx, dw, db, di});
     return {g[0], g[1], g[2], g[3], Tensor(), Tensor(), Tensor()};
   }
@@ -344,6 +356,7 @@ struct Scan : torch::autograd::Function<Scan> {
     a.dA = at_ptr<float>(dA); a.dD = at_ptr<float>(dD); a.ddt_bias = at_ptr<float>(dbias); a.dinitial_state = at_ptr<float>(di);
     a.workspace = ws.data_ptr(); a.workspace_bytes = ws.nbytes();
     check(rewy_scan_bwd(&a, stream()), "selective_scan backward");
+    backwards[SELECTIVE_SCAN]++;
     auto g = first_order({du, ddt, dA, dB, dC, dD, dz, dbias, di});
     g.resize(12);
     return g;
@@ -513,6 +526,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     a.dy = in(dy); a.dx = dx.data_ptr(); a.dgate = dg.data_ptr(); a.dweight = dw.data_ptr();
     a.workspace = ws.data_ptr(); a.workspace_bytes = ws.nbytes();
     check(rewy_gated_norm_bwd(&a, stream()), "gated_rms_norm backward");
+    backwards[GATED_RMS_NORM]++;
     auto g = first_order({dx, dg, dw});
     g.resize(6);
     return g;
@@ -570,6 +584,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     a.dy = in(dy); a.dresidual_out = in(dro); a.dx = dx.data_ptr(); a.dresidual = at_ptr<void>(dr); a.dweight = dw.data_ptr(); a.dscale = at_ptr<void>(ds);
     a.workspace = ws.data_ptr(); a.workspace_bytes = ws.nbytes();
     check(rewy_residual_norm_bwd(&a, stream()), "residual_rms_norm backward");
+    backwards[RESIDUAL_RMS_NORM]++;
     auto g = first_order({dx, dr, dw, ds});
     g.resize(6);
     return g;
@@ -658,6 +673,7 @@ TORCH_LIBRARY_FRAGMENT(rewy_b200, m) {
   m.def("residual_rms_norm(Tensor x, Tensor? residual, Tensor weight, Tensor? scale_vector, float scale, float eps) -> (Tensor, Tensor)");
   m.def("delta_step(int family, Tensor q, Tensor k, Tensor v, Tensor? g, Tensor? beta, Tensor? b, Tensor? w, Tensor(a!) state, float? scale, Tensor? slots, "
         "bool qk_norm, float beta_scale, Tensor? A_log, Tensor? dt_bias, bool state_v_first) -> Tensor");
+  m.def("layer_backwards() -> int[]", &layer_backwards);
 }
 TORCH_LIBRARY_IMPL(rewy_b200, CompositeImplicitAutograd, m) {
   m.impl("causal_conv", &causal_conv);

@@ -21,7 +21,20 @@ zero and no state changes.
 import torch
 
 from . import _capi
-from .runtime import record
+from .runtime import count_elsewhere, record
+
+
+def _backwards():
+    """Backwards since the last call, which autograd runs without passing through Python (csrc/layers.cpp)."""
+    if not _loaded:
+        return {}
+    counts = torch.ops.rewy_b200.layer_backwards()
+    return {f"{name}.optimized_backward": n for name, n in zip(_TRAINED, counts) if n}
+
+
+_TRAINED = ("causal_conv", "selective_scan", "gated_rms_norm", "residual_rms_norm")   # in the library's order
+_loaded = False
+count_elsewhere(_backwards)
 
 
 def _operator(op, kind=None):
@@ -29,9 +42,11 @@ def _operator(op, kind=None):
     fn, kind = None, kind or op
 
     def call(*args):
+        global _loaded
         nonlocal fn
         if fn is None:
             _capi.load_torch()
+            _loaded = True
             fn = getattr(torch.ops.rewy_b200, op).default
         out = fn(*args)
         record(kind, "optimized_forward")

@@ -35,13 +35,25 @@ class Selection:
 _selection = ContextVar("rewy_b200_selection", default=Selection())
 _counts = Counter()
 _warned = set()
+_elsewhere = []   # functions that hand over what was counted outside Python since their last call, as {"<op>.<event>": n}
 
 
 def record(op, event):
     _counts[f"{op}.{event}"] += 1
 
 
+def count_elsewhere(hand_over):
+    """Have ``hand_over`` asked for its counts whenever they are looked at."""
+    _elsewhere.append(hand_over)
+
+
+def _gather():
+    for hand_over in _elsewhere:
+        _counts.update(hand_over())
+
+
 def stats(reset=False):
+    _gather()
     result = dict(sorted(_counts.items()))
     if reset:
         _counts.clear()
@@ -79,6 +91,7 @@ def dispatch_report():
 
 def assert_used(ops=None, *, backward=True):
     ops = _selection.get().ops if ops is None else ops
+    _gather()
     suffix = "optimized_backward" if backward else "optimized_forward"
     missing = [op for op in ops if not _counts.get(f"{op}.{suffix}", 0)]
     if missing:

@@ -62,3 +62,21 @@ def test_transforms_give_slices_or_raise():
     assert torch.equal(got, torch.stack([rewy_b200.gated_rms_norm(v, gate, weight) for v in x]))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda v: rewy_b200.gated_rms_norm(v, gate, weight).sum())(x[0])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_backwards_are_counted(name):
+    """``assert_used`` as after any training step: both directions; a forward alone does not pass it."""
+    call, xs = _calls(_gen(34))[name]
+    rewy_b200.stats(reset=True)
+    mine = _leaves(xs)
+    out = call(**mine)
+    with pytest.raises(RuntimeError, match="No optimized_backward calls"):
+        rewy_b200.assert_used((name,))
+    for _ in range(2):
+        torch.autograd.grad(out[0].sum(), list(mine.values()), retain_graph=True, allow_unused=True)
+    rewy_b200.assert_used((name,))
+    assert rewy_b200.stats() == {f"{name}.optimized_backward": 2, f"{name}.optimized_forward": 1}
+    assert rewy_b200.stats(reset=True) and rewy_b200.stats() == {}
+    torch.autograd.grad(out[0].sum(), list(mine.values()), allow_unused=True)
+    assert rewy_b200.stats(reset=True) == {f"{name}.optimized_backward": 1}

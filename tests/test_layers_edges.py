@@ -147,3 +147,16 @@ def test_tensors_without_memory_are_refused():
         fake = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
         with pytest.raises(RuntimeError, match="needs tensors with memory of their own|Cannot access data pointer"):
             rewy_b200.residual_rms_norm(fake(3, 8), fake(3, 8), fake(8))
+
+
+def test_counts_kept_elsewhere_join_the_report(monkeypatch):
+    from rewy_b200 import layers, runtime
+    rewy_b200.stats(reset=True)
+    given = [{"causal_conv.optimized_backward": 2}, {}, {"causal_conv.optimized_backward": 1}]
+    monkeypatch.setattr(runtime, "_elsewhere", [lambda: given.pop(0) if given else {}])
+    rewy_b200.assert_used(("causal_conv",))
+    assert rewy_b200.stats() == {"causal_conv.optimized_backward": 2}
+    assert rewy_b200.stats(reset=True) == {"causal_conv.optimized_backward": 3} and rewy_b200.stats() == {}
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        _conv()
+    assert layers._backwards() == {}     # the library is loaded and has nothing to add
