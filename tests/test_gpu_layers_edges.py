@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 import rewy_b200
-from test_gpu_layers import BF16, FP32, NAMES, _calls, _compare, _gen, _leaves, oracle
+from test_gpu_layers import BF16, DEV, FP16, FP32, NAMES, _calls, _close, _compare, _gen, _leaves, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,125 @@ def test_backwards_are_counted(name):
     assert rewy_b200.stats(reset=True) and rewy_b200.stats() == {}
     torch.autograd.grad(out[0].sum(), list(mine.values()), allow_unused=True)
     assert rewy_b200.stats(reset=True) == {f"{name}.optimized_backward": 1}
+
+
+# ---- gradients of views, of single outputs and of long tensors -------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", (BF16, FP16, FP32))
+@pytest.mark.parametrize("shift", (0, 3))
+@pytest.mark.parametrize("T", (60, 700))
+def test_selective_scan_gradients_of_views(dtype, shift, T):
+    """u and z halves of one projection, B and C slices of another (aligned and at an odd offset), a transposed dt; in one segment of
+    tokens and in several."""
+    rn, M = _gen(35), 96 - (shift > 0)
+    xs = dict(wide=rn(2, T, 194).to(dtype), proj=rn(2, T, 48).to(dtype), steps=(0.2 * rn(2, M, T).abs()).to(dtype), A=-rn(M, 16).abs() - 0.05, D=rn(M))
+
+    def apply(scan, wide, proj, steps, A, D):
+        u, z, Bm, C = wide[..., :M], wide[..., 96:96 + M], proj[..., shift:shift + 16], proj[..., 16 + shift:32 + shift]
+        return scan(u, steps.transpose(1, 2), A, Bm, C, D, z)
+
+    _compare(lambda **x: apply(lambda u, dt, A, B, C, D, z: rewy_b200.selective_scan(u, dt, A, B, C, D, z=z, output_final_state=True), **x),
+             lambda **x: apply(lambda u, dt, A, B, C, D, z: oracle.selective_scan(u, dt, A, B[:, :, None], C[:, :, None], D, z), **x), xs, (dtype, FP32))
+
+
+def test_selective_scan_gradients_of_broadcast_inputs():
+    """One B for all groups, one C and one dt for all sequences: their gradients are the sums over what they were spread to."""
+    rn = _gen(36)
+    xs = dict(u=rn(3, 40, 24), dt=0.3 * rn(1, 40, 24).abs(), A=-rn(24, 16).abs() - 0.05, B=rn(3, 40, 1, 16), C=rn(1, 40, 2, 16))
+    spread = lambda u, dt, A, B, C: (u, dt.expand(3, -1, -1), A, B.expand(-1, -1, 2, -1), C.expand(3, -1, -1, -1))  # noqa: E731
+    _compare(lambda **x: rewy_b200.selective_scan(*spread(**x))[:1], lambda **x: oracle.selective_scan(*spread(**x))[:1], xs, (FP32,))
+
+
+VIEWS = {"heads of a slice": (BF16, (3, 50, 776), lambda g: g[..., :768].unflatten(-1, (6, 128))),
+         "at an odd offset": (BF16, (3, 50, 776), lambda g: g[..., 5:773].unflatten(-1, (6, 128))),
+         "transposed batch": (FP16, (50, 3, 6, 128), lambda g: g.transpose(0, 1)),
+         "rows apart": (FP32, (3, 50, 128, 6), lambda g: g.transpose(-1, -2)),
+         "three strides": (BF16, (3, 100, 12, 128), lambda g: g[:, ::2, ::2]),
+         "one for all heads": (FP32, (3, 50, 1, 128), lambda g: g.expand(-1, -1, 6, -1))}
+
+
+@pytest.mark.parametrize("view", VIEWS)
+def test_norm_gradients_of_views(view):
+    rn = _gen(37)
+    dtype, size, of = VIEWS[view]
+    xs = dict(x=rn(3, 50, 6, 128).to(dtype), base=rn(*size).to(dtype), weight=1 + 0.1 * rn(128))
+    for first in (False, True):
+        _compare(lambda x, base, weight: (rewy_b200.gated_rms_norm(x, of(base), weight, gate_first=first),),
+                 lambda x, base, weight: (oracle.gated_rms_norm(x, of(base), weight, gate_first=first),), xs, (dtype,))
+        _compare(lambda x, base, weight: (rewy_b200.gated_rms_norm(of(base), x, weight, gate_first=first),),
+                 lambda x, base, weight: (oracle.gated_rms_norm(of(base), x, weight, gate_first=first),), xs, (dtype,))
+    _compare(lambda x, base, weight: rewy_b200.residual_rms_norm(x, of(base), weight, scale=0.5),
+             lambda x, base, weight: oracle.residual_rms_norm(x, of(base), weight, 0.5), xs, (dtype, dtype))
+    _compare(lambda x, base, weight: rewy_b200.residual_rms_norm(of(base), x, weight, scale=0.5),
+             lambda x, base, weight: oracle.residual_rms_norm(of(base), x, weight, 0.5), xs, (dtype, dtype))
+
+
+@pytest.mark.parametrize("name", ("causal_conv", "selective_scan", "residual_rms_norm"))
+def test_gradients_of_the_last_output_alone(name):
+    """The final state or the residual without the output beside it, whose gradient then never comes."""
+    call, xs = _calls(_gen(38))[name]
+    definition = {"causal_conv": lambda **x: oracle.causal_conv(**x, activation="silu"), "selective_scan": lambda **x: oracle.selective_scan(**x, dt_softplus=True),
+                  "residual_rms_norm": oracle.residual_rms_norm}[name]
+    mine, exact = _leaves(xs), _leaves({n: x.double() for n, x in xs.items()})
+    got, want = call(**mine)[-1], definition(**exact)[-1]
+    seed = _gen(39)(*got.shape)
+    grads = torch.autograd.grad(got, list(mine.values()), seed, allow_unused=True)
+    exacts = torch.autograd.grad(want, list(exact.values()), seed.double(), allow_unused=True)
+    for (n, x), g, e in zip(xs.items(), grads, exacts):
+        _close(torch.zeros_like(x) if g is None else g, torch.zeros_like(x) if e is None else e, n)
+
+
+def test_gradients_beyond_32_bits():
+    """More than 2^31 elements in a tensor: the gradients of its last rows are what they are alone, bit for bit where a row's arithmetic
+    does not depend on the others, and the convolution's weight gradient is that of the definition over all rows."""
+    gen = torch.Generator(device=DEV).manual_seed(40)
+    rn = lambda *s, t=BF16: torch.empty(*s, device=DEV, dtype=t).normal_(generator=gen)  # noqa: E731
+    D, tail = 4096, 9
+    rows = (1 << 31) // D + 100
+    x, dy, weight = rn(1, rows, D), rn(1, rows, D), (rn(D, 4, t=FP32) / 2).requires_grad_()
+
+    def conv(x, dy, state=None):
+        x = x.detach().requires_grad_()
+        y, _ = rewy_b200.causal_conv(x, weight, activation="silu", initial_state=state)
+        return torch.autograd.grad(y, (x, weight), dy)
+
+    dx, dw = conv(x, dy)
+    alone, _ = conv(x[:, -tail:], dy[:, -tail:], x[:, -tail - 3:-tail].contiguous())
+    assert torch.equal(dx[:, -tail:], alone)
+    del dx
+    last = [v[..., -8:].double().detach().requires_grad_() for v in (x, weight.t())]
+    y, _ = oracle.causal_conv(last[0], last[1].t(), activation="silu")
+    _close(dw[-8:], torch.autograd.grad(y, last[1], dy[..., -8:].double())[0].t(), "dweight")
+    del y, last
+    norm = rn(D, t=FP32)
+
+    def gated(x, dy):
+        x, gate = x.detach().requires_grad_(), dy.detach().requires_grad_()
+        return torch.autograd.grad(rewy_b200.gated_rms_norm(x, gate, norm), (x, gate), dy)
+
+    whole = gated(x, dy)
+    for a, b in zip(whole, gated(x[:, -tail:], dy[:, -tail:])):
+        assert torch.equal(a[:, -tail:], b)
+    del whole
+
+    def residual(x, dy):
+        x, r = x.detach().requires_grad_(), dy.detach().requires_grad_()
+        return torch.autograd.grad(rewy_b200.residual_rms_norm(x, r, norm, scale=0.5), (x, r), (dy, x.detach()))
+
+    whole = residual(x, dy)
+    for a, b in zip(whole, residual(x[:, -tail:], dy[:, -tail:])):
+        assert torch.equal(a[:, -tail:], b)
+    del whole
+    M = 256
+    x, dy = x.view(1, -1, M), dy.view(1, -1, M)
+    A, Bm = -torch.rand(M, 16, device=DEV) - 0.5, rn(1, x.shape[1], 16)
+
+    def scan(u, dy, Bm):
+        u, dt, Bm = (v.detach().requires_grad_() for v in (u, u, Bm))
+        y, _ = rewy_b200.selective_scan(u, dt, A, Bm, Bm.detach(), dt_softplus=True)
+        return torch.autograd.grad(y, (u, dt, Bm), dy)
+
+    whole, short = scan(x, dy, Bm), scan(x[:, -2000:], dy[:, -2000:], Bm[:, -2000:])
+    for a, b in zip(whole, short):                          # 1000 tokens forget where they began; both sides are rounded to BF16
+        a, b = a[:, -1000:].double(), b[:, -1000:].double()
+        assert ((a - b).abs() <= 2 ** -7 * 1.01 * b.abs() + 1e-4 * b.square().mean().sqrt()).all()
