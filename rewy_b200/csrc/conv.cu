@@ -82,7 +82,6 @@ struct Columns {  // a warp's channels
     }
   }
   __device__ __forceinline__ void load_x(Pack<T, V>& d, int t) const { load_some<T, V>(d, x + t * a.x_token_stride + c0, valid, wide); }
-  __device__ __forceinline__ long long at(int row, long long rows_before) const { return (rows_before + row) * a.D + c0; }
   // the W-1 inputs before token t of sequence s
   __device__ __forceinline__ void window(F2 (&win)[W - 1][P], const Span& s, int t) const {
 #pragma unroll
@@ -451,7 +450,7 @@ int token_block(long long tokens, int warps_per_token) {
   return block;
 }
 
-ConvParams conv_params(const RewyConvArgs& a, int V, bool rows_wide) {
+ConvParams conv_params(const RewyConvArgs& a, int V) {
   ConvParams p;
   p.a = a;
   const int e = element_bytes(a.dtype), access = V * e;
@@ -459,7 +458,7 @@ ConvParams conv_params(const RewyConvArgs& a, int V, bool rows_wide) {
   p.token_block = token_block((long long)a.B * a.T, (a.D + 127) / 128);
   p.token_blocks = (a.T + p.token_block * WARPS - 1) / (p.token_block * WARPS);
   auto row = [&](const void* q) { return (reinterpret_cast<uintptr_t>(q) % access) == 0; };
-  p.wide = rows_wide && a.D % V == 0 && a.x_token_stride % V == 0 && a.x_batch_stride % V == 0 && row(a.x) && row(a.y) && row(a.dy) && row(a.dx) &&
+  p.wide = a.D % V == 0 && a.x_token_stride % V == 0 && a.x_batch_stride % V == 0 && row(a.x) && row(a.y) && row(a.dy) && row(a.dx) &&
            row(a.initial_state) && row(a.final_state) && row(a.dfinal_state) && row(a.dinitial_state);
   return p;
 }
@@ -482,7 +481,7 @@ extern "C" int rewy_conv_fwd(const RewyConvArgs* a, rewy_stream_t st) {
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = lane_channels<T>(), bytes = Ring<T, V, 1>::BYTES;
-    const ConvParams p = conv_params(*a, V, true);
+    const ConvParams p = conv_params(*a, V);
     const unsigned grid = (unsigned)((long long)p.channel_blocks * p.token_blocks * a->B);
     with_taps(a->W, [&](auto w) {
       auto go = [&](auto wide) {
@@ -500,7 +499,7 @@ extern "C" size_t rewy_conv_bwd_workspace_bytes(int32_t B, int32_t T, int32_t D,
   if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 4 || !conv_fits(B, T, D)) return 0;
   RewyConvArgs a{};
   a.B = B; a.T = T; a.D = D; a.W = W;
-  const ConvParams p = conv_params(a, 4, true);
+  const ConvParams p = conv_params(a, 4);
   return (size_t)p.token_blocks * B * (W + 1) * D * sizeof(float);
 }
 
@@ -515,7 +514,7 @@ extern "C" int rewy_conv_bwd(const RewyConvArgs* a, rewy_stream_t st) {
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = lane_channels<T>(), bytes = Ring<T, V, 2>::BYTES;
-    const ConvParams p = conv_params(*a, V, true);
+    const ConvParams p = conv_params(*a, V);
     parts = p.token_blocks * a->B;
     const unsigned grid = (unsigned)((long long)p.channel_blocks * parts);
     with_taps(a->W, [&](auto w) {
