@@ -82,6 +82,24 @@ def test_backwards_are_counted(name):
     assert rewy_b200.stats(reset=True) == {f"{name}.optimized_backward": 1}
 
 
+def test_decays_over_the_range_of_arguments():
+    """Through a step on a state of ones without input: exp(dt A) for arguments a from -1e-9 to -80.  A log2 e and its constant, the
+    product with dt and the multiply-add each round by 2^-24 of the argument at most, the offset that the multiply-add adds is below
+    2e-8, the exponential is within 2 ulp (2^-22).  Errors of one sign would gather up over a state's memory, token by token: on
+    average they stay below half a step of values under 1, 2^-24, as correctly rounded values' own errors do, plus the argument's."""
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    edges = (1e-9, 1e-8, 1e-7, 1e-6, 1e-5, 1e-4, 1e-3, 5e-3, 0.02, 0.1, 0.5, 1.0, 4.0, 16.0, 64.0)
+    for lo, hi in zip(edges, edges[1:]):
+        M, N, B = 1024, 64, 8
+        A = -(lo * (hi / lo) ** torch.rand(M, N, device=DEV, generator=gen, dtype=torch.float64)).float()
+        dt, state, none = 0.75 + 0.5 * torch.rand(B, M, device=DEV, generator=gen), torch.ones(B, M, N, device=DEV), torch.zeros(B, N, device=DEV)
+        rewy_b200.selective_scan_step(torch.zeros_like(dt), dt, A, none, none, state)
+        a = dt.double()[:, :, None] * A.double()
+        off = state.double() / a.exp() - 1
+        assert (off.abs() <= 2 ** -22 + 2e-8 - a * 4 * 2 ** -24).all(), (lo, off.abs().max().item())
+        assert off.mean().abs() <= 2 ** -24 - (a.mean() * 4 * 2 ** -24), (lo, off.mean().item())
+
+
 # ---- gradients of views, of single outputs and of long tensors -------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", (BF16, FP16, FP32))
