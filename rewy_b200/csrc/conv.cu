@@ -442,8 +442,10 @@ int check_conv(const RewyConvArgs* a) {
 }
 
 // Tokens per warp.  Long blocks load fewer rows twice (W-1 per block) and leave fewer sums; short ones give a small problem
-// enough warps: B=1 T=2000 D=1024 has 8 warps of channels, blocks of 8 make 2000 warps of them.  At B=2 T=4096 D=8192 the backward
-// takes 158 us with blocks of 64 against 175 with 32; 128 is no better and slower forward (76 us against 68).
+// enough warps.  Forward / backward with its sums in us, blocks of 8, 16, 32, 64, 128: B=2 T=4096 D=8192 86 / 239, 66 / 161, 62 / 125,
+// 62 / 109, 70 / 112 (64 taken); 16001 tokens in 12 documents, D=2048 47 / 144, 37 / 98, 35 / 76, 38 / 68, 40 / 63 (64); B=1 T=2000
+// D=1024 5.7 / 13, 6.1 / 12, 9.0 / 15, 15 / 22, 27 / 36 (8); B=8 T=500 D=768 7.0 / 20, 7.7 / 16, 9.1 / 16, 15 / 22, 24 / 29 (8).
+// A sequence of a fixed batch shorter than eight blocks leaves warps of its CTA idle: B=64 T=64 D=2048 takes 13 / 37.
 int token_block(long long tokens, int warps_per_token) {
   int block = 64;
   while (block > 8 && tokens / block * warps_per_token < 148 * 24) block /= 2;

@@ -6,8 +6,8 @@
 //
 // Everything is FP32 between the element types at both ends; nothing is kept in fewer bits in between.
 //
-// Recurrence.  A thread holds S states of one channel, L neighbouring lanes the states of a channel (N <= L S), a group of warps 8
-// to 32 channels, which it takes through a segment of the tokens in tiles of 32.  A second group of four warps works beside it:
+// Recurrence.  A thread holds S states of one channel, L neighbouring lanes the states of a channel (N <= L S), a group of two or four
+// warps 8 to 32 channels, which it takes through a segment of the tokens in tiles of 32.  A second group of four warps works beside it:
 // it puts the next tile's dt and dt u per channel, its B and its C into shared memory as FP32 (softplus and gate once per
 // element, eight elements per thread, loads asked for a tile ahead), and writes what came of the tile before.  One barrier per tile.
 // Arithmetic on two states at a time (FP32 pairs).
@@ -21,14 +21,18 @@
 // the gradient that leaves its first token), and the main pass starts every segment from those before it, joined by
 // h <- exp(A sum dt) h + end.  That doubles the exponentials and pays only where most SMs would idle.
 //
-// Measured, B=2 T=4096 M=4096 N=16 in BF16 with softplus, skip and gate: forward 295 us (the exponentials alone, 16 per clock and
-// SM, take 117, memory 41), backward 1020 us and 47 for the sums of dB and dC (memory 62 and 41).  Both are bound by latency and
-// issue together: 256 CTAs give an SM's schedulers two warps of recurrence each, issue is 50 % active, and what a warp waits for
-// are its own shuffles, exponentials and multiply-adds.  Before: every warp doing everything in turn, 456 and 1875 us; conditions
+// Measured, B=2 T=4096 M=4096 N=16 in BF16 with softplus, skip and gate: forward 294 us (the exponentials alone, 16 per clock and
+// SM, take 117, memory 41), backward 1030 us and 48 for the sums of dB and dC (memory 62 and 41).  Both are bound by latency and
+// issue together: two CTAs fit an SM (the backward's 256 threads take 128 registers each), so a scheduler has two warps of recurrence
+// in the backward and, with eight states to a thread, one in the forward; issue is 47 and 38 % active, and what a warp waits for are
+// its own shuffles, exponentials and multiply-adds.  Before: every warp doing everything in turn, 456 and 1875 us; conditions
 // inside the element loops, 340 and 1052.  Tried and not kept (backward): two states per thread and twice the warps 1758 us; eight
 // tokens in registers, half the code, 1031; registers moved from the second group to the first by setmaxnreg 1010; 64 channels
 // per CTA 994 with its sums, but half the CTAs for narrow layers; two warps in the second group 1131.  (Forward): tiles ahead by
 // asynchronous copies through shared memory 303; two warps in the second group 562.
+// N above 16: CTAs hold 16 (N <= 32) or 8 channels, one CTA fits an SM in the backward (117 and 184 KB of shared memory), and the
+// partial sums of dB and dC grow to 16 and 64 bytes per token and channel.  512 channels, 4000 tokens, forward and backward: N = 16
+// 131 us, N = 32 286, N = 64 638.
 #include <climits>
 #include "layer.cuh"
 
@@ -41,7 +45,10 @@ constexpr float LN2 = 0.6931471805599453f;
 
 // exp(dt A) from dt and A log2 e.  The exponential instruction gives results that are 2 to 3 parts in 10^8 too small on average for
 // arguments between -1 and -0.005, and a state that lives for hundreds of tokens would gather that up: 2.0e-6 of dA for 4096
-// tokens.  2.8e-8 on the argument, in the multiply-add that forms it, leaves 1e-8 either way (a step of zero still gives 1).
+// tokens.  2.8e-8 on the argument, in the multiply-add that forms it, leaves 1e-8 there either way (a step of zero still gives 1),
+// and from -1e-9 on no more than the correctly rounded values next to 1 have themselves: 3.7e-8 at most, between -1e-7 and -1e-8,
+// 1.4e-8 elsewhere.  Beyond -4 it does not count: the argument's own rounding is larger.  Segments are joined with one exponential
+// of a sum, which gathers nothing up and goes without.
 constexpr float EX2_LOW = 2.8e-8f;
 __device__ __forceinline__ float decay_of(float d, float A2) { return ex2(fmaf(d, A2, EX2_LOW)); }
 __device__ __forceinline__ F2 decay_of(F2 d, F2 A2) { return ex2_2(fma2(d, A2, both(EX2_LOW))); }
@@ -327,8 +334,8 @@ struct FwdShared {
 };
 
 // STATE_ONLY: the first pass of a scan in segments (all but the last one).
-// Two groups of four warps: the first runs the recurrence of a tile, the second meanwhile writes what came of the tile before
-// and prepares the tile behind.
+// Two groups of warps (two or four, and four): the first runs the recurrence of a tile, the second meanwhile writes what came of the
+// tile before and prepares the tile behind.
 template <class T, class C, bool STATE_ONLY>
 __global__ void __launch_bounds__(C::THREADS, 2) scan_fwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int CH = C::CH, NP = C::NP, YS = C::YS, L = C::L, S = C::S, P = C::P, TT = C::TT;
@@ -694,7 +701,7 @@ struct BwdShared {
   __device__ static __forceinline__ int place(int tok, int c) { return tok * CH + (c & ~7) + ((c ^ ((c >> 3) + CH / 8 * tok)) & 7); }
 };
 
-// Two groups of four warps, as in the forward: the recurrence of a tile beside what stands around the tiles next to it.
+// Two groups of four warps: the recurrence of a tile beside what stands around the tiles next to it.
 template <class T, class C>
 __global__ void __launch_bounds__(C::THREADS, 2) scan_bwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int CH = C::CH, NP = C::NP, YS = C::YS, L = C::L, S = C::S, P = C::P, TT = C::TT;
@@ -1101,7 +1108,9 @@ void with_shape(int N, F&& f) {
   else if (N <= 32) f(Shape<8, 4, 128, 128, 32>());
   else f(Shape<16, 4, 128, 128, 32>());
 }
-// The forward keeps no 16 tokens of states in registers: more of them to a thread
+// The forward keeps no 16 tokens of states in registers, so that eight of them fit a thread, with half the threads for the same
+// channels.  Eight / four per thread, B=2 T=4096 M=4096 without checkpoints: N = 16 273 / 298 us, N = 32 669 / 680, N = 64 1745 /
+// 1699; 4000 tokens of 512 channels: N = 32 61 / 63, N = 64 152 / 124.  Taken where it gains most.
 template <class F>
 void with_forward_shape(int N, F&& f) {
   if (N > 8 && N <= 16) f(Shape<2, 8, 64, 128, 32>());
@@ -1127,10 +1136,12 @@ Plan make_plan(int B, int T, int M, int N, int G, bool backward) {
   p.blocks = (Mg + CH - 1) / CH;
   p.ctas = (long long)p.blocks * G * B;
   const int tiles = (T + TILE - 1) / TILE;
-  // Two CTAs fit an SM.  Segments cost a first pass (0.6 of the forward, 0.25 of the backward), and a CTA alone on its SM is 1.5
-  // times as fast as one beside another: fewer than three segments do not pay.  As many as fill the GPU once, or twice where
-  // that leaves fewer tokens to each place (64 CTAs: 9 segments instead of 4 measure 442 us against 487 for 16001 tokens of
-  // 2048 channels; 32 CTAs: 9 instead of 13, which take two rounds, 84 us against 94 for 2000 tokens of 1024 channels).
+  // Two CTAs fit an SM (one in the backward with N above 16, where the same counts still measure best: 512 channels, 4000 tokens,
+  // forward and backward, 4 / 9 / 13 segments: N = 32 343 / 284 / 316 us, N = 64 690 / 636 / 670).  Segments cost a first pass (0.6 of
+  // the forward, 0.25 of the backward), and a CTA alone on its SM is 1.5 times as fast as one beside another: fewer than three
+  // segments do not pay.  As many as fill the GPU once, or twice where that leaves fewer tokens to each place (forward: 64 CTAs,
+  // 16001 tokens of 2048 channels, 4 / 9 / 13 segments 451 / 408 / 427 us; 32 CTAs, 2000 tokens of 1024 channels, 6 / 9 / 13 46 / 34 /
+  // 48; 16 CTAs, 16000 tokens of 512 channels, 13 / 18 / 26 147 / 113 / 159).
   const long long once = 2 * 148 / p.ctas, twice = 4 * 148 / p.ctas;
   long long want = 2 * once < 0.95 * twice ? twice : once;
   if (once < 3) want = 1;

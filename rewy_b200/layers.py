@@ -14,7 +14,7 @@ neighbours are copied first).  Every sum is FP32 and every output is rounded onc
 sequences work as in the chunked operators (``cu_seqlens``, batch 1, positive lengths; ``cu_seqlens_cpu`` avoids a copy to the
 host, which a captured call must avoid).  Gradients are first order and reverse mode: forward mode raises.
 
-The steps update ``state`` in place.  With ``slots`` (int32 or int64, one per row) row b works on ``state[slots[b]]`` of a
+The steps update ``state``, which must be contiguous, in place.  With ``slots`` (int32 or int64, one per row) row b works on ``state[slots[b]]`` of a
 pool; a row whose index lies outside the pool (-1: a padded row), or is that of a row before it, is skipped: its output is
 zero and no state changes.
 """
